@@ -12,6 +12,12 @@ _EXPORTS = {
     "MegaMoeSchedulerOptions": ("hyper_multicore_b200.modules.mega_moe", "MegaMoeSchedulerOptions"),
     "MegaGate": ("hyper_multicore_b200.modules.mega_gate", "MegaGate"),
     "MegaMhc": ("hyper_multicore_b200.modules.mega_mhc", "MegaMhc"),
+    "MegaLayerNorm": ("hyper_multicore_b200.modules.mega_norm", "MegaLayerNorm"),
+    "MegaRmsNorm": ("hyper_multicore_b200.modules.mega_norm", "MegaRmsNorm"),
+    "mega_layer_norm": ("hyper_multicore_b200.modules.mega_norm", "mega_layer_norm"),
+    "mega_rms_norm": ("hyper_multicore_b200.modules.mega_norm", "mega_rms_norm"),
+    "MegaCrossEntropy": ("hyper_multicore_b200.modules.mega_cross_entropy", "MegaCrossEntropy"),
+    "mega_cross_entropy": ("hyper_multicore_b200.modules.mega_cross_entropy", "mega_cross_entropy"),
     "hyper_mega_mhc": ("hyper_multicore_b200.modules.mega_mhc", "hyper_mega_mhc"),
 }
 

@@ -30,6 +30,10 @@ HMC_CTRL_SOURCE = 1296
 HMC_CTRL_COUNTS = 1552
 HMC_CLAMP_NONE, HMC_CLAMP_BEFORE_SILU, HMC_CLAMP_AFTER_SILU = 0, 1, 2
 HMC_PROFILE_KINDS = ("grouped_gemm", "mx_gemm", "mx_quant", "ep", "route")
+HMC_DTYPE_BF16, HMC_DTYPE_F16, HMC_DTYPE_F32 = 0, 1, 2
+HMC_DTYPE = {torch.bfloat16: HMC_DTYPE_BF16, torch.float16: HMC_DTYPE_F16, torch.float32: HMC_DTYPE_F32}
+HMC_NORM_MAX_HIDDEN = 1048576
+HMC_REDUCE = {"none": 0, "mean": 1, "sum": 2}
 HMC_MOE_LAYOUT = {"EIO": 0, "EOI": 1}
 HMC_MOE_DISPATCH = {"push": 0, "pull": 1}
 
@@ -411,6 +415,14 @@ SIGNATURES: dict[str, tuple] = {
     "hmc_mega_moe_mxfp8": (_I, [ctypes.POINTER(MegaMoeMxfp8Args), _P]),
     "hmc_mega_moe_mxfp8_grad": (_I, [ctypes.POINTER(MegaMoeMxfp8GradArgs), _P]),
     "hmc_mega_moe_mxfp8_abi_version": (_I, []),
+    "hmc_vocab_loss_state_bytes": (_L, [_L, _L]),
+    "hmc_vocab_loss_workspace_bytes": (_L, [_L, _L]),
+    "hmc_vocab_loss": (_I, [_P, _L, _P, _L, _P, _I, _L, _L, _L, _L, _I, _P, _P, _P, _L, _P, _P]),
+    "hmc_vocab_loss_grad_workspace_bytes": (_L, [_L, _L, _L]),
+    "hmc_vocab_loss_grad": (_I, [_P, _P, _L, _L, _L, _L, _I, _P, _P, _P, _P, _L, _P, _P]),
+    "hmc_row_norm": (_I, [_P, _L, _L, _L, _I, _P, _P, _I, _I, _F, _P, _P, _P, _P]),
+    "hmc_row_norm_grad_workspace_bytes": (_L, [_L, _L]),
+    "hmc_row_norm_grad": (_I, [_P, _L, _P, _L, _L, _L, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P, _L, _P]),
 }
 
 

@@ -1,0 +1,932 @@
+// Cross entropy of hidden states over a vocabulary, without keeping the logits:
+//   l_ij = x_i . w_j,  lse_i = log sum_j exp(l_ij),  loss_i = lse_i - l_i,t(i)
+//   p_ij = exp(l_ij - lse_i)
+//   dx_i = g_i (sum_{j != t(i)} p_ij w_j + (p_i,t(i) - 1) w_t(i))
+//   dw_j = sum_{i: t(i) != j} g_i p_ij x_i + sum_{i: t(i) = j} g_i (p_ij - 1) x_i
+// with g the gradient of the loss of a token. Tokens whose target is ignored are left out before anything is computed: the
+// rows that count are packed, and every kernel takes their number from the device.
+//
+// Forward: one GEMM over 256 x 256 tiles whose epilogue keeps a row's maximum and sum of exponentials per 128 columns, and
+// a kernel that joins those. Gradient: the same GEMM again, its epilogue writes p in BF16 for a piece of the vocabulary,
+// and two GEMMs take the piece to the two gradients. p without the target's entry only: that one is p - 1, which cancels for
+// a token the model is sure of and carries the largest weight for one it is not, so it stays in FP32 (expm1 of -loss) and
+// meets the products in FP32: for dx as the row w_t(i) in the epilogue, for dw as a sum over the tokens of a word made
+// beforehand. The rounding of the other entries to BF16 (2^-9 relative) averages over a sum of many.
+//
+// The GEMM: CTA pairs (tcgen05.mma.cta_group::2, M = N = 256), one TMA producer, one issuer, eight epilogue warps, two
+// accumulators; the layouts of the operands are those of the grouped GEMMs.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "gemm_shared.cuh"
+#include "sm100.cuh"
+
+namespace hmc {
+namespace {
+
+using namespace sm100;
+using gemm::A_TILE_BYTES;
+using gemm::ACC_STAGES;
+using gemm::BK;
+using gemm::CHUNK_BYTES;
+using gemm::EPI_WARPS;
+using gemm::NUM_THREADS;
+using gemm::PIPE_BUDGET_NS;
+using gemm::STORE_STAGE_BYTES;
+using gemm::SWIZZLE_128B;
+using gemm::TMEM_COLS;
+
+constexpr int TILE = 256;       // rows and columns of a pair's tile
+constexpr int HALF = TILE / 2;  // rows of A and columns of B that a CTA loads
+constexpr int STAGE_BYTES = 2 * A_TILE_BYTES;
+constexpr int STAGES = 6;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * STORE_STAGE_BYTES + 1024 + 256;
+constexpr int BAND = 8;  // tile rows that are walked together: 8 x 9 tiles in flight share their operands in L2
+
+enum Product { STATS, PROBS, GRAD_HIDDEN, GRAD_WEIGHT };
+
+struct Params {
+  int m, n, k;         // extents; the one that runs over tokens is the packed rows' number
+  const int* count;    // packed rows
+  const int* labels;   // [rows] target of a packed row, -1: none that exists
+  const float* lse;    // [rows]
+  const float* weights;  // [rows] gradient of a packed row's loss, up to `scale`
+  const float* scale;
+  const float* coef;   // [rows] weight * (p_target - 1)
+  float2* partial;     // STATS: [2 * n_tiles][pitch] maximum and sum
+  long long pitch;
+  float* target_logit;  // STATS
+  int first_word;       // PROBS, GRAD_*: first word of the piece
+  const int* row_of;    // GRAD_HIDDEN: token of a packed row
+  float* sums;          // GRAD_HIDDEN: [rows, n] FP32 sums over pieces, or NULL
+  int add, last;        // GRAD_HIDDEN: sums holds earlier pieces; this piece is the last
+  const __nv_bfloat16* head;  // GRAD_HIDDEN: the whole weight
+  long long head_stride;
+  __nv_bfloat16* out;         // GRAD_HIDDEN
+  const int* slots;           // GRAD_WEIGHT: [vocab] row of word_sums, or -1
+  const float* word_sums;     // GRAD_WEIGHT: [rows, n]
+  int* status;
+};
+
+// Tiles in bands of BAND tile rows, a band's columns one after the other.
+struct Walker {
+  int mt, nt;
+  __device__ Walker(int m, int n) : mt((m + TILE - 1) / TILE), nt((n + TILE - 1) / TILE) {}
+  __device__ bool get(long long idx, int& mi, int& ni) const {
+    if (idx >= static_cast<long long>(mt) * nt) return false;
+    const long long per_band = static_cast<long long>(BAND) * nt;
+    const int band = static_cast<int>(idx / per_band);
+    const int local = static_cast<int>(idx - band * per_band);
+    const int high = min(BAND, mt - band * BAND);
+    mi = band * BAND + local % high;
+    ni = local / high;
+    return true;
+  }
+};
+
+__device__ __forceinline__ float shifted_exp(float v, float top) { return __expf(v - top); }
+
+// Maximum and sum of exponentials of one row's 128 columns; the target's logit where it lies among them.
+__device__ __forceinline__ void epilogue_stats(const Params& p, uint32_t taddr, int row, bool row_ok, int col, int half_tile) {
+  const int label = row_ok ? p.labels[row] : -1;
+  float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < HALF; c += 32) {
+    if (col + c >= p.n) break;
+    __syncwarp();
+    uint32_t raw[32];
+    tmem_ld_32x32(taddr + c, raw);
+    tmem_ld_wait();
+    float high = top;
+    if (col + c + 32 > p.n) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col + c + j >= p.n) raw[j] = __float_as_uint(-INFINITY);
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) high = fmaxf(high, __uint_as_float(raw[j]));
+    const float shift = high == -INFINITY ? 0.0f : high;  // nothing but -inf so far: exp(-inf - 0), not exp(-inf + inf)
+    float add = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) add += shifted_exp(__uint_as_float(raw[j]), shift);
+    sum = sum * shifted_exp(top, shift) + add;
+    top = high;
+    const int at = label - (col + c);
+    if (at >= 0 && at < 32) {
+      float own = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j == at) own = __uint_as_float(raw[j]);
+      p.target_logit[row] = own;
+    }
+  }
+  if (row_ok) p.partial[half_tile * p.pitch + row] = make_float2(top, sum);
+}
+
+// 32 x 32 values leave as one BF16 box through shared memory; two boxes per warp in flight.
+__device__ __forceinline__ void store_box(const CUtensorMap* tm, uint8_t* stage, unsigned& issued, const float (&v)[32], int col,
+                                          int row, int lane) {
+  uint8_t* box = stage + (issued & 1) * (STORE_STAGE_BYTES / 2);
+  if (issued > 1) {
+    if (lane == 0) bulk_wait_read_but_one();
+    __syncwarp();
+  }
+  uint8_t* base = box + lane * 64;  // 64-byte rows under the 64-byte swizzle
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<uint4*>(base + ((q ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                   pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(tm, box, col, row);
+    bulk_commit_group();
+  }
+  ++issued;
+}
+
+// p of one row's 128 columns times the row's gradient, the target's entry left out.
+__device__ __forceinline__ void epilogue_probs(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
+                                               unsigned& issued, int first_row, int row, bool row_ok, int col, int lane) {
+  const float lse = row_ok ? p.lse[row] : 0.0f;
+  const float weight = row_ok ? p.weights[row] : 0.0f;
+  const int label = row_ok ? p.labels[row] - p.first_word : -1;
+#pragma unroll 1
+  for (int c = 0; c < HALF; c += 32) {
+    if (col + c >= p.n) break;
+    __syncwarp();
+    uint32_t raw[32];
+    tmem_ld_32x32(taddr + c, raw);
+    tmem_ld_wait();
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      v[j] = row_ok && col + c + j != label ? shifted_exp(__uint_as_float(raw[j]), lse) * weight : 0.0f;
+    store_box(tm, stage, issued, v, col + c, first_row, lane);
+  }
+}
+
+__device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t taddr, int row, bool row_ok, int col) {
+  const float scale = *p.scale;
+  const float coef = row_ok ? p.coef[row] : 0.0f;
+  const int label = row_ok ? p.labels[row] : -1;
+  const long long token = row_ok ? p.row_of[row] : 0;
+  float* sums = p.sums + static_cast<long long>(row) * p.n + col;
+  const __nv_bfloat16* word = p.head + (label >= 0 ? label : 0) * p.head_stride + col;
+  __nv_bfloat16* dst = p.out + token * p.n + col;
+#pragma unroll 1
+  for (int c = 0; c < HALF; c += 32) {
+    if (col + c >= p.n) break;
+    __syncwarp();
+    uint32_t raw[32];
+    tmem_ld_32x32(taddr + c, raw);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      if (!row_ok || col + c + j >= p.n) continue;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(raw[j + e]);
+      if (p.add) {
+        const float4 a = *reinterpret_cast<const float4*>(sums + c + j), b = *reinterpret_cast<const float4*>(sums + c + j + 4);
+        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+      }
+      if (!p.last) {
+        *reinterpret_cast<float4*>(sums + c + j) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(sums + c + j + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        continue;
+      }
+      if (label >= 0) {
+        const uint4 w = ld_16(word + c + j);
+        const uint32_t parts[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack_bf16x2(parts[e]);
+          v[2 * e] += coef * f.x;
+          v[2 * e + 1] += coef * f.y;
+        }
+      }
+      st_16(dst + c + j, make_uint4(pack_bf16x2(v[0] * scale, v[1] * scale), pack_bf16x2(v[2] * scale, v[3] * scale),
+                                    pack_bf16x2(v[4] * scale, v[5] * scale), pack_bf16x2(v[6] * scale, v[7] * scale)));
+    }
+  }
+}
+
+__device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
+                                                     unsigned& issued, int first_row, int row, bool row_ok, int col, int lane,
+                                                     bool empty) {
+  const float scale = *p.scale;
+  const int slot = row_ok ? p.slots[p.first_word + row] : -1;
+  const float* more = p.word_sums + static_cast<long long>(slot >= 0 ? slot : 0) * p.n + col;
+#pragma unroll 1
+  for (int c = 0; c < HALF; c += 32) {
+    if (col + c >= p.n) break;
+    __syncwarp();
+    float v[32];
+    if (empty) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+    } else {
+      uint32_t raw[32];
+      tmem_ld_32x32(taddr + c, raw);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+      if (slot >= 0) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          if (col + c + j < p.n) {
+            const float4 a = *reinterpret_cast<const float4*>(more + c + j);
+            v[j] += a.x, v[j + 1] += a.y, v[j + 2] += a.z, v[j + 3] += a.w;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= scale;
+    }
+    store_box(tm, stage, issued, v, col + c, first_row, lane);
+  }
+}
+
+template <Product KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                 const __grid_constant__ CUtensorMap tm_c, Params p) {
+  constexpr int A_MAJOR = KIND == GRAD_WEIGHT ? HMC_MAJOR_MN : HMC_MAJOR_K;
+  constexpr int B_MAJOR = KIND == GRAD_WEIGHT || KIND == GRAD_HIDDEN ? HMC_MAJOR_MN : HMC_MAJOR_K;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* store_stage = smem + STAGES * STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(store_stage + EPI_WARPS * STORE_STAGE_BYTES);
+  uint64_t* full_bar = bars;                               // leader only: the loads of both CTAs
+  uint64_t* empty_bar = bars + STAGES;                     // one set per CTA
+  uint64_t* acc_full_bar = bars + 2 * STAGES;              // one set per CTA
+  uint64_t* acc_empty_bar = acc_full_bar + ACC_STAGES;     // leader only
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty_bar + ACC_STAGES);
+  volatile int* abort_word = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();  // 0 = leader
+  const long long pair = blockIdx.x >> 1;
+  const long long pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int s = 0; s < ACC_STAGES; ++s) {
+      mbar_init(&acc_full_bar[s], 1);
+      mbar_init(&acc_empty_bar[s], 2 * EPI_WARPS);  // every epilogue warp of both CTAs
+    }
+    *abort_word = 0;
+    mbar_fence_init();
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA signal
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int count = *p.count;
+  if (KIND == GRAD_WEIGHT) p.k = count;
+  else p.m = count;
+  const int kiters = (p.k + BK - 1) / BK;
+  const Walker walker(p.m, p.n);
+  int mi, ni;
+
+  if (warp == 0) {
+    // ======================================================================== TMA producer (both CTAs)
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (long long idx = pair; ok && walker.get(idx, mi, ni); idx += pairs) {
+        const int m0 = mi * TILE + static_cast<int>(rank) * HALF;
+        const int n0 = ni * TILE + static_cast<int>(rank) * HALF;
+        for (int kb = 0; kb < kiters; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
+            report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 0, stage, kb);
+            ok = false;
+            break;
+          }
+          uint8_t* a_dst = smem + stage * STAGE_BYTES;
+          uint8_t* b_dst = a_dst + A_TILE_BYTES;
+          // the leader's barrier counts the bytes of both CTAs
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+          if (A_MAJOR == HMC_MAJOR_K) {
+            tma_load_2d_pair(a_dst, &tm_a, &full_bar[stage], kb * BK, m0);
+          } else {
+            tma_load_2d_pair(a_dst, &tm_a, &full_bar[stage], m0, kb * BK);
+            tma_load_2d_pair(a_dst + CHUNK_BYTES, &tm_a, &full_bar[stage], m0 + 64, kb * BK);
+          }
+          if (B_MAJOR == HMC_MAJOR_K) {
+            tma_load_2d_pair(b_dst, &tm_b, &full_bar[stage], kb * BK, n0);
+          } else {
+            tma_load_2d_pair(b_dst, &tm_b, &full_bar[stage], n0, kb * BK);
+            tma_load_2d_pair(b_dst + CHUNK_BYTES, &tm_b, &full_bar[stage], n0 + 64, kb * BK);
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ======================================================================== MMA issuer (leader only)
+    if (rank == 0 && kiters > 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      constexpr uint32_t idesc = make_idesc_f32acc(1u, TILE, TILE, A_MAJOR, B_MAJOR);
+      constexpr uint32_t A_LBO = A_MAJOR == HMC_MAJOR_MN ? CHUNK_BYTES : 16;
+      constexpr uint32_t B_LBO = B_MAJOR == HMC_MAJOR_MN ? CHUNK_BYTES : 16;
+      constexpr uint32_t A_KSTEP = A_MAJOR == HMC_MAJOR_MN ? (16 * 128) >> 4 : 32 >> 4;
+      constexpr uint32_t B_KSTEP = B_MAJOR == HMC_MAJOR_MN ? (16 * 128) >> 4 : 32 >> 4;
+      for (long long idx = pair; ok && walker.get(idx, mi, ni); idx += pairs) {
+        if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
+          if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 1, acc, 0);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * TILE);
+        for (int kb = 0; kb < kiters; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_word, PIPE_BUDGET_NS)) {
+            if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 2, stage, kb);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          if (lane == 0) {
+            uint8_t* a_src = smem + stage * STAGE_BYTES;
+            uint64_t da = make_smem_desc(smem_u32(a_src), A_LBO, 1024, SWIZZLE_128B);
+            uint64_t db = make_smem_desc(smem_u32(a_src + A_TILE_BYTES), B_LBO, 1024, SWIZZLE_128B);
+#pragma unroll
+            for (int ks = 0; ks < BK / 16; ++ks) {
+              umma_bf16_pair(tmem_d, da, db, idesc, (kb > 0 || ks > 0) ? 1u : 0u);
+              da += A_KSTEP;
+              db += B_KSTEP;
+            }
+            umma_commit_pair(&empty_bar[stage]);  // frees the slot in both CTAs
+            if (kb == kiters - 1) umma_commit_pair(&acc_full_bar[acc]);
+          }
+          __syncwarp();
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (++acc == ACC_STAGES) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+    }
+  } else {
+    // ======================================================================== epilogue (both CTAs)
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    const int quarter = warp & 3;      // TMEM lane quarter this warp may read
+    const int half = (warp - 2) >> 2;  // which half of the tile's columns this warp handles
+    uint8_t* my_stage = store_stage + (warp - 2) * STORE_STAGE_BYTES;
+    unsigned issued = 0;
+    const uint32_t leader_acc_empty = map_to_cta(smem_u32(acc_empty_bar), 0);
+    for (long long idx = pair; ok && walker.get(idx, mi, ni); idx += pairs) {
+      const int first_row = mi * TILE + static_cast<int>(rank) * HALF + quarter * 32;
+      const int row = first_row + lane;
+      const bool row_ok = row < p.m;
+      const int col = ni * TILE + half * HALF;
+      if (kiters == 0) {  // no token counts: the weight's gradient is zero
+        if (KIND == GRAD_WEIGHT) epilogue_grad_weight(p, &tm_c, 0, my_stage, issued, first_row, row, row_ok, col, lane, true);
+        continue;
+      }
+      if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_word, PIPE_BUDGET_NS)) {
+        if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 3, acc, 0);
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * TILE + half * HALF);
+      if (KIND == STATS) epilogue_stats(p, taddr, row, row_ok, col, 2 * ni + half);
+      if (KIND == PROBS) epilogue_probs(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane);
+      if (KIND == GRAD_HIDDEN) epilogue_grad_hidden(p, taddr, row, row_ok, col);
+      if (KIND == GRAD_WEIGHT)
+        epilogue_grad_weight(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane, false);
+      tc_fence_before_sync();
+      __syncwarp();
+      // the MMA issuer lives in the leader: signal its barrier from either CTA
+      if (lane == 0) mbar_arrive_cluster(leader_acc_empty + static_cast<uint32_t>(acc) * 8u);
+      if (++acc == ACC_STAGES) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    if (issued > 0 && lane == 0) bulk_wait_all();  // this thread's stores are in global memory
+  }
+
+  // Teardown: no CTA may leave while its partner can still reach into its shared memory or TMEM.
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- packing
+constexpr int PACK_TOKENS = 32;  // tokens per block
+constexpr int PACK_THREADS = 256;
+
+struct Targets {
+  const void* data;
+  int wide;  // INT64
+  long long ignored, vocab;
+  __device__ long long at(long long i) const {
+    return wide ? static_cast<const long long*>(data)[i] : static_cast<const int*>(data)[i];
+  }
+};
+
+__device__ __forceinline__ int block_count(int v) {  // sum over the block, in every thread
+  __shared__ int slots[PACK_THREADS / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < PACK_THREADS / 32; ++w) v += slots[w];
+  __syncthreads();
+  return v;
+}
+
+// The tokens that count, in their order, as rows without gaps. A block finds its place by counting the targets before
+// its own; the last one writes the number of rows and clears the rows up to the next k-block of a contraction over them.
+__global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bfloat16* __restrict__ x, long long x_stride,
+                                                                 Targets targets, long long tokens, int hidden, int vector,
+                                                                 int* __restrict__ count, int* __restrict__ position,
+                                                                 int* __restrict__ row_of, int* __restrict__ labels,
+                                                                 __nv_bfloat16* __restrict__ packed,
+                                                                 float* __restrict__ token_loss) {
+  __shared__ int place[PACK_TOKENS];
+  const long long first = static_cast<long long>(blockIdx.x) * PACK_TOKENS;
+  int before = 0;
+  for (long long i = threadIdx.x; i < first; i += PACK_THREADS) before += targets.at(i) != targets.ignored;
+  before = block_count(before);
+  if (threadIdx.x < 32) {
+    const long long i = first + threadIdx.x;
+    const long long target = i < tokens ? targets.at(i) : targets.ignored;
+    const bool counts = i < tokens && target != targets.ignored;
+    const unsigned mask = __ballot_sync(0xffffffffu, counts);
+    const int at = before + __popc(mask & ((1u << threadIdx.x) - 1u));
+    place[threadIdx.x] = counts ? at : -1;
+    if (i < tokens) position[i] = counts ? at : -1;
+    if (counts) {
+      row_of[at] = static_cast<int>(i);
+      labels[at] = target >= 0 && target < targets.vocab ? static_cast<int>(target) : -1;
+    } else if (i < tokens && token_loss != nullptr) {
+      token_loss[i] = 0.0f;
+    }
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int t = warp; t < PACK_TOKENS; t += PACK_THREADS / 32) {
+    if (place[t] < 0) continue;
+    const __nv_bfloat16* src = x + (first + t) * x_stride;
+    __nv_bfloat16* dst = packed + static_cast<long long>(place[t]) * hidden;
+    if (vector) {
+      for (int c = lane * 8; c < hidden; c += 256) st_16(dst + c, ld_16(src + c));
+    } else {
+      for (int c = lane; c < hidden; c += 32) dst[c] = src[c];
+    }
+  }
+  if (blockIdx.x != gridDim.x - 1) return;
+  int rows = 0;
+  for (int t = 0; t < PACK_TOKENS; ++t) rows += place[t] >= 0;
+  rows += before;
+  if (threadIdx.x == 0) *count = rows;
+  const long long end = min(tokens, static_cast<long long>((rows + BK - 1) / BK) * BK);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (long long c = rows * static_cast<long long>(hidden) + threadIdx.x * 8; c < end * hidden; c += PACK_THREADS * 8)
+    st_16(packed + c, zero);
+}
+
+// ------------------------------------------------------------------------------------------- joining
+constexpr int JOIN_SLICES = 32;
+
+// Maximum and sum of a packed row from its parts, 32 rows per block: every slice its share of the parts in their order,
+// then the slices in theirs.
+__global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __restrict__ partial, long long pitch, int parts,
+                                                                const int* __restrict__ count,
+                                                                const int* __restrict__ labels,
+                                                                const int* __restrict__ row_of,
+                                                                const float* __restrict__ target_logit,
+                                                                float* __restrict__ lse, float* __restrict__ losses,
+                                                                float* __restrict__ token_loss) {
+  __shared__ float2 sums[JOIN_SLICES][33];
+  const int row = blockIdx.x * 32 + threadIdx.x;
+  const bool ok = row < *count;
+  float top = -INFINITY, sum = 0.0f;
+  if (ok) {
+    // without a branch per part, so that several loads are in flight
+    for (int i = threadIdx.y; i < parts; i += JOIN_SLICES) {
+      const float2 part = partial[i * pitch + row];
+      const float high = fmaxf(top, part.x), shift = high == -INFINITY ? 0.0f : high;
+      sum = sum * shifted_exp(top, shift) + part.y * shifted_exp(part.x, shift);
+      top = high;
+    }
+  }
+  sums[threadIdx.y][threadIdx.x] = make_float2(top, sum);
+  __syncthreads();
+  if (threadIdx.y != 0 || !ok) return;
+  for (int s = 1; s < JOIN_SLICES; ++s) top = fmaxf(top, sums[s][threadIdx.x].x);
+  const float shift = top == -INFINITY ? 0.0f : top;
+  sum = 0.0f;
+  for (int s = 0; s < JOIN_SLICES; ++s) sum += sums[s][threadIdx.x].y * shifted_exp(sums[s][threadIdx.x].x, shift);
+  const float log_sum = logf(sum);
+  // a target outside the vocabulary has no loss: NaN, which no later sum hides
+  const float loss = labels[row] >= 0 ? log_sum + (shift - target_logit[row]) : __int_as_float(0x7fffffff);
+  lse[row] = shift + log_sum;
+  losses[row] = loss;
+  if (token_loss != nullptr) token_loss[row_of[row]] = loss;
+}
+
+// Sum (or mean) of the packed rows' losses by one block, in a fixed order.
+__global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ losses, const int* __restrict__ count, int mean,
+                                                      float* __restrict__ loss) {
+  __shared__ float slots[32];
+  const int rows = *count;
+  float v = 0.0f;
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) v += losses[i];
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  v = warp_sum(slots[threadIdx.x]);
+  if (threadIdx.x == 0) *loss = mean ? v / static_cast<float>(rows) : v;  // no row: the mean is NaN
+}
+
+// ------------------------------------------------------------------------------------------- gradient
+// Per packed row the gradient of its loss (up to a common scale, which stays out of the BF16 products) and the weight of
+// its target's row; per word the first row that has it as target and the number of them.
+__global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict__ grad, int reduction,
+                                                        const int* __restrict__ count, const int* __restrict__ labels,
+                                                        const int* __restrict__ row_of, const float* __restrict__ losses,
+                                                        float* __restrict__ weights, float* __restrict__ coef,
+                                                        float* __restrict__ scale, unsigned* __restrict__ slots,
+                                                        int* __restrict__ members) {
+  const int rows = *count;
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i == 0) {
+    float s = 1.0f;
+    if (reduction == HMC_REDUCE_SUM) s = grad[0];
+    if (reduction == HMC_REDUCE_MEAN) s = rows > 0 ? grad[0] / static_cast<float>(rows) : 0.0f;
+    *scale = s;
+  }
+  if (i >= rows) return;
+  const int label = labels[i];
+  float w = reduction == HMC_REDUCE_NONE ? grad[row_of[i]] : 1.0f;
+  if (label < 0) w = __int_as_float(0x7fffffff);
+  weights[i] = w;
+  coef[i] = label >= 0 ? w * expm1f(-losses[i]) : 0.0f;  // w (p_target - 1)
+  if (slots != nullptr && label >= 0) {
+    atomicMin(&slots[label], static_cast<unsigned>(i));  // the smallest row, whatever the order of arrival
+    atomicAdd(&members[label], 1);                       // from -1
+  }
+}
+
+// word_sums[first row of a word] = sum of coef_i x_i over the rows with that word as target, in their order. A block per row and
+// 1024 columns; rows that are not the first of their word have nothing to do.
+constexpr int WORD_THREADS = 128;
+__global__ void __launch_bounds__(WORD_THREADS) word_sums_kernel(const __nv_bfloat16* __restrict__ packed, int hidden,
+                                                                 const int* __restrict__ count,
+                                                                 const int* __restrict__ labels,
+                                                                 const float* __restrict__ coef,
+                                                                 const unsigned* __restrict__ slots,
+                                                                 const int* __restrict__ members,
+                                                                 float* __restrict__ word_sums) {
+  __shared__ int found[WORD_THREADS];
+  __shared__ int warp_found[WORD_THREADS / 32];
+  const int rows = *count;
+  const int row = blockIdx.x;
+  if (row >= rows) return;
+  const int label = labels[row];
+  if (label < 0 || slots[label] != static_cast<unsigned>(row)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = (blockIdx.y * WORD_THREADS + threadIdx.x) * 8;
+  const bool col_ok = col < hidden;
+  float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  int left = members[label] + 1;
+  for (int base = row; left > 0 && base < rows; base += WORD_THREADS) {
+    const int at = base + threadIdx.x;
+    const bool match = at < rows && labels[at] == label;
+    const unsigned mask = __ballot_sync(0xffffffffu, match);
+    if (lane == 0) warp_found[warp] = __popc(mask);
+    __syncthreads();
+    int place = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < WORD_THREADS / 32; ++w) {
+      if (w < warp) place += warp_found[w];
+      total += warp_found[w];
+    }
+    if (match) found[place + __popc(mask & ((1u << lane) - 1u))] = at;
+    __syncthreads();
+    if (col_ok) {
+#pragma unroll 4
+      for (int i = 0; i < total; ++i) {
+        const int from = found[i];
+        const float c = coef[from];
+        const uint4 q = ld_16(packed + static_cast<long long>(from) * hidden + col);
+        const uint32_t parts[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack_bf16x2(parts[e]);
+          sum[2 * e] += c * f.x;
+          sum[2 * e + 1] += c * f.y;
+        }
+      }
+    }
+    left -= total;
+    __syncthreads();
+  }
+  if (!col_ok) return;
+  float* dst = word_sums + static_cast<long long>(row) * hidden + col;
+  *reinterpret_cast<float4*>(dst) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+  *reinterpret_cast<float4*>(dst + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+}
+
+__global__ void __launch_bounds__(128) zero_ignored_kernel(const int* __restrict__ position, int hidden,
+                                                           __nv_bfloat16* __restrict__ grad_hidden) {
+  const long long token = blockIdx.x;
+  if (position[token] >= 0) return;
+  for (int c = threadIdx.x * 8; c < hidden; c += 128 * 8) st_16(grad_hidden + token * hidden + c, make_uint4(0, 0, 0, 0));
+}
+
+// ------------------------------------------------------------------------------------------- host
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = []() -> EncodeTiledFn {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &found) == cudaSuccess &&
+        found == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(sym);
+    return nullptr;
+  }();
+  return fn;
+}
+
+// [rows, width] BF16 matrix with rows `pitch` elements apart, in boxes of box_width x box_rows.
+int make_map(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch, int box_width, int box_rows,
+             CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  HMC_REQUIRE(fn != nullptr, HMC_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * 2};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_width), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t step[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  HMC_REQUIRE(r == CUDA_SUCCESS, HMC_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return 0;
+}
+int map_k_major(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch) {
+  return make_map(map, base, width, rows, pitch, BK, HALF, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int map_mn_major(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch) {
+  return make_map(map, base, width, rows, pitch, 64, BK, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int map_store(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch) {
+  return make_map(map, base, width, rows, pitch, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+long long tiles_of(long long v) { return (v + TILE - 1) / TILE; }
+
+template <Product KIND>
+int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const Params& p, long long tiles,
+                   cudaStream_t stream) {
+  static PerDeviceFlag configured{};
+  if (int rc = allow_dynamic_smem(head_gemm_kernel<KIND>, SMEM_BYTES, configured)) return rc;
+  const long long most = sm_count() / 2;
+  const int grid = static_cast<int>(2 * (tiles < most ? tiles : most));
+  head_gemm_kernel<KIND><<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(a, b, c, p);
+  HMC_LAUNCH_OK();
+  return 0;
+}
+
+long long up256(long long bytes) { return (bytes + 255) / 256 * 256; }
+
+// What a forward leaves for its gradient, in one buffer of the caller.
+struct State {
+  int *count, *position, *row_of, *labels;
+  float *lse, *losses;
+  __nv_bfloat16* packed;
+  long long bytes;
+  State(void* base, long long tokens, long long hidden) {
+    char* p = static_cast<char*>(base);
+    const long long words = up256(4 * tokens);
+    count = reinterpret_cast<int*>(p);
+    position = reinterpret_cast<int*>(p + 256);
+    row_of = reinterpret_cast<int*>(p + 256 + words);
+    labels = reinterpret_cast<int*>(p + 256 + 2 * words);
+    lse = reinterpret_cast<float*>(p + 256 + 3 * words);
+    losses = reinterpret_cast<float*>(p + 256 + 4 * words);
+    packed = reinterpret_cast<__nv_bfloat16*>(p + 256 + 5 * words);
+    bytes = 256 + 5 * words + 2 * tokens * hidden;
+  }
+};
+
+// A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size.
+constexpr long long PIECE_BYTES = 512ll << 20;
+long long piece_words(long long tokens, long long vocab) {
+  long long most = PIECE_BYTES / (2 * tokens) / TILE * TILE;
+  if (most < 4096) most = 4096;
+  const long long pieces = (vocab + most - 1) / most;
+  return tiles_of((vocab + pieces - 1) / pieces) * TILE;
+}
+
+struct GradSpace {
+  float *scale, *weights, *coef, *word_sums, *sums;
+  unsigned* slots;
+  int* members;
+  __nv_bfloat16* probs;
+  long long slot_bytes, bytes, piece;
+  GradSpace(void* base, long long tokens, long long hidden, long long vocab) {
+    piece = piece_words(tokens, vocab);
+    long long at = 0;
+    auto take = [&](long long size) {
+      char* p = static_cast<char*>(base) + at;
+      at += up256(size);
+      return p;
+    };
+    scale = reinterpret_cast<float*>(take(4));
+    weights = reinterpret_cast<float*>(take(4 * tokens));
+    coef = reinterpret_cast<float*>(take(4 * tokens));
+    slots = reinterpret_cast<unsigned*>(take(4 * vocab));
+    members = reinterpret_cast<int*>(take(4 * vocab));
+    slot_bytes = reinterpret_cast<char*>(members) - reinterpret_cast<char*>(slots) + 4 * vocab;
+    word_sums = reinterpret_cast<float*>(take(4 * tokens * hidden));
+    sums = piece < vocab ? reinterpret_cast<float*>(take(4 * tokens * hidden)) : nullptr;
+    probs = reinterpret_cast<__nv_bfloat16*>(take(2 * tokens * piece));
+    bytes = at;
+  }
+};
+
+int check_sizes(const char* name, int64_t tokens, int64_t hidden, int64_t vocab, int64_t weight_stride, const void* weight,
+                int reduction) {
+  HMC_REQUIRE(tokens > 0 && tokens < (1ll << 31) - TILE, HMC_ERR_INVALID, "%s: tokens (%lld) must be positive and below 2^31",
+              name, (long long)tokens);
+  HMC_REQUIRE(vocab > 0 && vocab < (1ll << 31) - TILE, HMC_ERR_INVALID, "%s: vocab (%lld) must be positive and below 2^31", name,
+              (long long)vocab);
+  HMC_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden < (1ll << 30), HMC_ERR_INVALID,
+              "%s: hidden (%lld) must be a positive multiple of 8", name, (long long)hidden);
+  HMC_REQUIRE(weight != nullptr && aligned16(weight) && weight_stride >= hidden && weight_stride % 8 == 0, HMC_ERR_INVALID,
+              "%s: weight rows must start on 16-byte boundaries, at least hidden apart", name);
+  HMC_REQUIRE(reduction >= HMC_REDUCE_NONE && reduction <= HMC_REDUCE_SUM, HMC_ERR_INVALID, "%s: unknown reduction %d", name,
+              reduction);
+  return 0;
+}
+
+}  // namespace
+}  // namespace hmc
+
+extern "C" int64_t hmc_vocab_loss_state_bytes(int64_t tokens, int64_t hidden) {
+  return tokens > 0 && hidden > 0 ? hmc::State(nullptr, tokens, hidden).bytes : 0;
+}
+
+extern "C" int64_t hmc_vocab_loss_workspace_bytes(int64_t tokens, int64_t vocab) {
+  using namespace hmc;
+  return tokens > 0 && vocab > 0 ? up256(4 * tokens) + 2 * tiles_of(vocab) * tokens * 8 : 0;
+}
+
+extern "C" int64_t hmc_vocab_loss_grad_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab) {
+  return tokens > 0 && hidden > 0 && vocab > 0 ? hmc::GradSpace(nullptr, tokens, hidden, vocab).bytes : 0;
+}
+
+extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* targets,
+                              int targets_i64, int64_t tokens, int64_t hidden, int64_t vocab, int64_t ignore_index, int reduction,
+                              void* state, float* loss, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  using namespace hmc;
+  if (int rc = check_sizes("hmc_vocab_loss", tokens, hidden, vocab, weight_stride, weight, reduction)) return rc;
+  HMC_REQUIRE(x != nullptr && targets != nullptr && state != nullptr && loss != nullptr && x_stride >= 0, HMC_ERR_INVALID,
+              "hmc_vocab_loss: null tensor pointer or negative row stride");
+  HMC_REQUIRE(aligned16(state) && workspace != nullptr && aligned16(workspace) &&
+                  workspace_bytes >= hmc_vocab_loss_workspace_bytes(tokens, vocab),
+              HMC_ERR_INVALID, "hmc_vocab_loss: the workspace must hold %lld bytes, it and the state on 16-byte boundaries",
+              (long long)hmc_vocab_loss_workspace_bytes(tokens, vocab));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const State st(state, tokens, hidden);
+  float* target_logit = static_cast<float*>(workspace);
+  float2* partial = reinterpret_cast<float2*>(static_cast<char*>(workspace) + up256(4 * tokens));
+  float* token_loss = reduction == HMC_REDUCE_NONE ? loss : nullptr;
+  const Targets given{targets, targets_i64, ignore_index, vocab};
+  const int vector = aligned16(x) && x_stride % 8 == 0;
+  pack_rows_kernel<<<static_cast<unsigned>((tokens + PACK_TOKENS - 1) / PACK_TOKENS), PACK_THREADS, 0, s>>>(
+      static_cast<const __nv_bfloat16*>(x), x_stride, given, tokens, static_cast<int>(hidden), vector, st.count, st.position,
+      st.row_of, st.labels, st.packed, token_loss);
+  HMC_LAUNCH_OK();
+
+  Params p{};
+  p.n = static_cast<int>(vocab), p.k = static_cast<int>(hidden);
+  p.count = st.count, p.labels = st.labels, p.partial = partial, p.pitch = tokens, p.target_logit = target_logit, p.status = status;
+  CUtensorMap a, b;
+  if (int rc = map_k_major(&a, st.packed, hidden, tokens, hidden)) return rc;
+  if (int rc = map_k_major(&b, weight, hidden, vocab, weight_stride)) return rc;
+  if (int rc = launch_product<STATS>(a, b, a, p, tiles_of(tokens) * tiles_of(vocab), s)) return rc;
+  join_kernel<<<static_cast<unsigned>((tokens + 31) / 32), dim3(32, JOIN_SLICES), 0, s>>>(
+      partial, tokens, static_cast<int>(2 * tiles_of(vocab)), st.count, st.labels, st.row_of, target_logit, st.lse, st.losses,
+      token_loss);
+  HMC_LAUNCH_OK();
+  if (reduction != HMC_REDUCE_NONE) {
+    reduce_kernel<<<1, 1024, 0, s>>>(st.losses, st.count, reduction == HMC_REDUCE_MEAN, loss);
+    HMC_LAUNCH_OK();
+  }
+  return 0;
+}
+
+extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_t weight_stride, int64_t tokens, int64_t hidden,
+                                   int64_t vocab, int reduction, const float* grad_loss, void* grad_hidden, void* grad_weight,
+                                   void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  using namespace hmc;
+  if (int rc = check_sizes("hmc_vocab_loss_grad", tokens, hidden, vocab, weight_stride, weight, reduction)) return rc;
+  HMC_REQUIRE(state != nullptr && grad_loss != nullptr && aligned16(state), HMC_ERR_INVALID,
+              "hmc_vocab_loss_grad: null tensor pointer or a state off a 16-byte boundary");
+  HMC_REQUIRE(aligned16(grad_hidden) && aligned16(grad_weight), HMC_ERR_INVALID,
+              "hmc_vocab_loss_grad: gradients must be 16-byte aligned");
+  if (grad_hidden == nullptr && grad_weight == nullptr) return 0;
+  HMC_REQUIRE(workspace != nullptr && aligned16(workspace) &&
+                  workspace_bytes >= hmc_vocab_loss_grad_workspace_bytes(tokens, hidden, vocab),
+              HMC_ERR_INVALID, "hmc_vocab_loss_grad: the workspace must hold %lld bytes on a 16-byte boundary",
+              (long long)hmc_vocab_loss_grad_workspace_bytes(tokens, hidden, vocab));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const State st(const_cast<void*>(state), tokens, hidden);
+  const GradSpace w(workspace, tokens, hidden, vocab);
+  const int width = static_cast<int>(hidden);
+  if (grad_weight != nullptr) HMC_CUDA_OK(cudaMemsetAsync(w.slots, 0xff, w.slot_bytes, s));  // no first row, -1 members
+  grad_rows_kernel<<<static_cast<unsigned>((tokens + 255) / 256), 256, 0, s>>>(
+      grad_loss, reduction, st.count, st.labels, st.row_of, st.losses, w.weights, w.coef, w.scale,
+      grad_weight != nullptr ? w.slots : nullptr, w.members);
+  HMC_LAUNCH_OK();
+  if (grad_weight != nullptr) {
+    const dim3 grid(static_cast<unsigned>(tokens), (width / 8 + WORD_THREADS - 1) / WORD_THREADS);
+    word_sums_kernel<<<grid, WORD_THREADS, 0, s>>>(st.packed, width, st.count, st.labels, w.coef, w.slots, w.members, w.word_sums);
+    HMC_LAUNCH_OK();
+  }
+  if (grad_hidden != nullptr) {
+    zero_ignored_kernel<<<static_cast<unsigned>(tokens), 128, 0, s>>>(st.position, width, static_cast<__nv_bfloat16*>(grad_hidden));
+    HMC_LAUNCH_OK();
+  }
+
+  Params base{};
+  base.count = st.count, base.labels = st.labels, base.lse = st.lse, base.weights = w.weights, base.scale = w.scale;
+  base.coef = w.coef, base.row_of = st.row_of, base.status = status;
+  CUtensorMap rows_k, rows_mn;
+  if (int rc = map_k_major(&rows_k, st.packed, hidden, tokens, hidden)) return rc;
+  if (int rc = map_mn_major(&rows_mn, st.packed, hidden, tokens, hidden)) return rc;
+  for (long long first = 0; first < vocab; first += w.piece) {
+    const long long words = vocab - first < w.piece ? vocab - first : w.piece;
+    const __nv_bfloat16* head = static_cast<const __nv_bfloat16*>(weight) + first * weight_stride;
+    CUtensorMap head_k, head_mn, probs_store, probs_k, probs_mn;
+    if (int rc = map_k_major(&head_k, head, hidden, words, weight_stride)) return rc;
+    if (int rc = map_store(&probs_store, w.probs, words, tokens, w.piece)) return rc;
+    Params p = base;
+    p.first_word = static_cast<int>(first);
+    p.n = static_cast<int>(words), p.k = width;
+    if (int rc = launch_product<PROBS>(rows_k, head_k, probs_store, p, tiles_of(tokens) * tiles_of(words), s)) return rc;
+    if (grad_hidden != nullptr) {
+      if (int rc = map_k_major(&probs_k, w.probs, words, tokens, w.piece)) return rc;
+      if (int rc = map_mn_major(&head_mn, head, hidden, words, weight_stride)) return rc;
+      p.n = width, p.k = static_cast<int>(words);
+      p.sums = w.sums, p.add = first > 0, p.last = first + words == vocab;
+      p.head = static_cast<const __nv_bfloat16*>(weight), p.head_stride = weight_stride;
+      p.out = static_cast<__nv_bfloat16*>(grad_hidden);
+      if (int rc = launch_product<GRAD_HIDDEN>(probs_k, head_mn, probs_k, p, tiles_of(tokens) * tiles_of(width), s)) return rc;
+    }
+    if (grad_weight != nullptr) {
+      CUtensorMap grad_store;
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(grad_weight) + first * hidden;
+      if (int rc = map_mn_major(&probs_mn, w.probs, words, tokens, w.piece)) return rc;
+      if (int rc = map_store(&grad_store, dst, hidden, words, hidden)) return rc;
+      p.m = static_cast<int>(words), p.n = width;
+      p.slots = reinterpret_cast<const int*>(w.slots), p.word_sums = w.word_sums;
+      if (int rc = launch_product<GRAD_WEIGHT>(probs_mn, rows_mn, grad_store, p, tiles_of(words) * tiles_of(width), s)) return rc;
+    }
+  }
+  return 0;
+}

@@ -969,6 +969,54 @@ int hmc_mega_moe_mxfp8_grad(const hmc_mega_moe_mxfp8_grad_args* args, void* stre
 /* ABI version of the MXFP8 operator pair the reference's loader asserts (mega_moe_mxfp8.cpp: == 3). */
 int hmc_mega_moe_mxfp8_abi_version(void);
 
+/* ------------------------------------------------------------------------------------------
+ * Norms of rows (layer norm and RMSNorm) and the cross entropy over a vocabulary: what follows the last block boundary
+ * of a model. No counterpart in the reference, whose only norm is the one inside hyper_mega_mhc.
+ * ------------------------------------------------------------------------------------------ */
+#define HMC_DTYPE_BF16 0
+#define HMC_DTYPE_F16 1
+#define HMC_DTYPE_F32 2
+#define HMC_NORM_MAX_HIDDEN 1048576
+
+/* y[r] = (x[r] - mean) * rstd * weight + bias with mean and rstd = 1 / sqrt(mean((x - mean)^2) + eps) of the row's
+ * `hidden` values; center == 0: mean = 0 and no bias (RMSNorm). x rows start x_stride elements apart (0: the same row
+ * again), y is [rows, hidden] without gaps, both of `dtype`; weight and bias [hidden] of affine_dtype (dtype or FP32),
+ * either may be NULL (1 and 0). mean and rstd, FP32 [rows], are what hmc_row_norm_grad reads: both or neither; without
+ * centring there is no mean. Statistics in FP32, y rounded once. rows < 2^31, hidden <= HMC_NORM_MAX_HIDDEN. */
+int hmc_row_norm(const void* x, int64_t x_stride, int64_t rows, int64_t hidden, int dtype, const void* weight,
+                 const void* bias, int affine_dtype, int center, float eps, void* y, float* mean, float* rstd, void* stream);
+/* Gradients from grad = dy [rows, hidden] (rows grad_stride elements apart): grad_x [rows, hidden] of `dtype` without
+ * gaps, grad_weight and grad_bias [hidden] of affine_dtype, summed over the rows in FP32 in an order that follows from
+ * rows and hidden alone. Each of the three may be NULL. `workspace` (16-byte aligned, of ..._workspace_bytes, which do
+ * not fall as rows grow) is read for grad_weight and grad_bias only. */
+int64_t hmc_row_norm_grad_workspace_bytes(int64_t rows, int64_t hidden);
+int hmc_row_norm_grad(const void* x, int64_t x_stride, const void* grad, int64_t grad_stride, int64_t rows, int64_t hidden,
+                      int dtype, const void* weight, int affine_dtype, int center, const float* mean, const float* rstd,
+                      void* grad_x, void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Cross entropy of hidden states over a vocabulary: loss_i = log sum_j exp(x_i . w_j) - x_i . w_target(i), without ever
+ * holding the logits. x [tokens, hidden] and weight [vocab, hidden] BF16 with rows x_stride and weight_stride elements
+ * apart (weight rows on 16-byte boundaries, hidden a multiple of 8), targets INT32 or INT64. Tokens whose target is
+ * ignore_index have no loss and are not read; a target outside [0, vocab) gives a loss of NaN. reduction: loss [tokens] (0 for
+ * ignored tokens), or loss [1], the sum or the mean over the tokens that count (NaN where none does). `state` (16-byte
+ * aligned, of ..._state_bytes) keeps what the gradient needs, the counted rows of x among it. Logits and sums in FP32. */
+#define HMC_REDUCE_NONE 0
+#define HMC_REDUCE_MEAN 1
+#define HMC_REDUCE_SUM 2
+int64_t hmc_vocab_loss_state_bytes(int64_t tokens, int64_t hidden);
+int64_t hmc_vocab_loss_workspace_bytes(int64_t tokens, int64_t vocab);
+int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* targets,
+                   int targets_i64, int64_t tokens, int64_t hidden, int64_t vocab, int64_t ignore_index, int reduction,
+                   void* state, float* loss, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+/* Gradients from the state of a forward with the same sizes, weight and reduction, and grad_loss (FP32 [tokens] or [1]):
+ * grad_hidden [tokens, hidden] (zeros for ignored tokens) and grad_weight [vocab, hidden], BF16 without gaps; either may be
+ * NULL. The vocabulary is walked in pieces whose BF16 probabilities fit the workspace, the logits are computed again. Results do
+ * not depend on timing. */
+int64_t hmc_vocab_loss_grad_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab);
+int hmc_vocab_loss_grad(const void* state, const void* weight, int64_t weight_stride, int64_t tokens, int64_t hidden,
+                        int64_t vocab, int reduction, const float* grad_loss, void* grad_hidden, void* grad_weight,
+                        void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
