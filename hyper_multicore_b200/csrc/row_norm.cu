@@ -258,6 +258,501 @@ __global__ void __launch_bounds__(512) row_norm_grad_kernel(const T* __restrict_
   }
 }
 
+// ------------------------------------------------------------------------------------------- many rows
+// 16 bytes of T as FP32 pairs: the arithmetic of the kernels below takes two values per instruction, because counted in
+// single ones it is longer than the memory's time (34 instructions per value in a first version, 123 us for 16384 rows of
+// 7168 against 72 us of traffic).
+template <typename T>
+struct Quad;
+template <>
+struct Quad<float> {
+  static constexpr int PAIRS = 2;
+  static __device__ __forceinline__ void widen(const uint4& q, float2* v) {
+    v[0] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+    v[1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
+  }
+  static __device__ __forceinline__ uint4 narrow(const float2* v) {
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+  }
+};
+template <>
+struct Quad<__nv_bfloat16> {
+  static constexpr int PAIRS = 4;
+  static __device__ __forceinline__ float2 pair(uint32_t w) {  // a BF16 is the upper half of its FP32
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ void widen(const uint4& q, float2* v) {
+    v[0] = pair(q.x), v[1] = pair(q.y), v[2] = pair(q.z), v[3] = pair(q.w);
+  }
+  static __device__ __forceinline__ uint4 narrow(const float2* v) {
+    return make_uint4(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[1].x, v[1].y), pack_bf16x2(v[2].x, v[2].y),
+                      pack_bf16x2(v[3].x, v[3].y));
+  }
+};
+template <>
+struct Quad<__half> {
+  static constexpr int PAIRS = 4;
+  static __device__ __forceinline__ float2 pair(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+  static __device__ __forceinline__ uint32_t word(float2 v) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ void widen(const uint4& q, float2* v) {
+    v[0] = pair(q.x), v[1] = pair(q.y), v[2] = pair(q.z), v[3] = pair(q.w);
+  }
+  static __device__ __forceinline__ uint4 narrow(const float2* v) {
+    return make_uint4(word(v[0]), word(v[1]), word(v[2]), word(v[3]));
+  }
+};
+// 2 * PAIRS parameters from p: one or two loads
+template <typename W, int PAIRS>
+__device__ __forceinline__ void widen_params(const W* p, float2* v) {
+#pragma unroll
+  for (int i = 0; i < PAIRS / Quad<W>::PAIRS; ++i)
+    Quad<W>::widen(ld_16(p + i * 2 * Quad<W>::PAIRS), v + i * Quad<W>::PAIRS);
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 times2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 madd2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+constexpr int STREAM_THREADS = 512;
+constexpr int STREAM_WARPS = STREAM_THREADS / 32;
+
+// row_sum for at most STREAM_WARPS warps: every thread reads the slots four at a time, the unused ones are zero.
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float* slots) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) slots[i * STREAM_WARPS + (threadIdx.x >> 5)] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float4 q[STREAM_WARPS / 4];
+#pragma unroll
+    for (int w = 0; w < STREAM_WARPS / 4; ++w) q[w] = reinterpret_cast<const float4*>(slots + i * STREAM_WARPS)[w];
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < STREAM_WARPS / 4; ++w) sum += (q[w].x + q[w].y) + (q[w].z + q[w].w);
+    v[i] = sum;
+  }
+}
+
+// A block walks the rows blockIdx.x, + gridDim.x, ... and copies the next ones asynchronously while it works on one: a ring
+// of rows in shared memory in which a thread writes and reads its own packs only, so that the copies need no barrier.
+// What is left per row is the reduction's, at which the blocks of an SM take turns.
+constexpr int FORWARD_STAGES = 4;
+constexpr int GRAD_STAGES = 3;
+
+template <typename T, typename W, int NV, bool CENTER>
+__global__ void __launch_bounds__(STREAM_THREADS)
+stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, int hidden, const W* __restrict__ weight,
+                   const W* __restrict__ bias, float eps, T* __restrict__ y, float* __restrict__ mean_out,
+                   float* __restrict__ rstd_out) {
+  extern __shared__ uint4 ring_raw[];
+  constexpr int stages = FORWARD_STAGES;
+  __shared__ __align__(16) float slots[2][STREAM_WARPS];
+  constexpr int PAIRS = Quad<T>::PAIRS, VEC = 2 * PAIRS;
+  const int threads = blockDim.x, width = NV * threads;  // packs of a row in the ring
+  const int packs = hidden / VEC;
+  const float scale = 1.0f / static_cast<float>(hidden);
+  uint4* ring = ring_raw + threadIdx.x;
+  if (threadIdx.x < STREAM_WARPS) slots[0][threadIdx.x] = slots[1][threadIdx.x] = 0.0f;
+  bool here[NV];
+  float2 w[NV][PAIRS], b[CENTER ? NV : 1][PAIRS];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int at = j * threads + threadIdx.x;
+    here[j] = at < packs;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      w[j][i] = both(1.0f);
+      if (CENTER) b[j][i] = both(0.0f);
+    }
+    if (here[j] && weight != nullptr) widen_params<W, PAIRS>(weight + at * VEC, w[j]);
+    if (CENTER && here[j] && bias != nullptr) widen_params<W, PAIRS>(bias + at * VEC, b[j]);
+  }
+  const T* mine = x + threadIdx.x * VEC;
+  auto fetch = [&](long long row, int stage) {
+    if (row < rows) {
+      const T* src = mine + row * x_stride;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (here[j]) copy_async_16(ring + stage * width + j * threads, src + j * threads * VEC);
+    }
+    copy_async_commit();
+  };
+  for (int s = 0; s < stages - 1; ++s) fetch(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  __syncthreads();  // the slots are zero
+  int stage = 0, last = stages - 1;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    fetch(row + static_cast<long long>(stages - 1) * gridDim.x, last);
+    copy_async_wait<stages - 1>();  // the copies of a row are one group
+    float2 v[NV][PAIRS];
+    float2 part[2] = {both(0.0f), both(0.0f)};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (here[j]) q = ring[stage * width + j * threads];
+      Quad<T>::widen(q, v[j]);
+      if (CENTER) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) part[i & 1] = add2(part[i & 1], v[j][i]);
+      }
+    }
+    float mean = 0.0f;
+    if (CENTER) {
+      const float2 all = add2(part[0], part[1]);
+      float sum[1] = {all.x + all.y};
+      block_sum(sum, slots[0]);
+      mean = sum[0] * scale;
+      part[0] = part[1] = both(0.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          if (CENTER) v[j][i] = add2(v[j][i], both(-mean));
+          part[i & 1] = madd2(v[j][i], v[j][i], part[i & 1]);
+        }
+      }
+    const float2 all = add2(part[0], part[1]);
+    float square[1] = {all.x + all.y};
+    // a centred row has two reductions and so a barrier between two uses of a slot; the others alternate
+    block_sum(square, slots[CENTER ? 1 : (row / gridDim.x) & 1]);
+    const float rstd = rsqrtf(square[0] * scale + eps);
+    T* dst = y + row * hidden + threadIdx.x * VEC;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          v[j][i] = times2(v[j][i], both(rstd));
+          v[j][i] = CENTER ? madd2(v[j][i], w[j][i], b[j][i]) : times2(v[j][i], w[j][i]);
+        }
+        st_16(dst + j * threads * VEC, Quad<T>::narrow(v[j]));
+      }
+    if (threadIdx.x == 0 && rstd_out != nullptr) {
+      if (CENTER) mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    last = stage;
+    if (++stage == stages) stage = 0;
+  }
+}
+
+// The gradient over the same ring, ROWS rows of x and dy per stage. Threads own columns: the parameters' gradients stay in
+// registers over all rows of a block, so that x and dy are read once. So do g and u of the ROWS rows between the reduction
+// and dx: widening the packs a second time made a row cost 29 instructions per value (163 us for 16384 rows of 7168).
+template <typename T, typename W, int NV, int ROWS, int PITCH, bool CENTER>
+__global__ void __launch_bounds__(PITCH, STREAM_THREADS / PITCH)
+stream_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
+                        long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
+                        const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
+                        float* __restrict__ partial_bias) {
+  extern __shared__ uint4 ring_raw[];
+  constexpr int stages = GRAD_STAGES, SUMS = CENTER ? 2 * ROWS : ROWS;
+  __shared__ __align__(16) float slots[2][SUMS * STREAM_WARPS];
+  constexpr int PAIRS = Quad<T>::PAIRS, VEC = 2 * PAIRS;
+  constexpr int WIDTH = NV * PITCH;  // known at compile time: offsets in the ring cost no arithmetic
+  const int threads = blockDim.x;
+  const int packs = hidden / VEC;
+  const float scale = 1.0f / static_cast<float>(hidden);
+  uint4* ring = ring_raw + threadIdx.x;  // [stage][row][x, dy][NV][PITCH]
+  for (int i = threadIdx.x; i < SUMS * STREAM_WARPS; i += threads) slots[0][i] = slots[1][i] = 0.0f;
+  bool here[NV];
+  constexpr int QUADS = PAIRS / Quad<W>::PAIRS;  // 16-byte pieces of a pack's parameters, kept as they are
+  uint4 params[NV][QUADS];
+  float2 sum_weight[NV][PAIRS], sum_bias[CENTER ? NV : 1][PAIRS];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int at = j * threads + threadIdx.x;
+    here[j] = at < packs;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      sum_weight[j][i] = both(0.0f);
+      if (CENTER) sum_bias[j][i] = both(0.0f);
+    }
+    float2 ones[Quad<W>::PAIRS];
+#pragma unroll
+    for (int i = 0; i < Quad<W>::PAIRS; ++i) ones[i] = both(1.0f);
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i)
+      params[j][i] = here[j] && weight != nullptr ? ld_16(weight + at * VEC + i * 2 * Quad<W>::PAIRS) : Quad<W>::narrow(ones);
+  }
+  const T *mine_x = x + threadIdx.x * VEC, *mine_grad = grad + threadIdx.x * VEC;
+  auto fetch = [&](long long first, int stage) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (first + r < rows) {
+        const T *a = mine_x + (first + r) * x_stride, *d = mine_grad + (first + r) * grad_stride;
+        uint4* dst = ring + (stage * ROWS + r) * 2 * WIDTH;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (here[j]) {
+            copy_async_16(dst + j * PITCH, a + j * threads * VEC);
+            copy_async_16(dst + WIDTH + j * PITCH, d + j * threads * VEC);
+          }
+      }
+    copy_async_commit();
+  };
+  const long long step = static_cast<long long>(ROWS) * gridDim.x;
+  for (int s = 0; s < stages - 1; ++s) fetch(ROWS * static_cast<long long>(blockIdx.x) + s * step, s);
+  __syncthreads();  // the slots are zero
+  int stage = 0, last = stages - 1, turn = 0;
+  float next_mean[ROWS], next_rstd[ROWS];
+  auto stats = [&](long long first) {  // a row that does not exist has scale 0 and adds nothing
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      next_mean[r] = CENTER && first + r < rows ? mean_in[first + r] : 0.0f;
+      next_rstd[r] = first + r < rows ? rstd_in[first + r] : 0.0f;
+    }
+  };
+  stats(ROWS * static_cast<long long>(blockIdx.x));
+  for (long long first = ROWS * static_cast<long long>(blockIdx.x); first < rows; first += step, turn ^= 1) {
+    float mean[ROWS], rstd[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) mean[r] = next_mean[r], rstd[r] = next_rstd[r];
+    stats(first + step);
+    fetch(first + (stages - 1) * step, last);
+    copy_async_wait<stages - 1>();
+    float2 u[ROWS][NV][PAIRS], g[ROWS][NV][PAIRS];
+    float2 along[ROWS], total[ROWS];  // sums of g u and of g
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) along[r] = total[r] = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float2 w[PAIRS];
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) Quad<W>::widen(params[j][i], w + i * Quad<W>::PAIRS);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const uint4* src = ring + ((stage * ROWS + r) * 2 * WIDTH + j * PITCH);
+        uint4 in = make_uint4(0, 0, 0, 0), dy = in;
+        if (here[j] && (r == 0 || first + r < rows)) in = src[0], dy = src[WIDTH];
+        Quad<T>::widen(in, u[r][j]);
+        Quad<T>::widen(dy, g[r][j]);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          float2 &a = u[r][j][i], &d = g[r][j][i];
+          if (CENTER) a = add2(a, both(-mean[r]));
+          a = times2(a, both(rstd[r]));
+          sum_weight[j][i] = madd2(d, a, sum_weight[j][i]);
+          if (CENTER) sum_bias[j][i] = add2(sum_bias[j][i], d);
+          d = times2(d, w[i]);
+          along[r] = madd2(d, a, along[r]);
+          if (CENTER) total[r] = add2(total[r], d);
+        }
+      }
+    }
+    float sums[SUMS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      sums[r] = along[r].x + along[r].y;
+      if (CENTER) sums[ROWS + r] = total[r].x + total[r].y;
+    }
+    block_sum(sums, slots[turn]);
+    if (grad_x != nullptr) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (r > 0 && first + r >= rows) break;
+        T* dst = grad_x + (first + r) * hidden + threadIdx.x * VEC;
+        const float2 by = both(rstd[r]), back = both(-sums[r] * scale * rstd[r]);
+        const float2 offset = CENTER ? both(-sums[ROWS + r] * scale * rstd[r]) : both(0.0f);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (here[j]) {
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+              const float2 v = CENTER ? madd2(g[r][j][i], by, offset) : times2(g[r][j][i], by);
+              g[r][j][i] = madd2(u[r][j][i], back, v);
+            }
+            st_16(dst + j * threads * VEC, Quad<T>::narrow(g[r][j]));
+          }
+      }
+    }
+    last = stage;
+    if (++stage == stages) stage = 0;
+  }
+  if (partial_weight == nullptr) return;
+  const long long base = static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (here[j]) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; i += 2) {
+        const long long at = base + j * threads * VEC + 2 * i;
+        *reinterpret_cast<float4*>(partial_weight + at) =
+            make_float4(sum_weight[j][i].x, sum_weight[j][i].y, sum_weight[j][i + 1].x, sum_weight[j][i + 1].y);
+        if (CENTER)
+          *reinterpret_cast<float4*>(partial_bias + at) =
+              make_float4(sum_bias[j][i].x, sum_bias[j][i].y, sum_bias[j][i + 1].x, sum_bias[j][i + 1].y);
+      }
+    }
+}
+
+// The same for rows whose u and g do not fit the registers of two blocks per SM beside the sums: one row at a time, which is
+// widened again from the ring behind the reduction. More instructions, but 28 instead of 14 warps to issue them.
+constexpr int WIDE_THREADS = 448;
+template <typename T, typename W, int NV, bool CENTER>
+__global__ void __launch_bounds__(WIDE_THREADS, 2)
+stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
+                        long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
+                        const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
+                        float* __restrict__ partial_bias) {
+  extern __shared__ uint4 ring_raw[];
+  constexpr int stages = GRAD_STAGES, SUMS = CENTER ? 2 : 1;
+  __shared__ __align__(16) float slots[2][SUMS * STREAM_WARPS];
+  constexpr int PAIRS = Quad<T>::PAIRS, VEC = 2 * PAIRS;
+  constexpr int PITCH = WIDE_THREADS, WIDTH = NV * PITCH;  // known at compile time: offsets in the ring cost no arithmetic
+  const int threads = blockDim.x;
+  const int packs = hidden / VEC;
+  const float scale = 1.0f / static_cast<float>(hidden);
+  uint4* ring = ring_raw + threadIdx.x;  // [stage][x, dy][NV][PITCH]; the weight in FP32 [NV][PAIRS / 2][PITCH]
+  float4* gain = reinterpret_cast<float4*>(ring_raw + 2 * stages * WIDTH) + threadIdx.x;
+  for (int i = threadIdx.x; i < SUMS * STREAM_WARPS; i += threads) slots[0][i] = slots[1][i] = 0.0f;
+  bool here[NV];
+  float2 sum_weight[NV][PAIRS], sum_bias[CENTER ? NV : 1][PAIRS];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int at = j * threads + threadIdx.x;
+    here[j] = at < packs;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      sum_weight[j][i] = both(0.0f);
+      if (CENTER) sum_bias[j][i] = both(0.0f);
+    }
+    float2 w[PAIRS];
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) w[i] = both(1.0f);
+    if (here[j] && weight != nullptr) widen_params<W, PAIRS>(weight + at * VEC, w);
+#pragma unroll
+    for (int i = 0; i < PAIRS; i += 2)
+      gain[(j * PAIRS + i) / 2 * PITCH] = make_float4(w[i].x, w[i].y, w[i + 1].x, w[i + 1].y);
+  }
+  const T *mine_x = x + threadIdx.x * VEC, *mine_grad = grad + threadIdx.x * VEC;
+  auto fetch = [&](long long row, int stage) {
+    if (row < rows) {
+      const T *a = mine_x + row * x_stride, *d = mine_grad + row * grad_stride;
+      uint4* dst = ring + stage * 2 * WIDTH;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (here[j]) {
+          copy_async_16(dst + j * PITCH, a + j * threads * VEC);
+          copy_async_16(dst + WIDTH + j * PITCH, d + j * threads * VEC);
+        }
+    }
+    copy_async_commit();
+  };
+  for (int s = 0; s < stages - 1; ++s) fetch(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  __syncthreads();  // the slots are zero
+  int stage = 0, last = stages - 1, turn = 0;
+  float next_mean = CENTER && blockIdx.x < rows ? mean_in[blockIdx.x] : 0.0f;
+  float next_rstd = blockIdx.x < rows ? rstd_in[blockIdx.x] : 0.0f;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
+    const long long next = row + gridDim.x;
+    if (next < rows) {
+      if (CENTER) next_mean = mean_in[next];
+      next_rstd = rstd_in[next];
+    }
+    fetch(row + static_cast<long long>(stages - 1) * gridDim.x, last);
+    copy_async_wait<stages - 1>();
+    const uint4* src = ring + stage * 2 * WIDTH;
+    float2 along = both(0.0f), total = both(0.0f);  // rstd times the sums of g (x - mean) and of g
+    auto widen = [&](int j, float2* c, float2* d, float2* w) {  // x - mean, dy, weight
+      Quad<T>::widen(src[j * PITCH], c);
+      Quad<T>::widen(src[WIDTH + j * PITCH], d);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        if (CENTER) c[i] = add2(c[i], both(-mean));
+        if ((i & 1) == 0) {
+          const float4 q = gain[(j * PAIRS + i) / 2 * PITCH];
+          w[i] = make_float2(q.x, q.y), w[i + 1] = make_float2(q.z, q.w);
+        }
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+        float2 c[PAIRS], d[PAIRS], w[PAIRS];
+        widen(j, c, d, w);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          if (CENTER) sum_bias[j][i] = add2(sum_bias[j][i], d[i]);
+          d[i] = times2(d[i], both(rstd));
+          sum_weight[j][i] = madd2(d[i], c[i], sum_weight[j][i]);
+          d[i] = times2(d[i], w[i]);
+          along = madd2(d[i], c[i], along);
+          if (CENTER) total = add2(total, d[i]);
+        }
+      }
+    float sums[SUMS];
+    sums[0] = along.x + along.y;
+    if (CENTER) sums[SUMS - 1] = total.x + total.y;
+    block_sum(sums, slots[turn]);
+    if (grad_x != nullptr) {
+      T* dst = grad_x + row * hidden + threadIdx.x * VEC;
+      // dx = rstd g - (x - mean) rstd^2 mean(g u) - rstd mean(g), u = (x - mean) rstd
+      const float2 back = both(-sums[0] * scale * rstd * rstd), offset = both(CENTER ? -sums[SUMS - 1] * scale : 0.0f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (here[j]) {
+          float2 c[PAIRS], d[PAIRS], w[PAIRS];
+          widen(j, c, d, w);
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) {
+            d[i] = times2(d[i], both(rstd));
+            d[i] = CENTER ? madd2(d[i], w[i], offset) : times2(d[i], w[i]);
+            d[i] = madd2(c[i], back, d[i]);
+          }
+          st_16(dst + j * threads * VEC, Quad<T>::narrow(d));
+        }
+    }
+    last = stage;
+    if (++stage == stages) stage = 0;
+  }
+  if (partial_weight == nullptr) return;
+  const long long base = static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (here[j]) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; i += 2) {
+        const long long at = base + j * threads * VEC + 2 * i;
+        *reinterpret_cast<float4*>(partial_weight + at) =
+            make_float4(sum_weight[j][i].x, sum_weight[j][i].y, sum_weight[j][i + 1].x, sum_weight[j][i + 1].y);
+        if (CENTER)
+          *reinterpret_cast<float4*>(partial_bias + at) =
+              make_float4(sum_bias[j][i].x, sum_bias[j][i].y, sum_bias[j][i + 1].x, sum_bias[j][i + 1].y);
+      }
+    }
+}
+
 // Rows too long for a block's registers: dx by one block per row, the parameters' partial sums by columns.
 template <typename T, typename W, bool CENTER>
 __global__ void __launch_bounds__(1024) long_row_norm_grad_kernel(const T* __restrict__ x, long long x_stride,
@@ -306,7 +801,7 @@ __global__ void __launch_bounds__(256) column_grad_kernel(const T* __restrict__ 
 }
 
 // Parameters' gradients: the partial sums of a column in the order of the blocks that made them.
-constexpr int FINISH_SLICES = 8;
+constexpr int FINISH_SLICES = 32;
 template <typename W>
 __global__ void __launch_bounds__(32 * FINISH_SLICES) param_grad_kernel(const float* __restrict__ partial_weight,
                                                                         const float* __restrict__ partial_bias, int parts,
@@ -328,7 +823,7 @@ __global__ void __launch_bounds__(32 * FINISH_SLICES) param_grad_kernel(const fl
   W* out = threadIdx.y == 0 ? grad_weight : grad_bias;
   if (out == nullptr) return;
   float v = 0.0f;
-#pragma unroll
+#pragma unroll 8
   for (int s = 0; s < FINISH_SLICES; ++s) v += sums[threadIdx.y][s][threadIdx.x];
   out[c] = narrow<W>(v);
 }
@@ -354,9 +849,10 @@ struct NormCall {
   cudaStream_t stream;
 };
 
-// Blocks of the gradient kernel: two per SM, each with partial sums of its own.
+// Blocks of the gradient kernels: two per SM at most, each with partial sums of its own.
+constexpr int GRAD_BLOCKS = 2;
 long long grad_parts(long long rows) {
-  const long long most = 2ll * sm_count();
+  const long long most = static_cast<long long>(GRAD_BLOCKS) * sm_count();
   return rows < most ? rows : most;
 }
 
@@ -373,11 +869,115 @@ int launch_forward(const NormCall& c) {
   return 0;
 }
 
+constexpr int SM_SHARED = 227 * 1024;
+constexpr int STREAM_SHARED = SM_SHARED - 2048;  // beside the reductions' slots
+
+// Blocks of `threads` threads with `bytes` of shared memory that an SM holds of a kernel; asked once per block size.
+struct Residency {
+  int blocks[HMC_MAX_DEVICES][STREAM_WARPS + 1];
+};
+template <typename Kernel>
+int resident_blocks(Kernel kernel, int threads, int bytes, Residency& known, int* blocks) {
+  int dev = 0;
+  HMC_CUDA_OK(cudaGetDevice(&dev));
+  int* slot = dev < HMC_MAX_DEVICES ? &known.blocks[dev][threads / 32] : nullptr;
+  if (slot == nullptr || *slot == 0) {
+    HMC_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SHARED));
+    int found = 0;
+    HMC_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&found, kernel, threads, bytes));
+    if (found < 1) found = 1;
+    if (slot == nullptr) {
+      *blocks = found;
+      return 0;
+    }
+    *slot = found;
+  }
+  *blocks = *slot;
+  return 0;
+}
+
+template <typename T, typename W, int NV, bool CENTER>
+int launch_stream(const NormCall& c) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
+  const int bytes = FORWARD_STAGES * NV * threads * 16;
+  static Residency known{};
+  auto kernel = stream_norm_kernel<T, W, NV, CENTER>;
+  int blocks = 0;
+  if (int rc = resident_blocks(kernel, threads, bytes, known, &blocks)) return rc;
+  const long long most = static_cast<long long>(blocks) * sm_count();
+  kernel<<<static_cast<unsigned>(c.rows < most ? c.rows : most), threads, bytes, c.stream>>>(
+      static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
+      c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
+  HMC_LAUNCH_OK();
+  return 0;
+}
+
+// Packs per thread, so that a row has about 256 threads and no more than STREAM_THREADS.
+template <typename T, typename W, bool CENTER>
+int stream(const NormCall& c) {
+  const int packs = c.hidden / (16 / static_cast<int>(sizeof(T)));
+  if (packs <= 256) return launch_stream<T, W, 1, CENTER>(c);
+  return packs <= 512 ? launch_stream<T, W, 2, CENTER>(c) : launch_stream<T, W, 4, CENTER>(c);
+}
+
+template <typename T, typename W, int NV, int ROWS, int PITCH, bool CENTER>
+int launch_stream_grad(NormCall& c) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
+  const int bytes = GRAD_STAGES * ROWS * 2 * NV * PITCH * 16;
+  static Residency known{};
+  auto kernel = stream_norm_grad_kernel<T, W, NV, ROWS, PITCH, CENTER>;
+  int blocks = 0;
+  if (int rc = resident_blocks(kernel, threads, bytes, known, &blocks)) return rc;
+  if (blocks > GRAD_BLOCKS) blocks = GRAD_BLOCKS;
+  const long long most = static_cast<long long>(blocks) * sm_count(), pieces = (c.rows + ROWS - 1) / ROWS;
+  c.parts = static_cast<int>(pieces < most ? pieces : most);
+  kernel<<<static_cast<unsigned>(c.parts), threads, bytes, c.stream>>>(
+      static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
+      static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias);
+  HMC_LAUNCH_OK();
+  return 0;
+}
+
+template <typename T, typename W, int NV, bool CENTER>
+int launch_wide_grad(NormCall& c) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
+  const int bytes = NV * WIDE_THREADS * (GRAD_STAGES * 2 * 16 + VEC * 4);
+  static Residency known{};
+  auto kernel = stream_wide_grad_kernel<T, W, NV, CENTER>;
+  int blocks = 0;
+  if (int rc = resident_blocks(kernel, threads, bytes, known, &blocks)) return rc;
+  if (blocks > GRAD_BLOCKS) blocks = GRAD_BLOCKS;
+  const long long most = static_cast<long long>(blocks) * sm_count();
+  c.parts = static_cast<int>(c.rows < most ? c.rows : most);
+  kernel<<<static_cast<unsigned>(c.parts), threads, bytes, c.stream>>>(
+      static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
+      static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias);
+  HMC_LAUNCH_OK();
+  return 0;
+}
+
+// Threads of the gradient of the longest rows that stream, 32 values each: three stages of x and dy fill shared memory.
+template <typename T>
+constexpr int LONGEST = sizeof(T) == 4 ? 288 : STREAM_THREADS;
+
+template <typename T, typename W, bool CENTER>
+int stream_grad(NormCall& c) {
+  constexpr int NV = sizeof(T) == 4 ? 4 : 2;  // 16 values per thread
+  if (c.hidden <= 16 * 256) return launch_stream_grad<T, W, NV, 2, 256, CENTER>(c);
+  if (c.hidden <= 16 * WIDE_THREADS) return launch_wide_grad<T, W, NV, CENTER>(c);
+  return launch_stream_grad<T, W, 2 * NV, 1, LONGEST<T>, CENTER>(c);
+}
+
 template <typename T, typename W, bool CENTER>
 int forward(const NormCall& c) {
   constexpr int VEC = 16 / sizeof(T);
   const bool wide = c.hidden % VEC == 0 && c.x_stride % VEC == 0 && aligned_to(c.x, 16) && aligned_to(c.y, 16) &&
                     aligned_to(c.weight, 16) && aligned_to(c.bias, 16);
+  if (wide && c.rows > 2ll * sm_count() && c.hidden > 32 * VEC * FORWARD_PACKS && c.hidden <= STREAM_THREADS * VEC * FORWARD_PACKS)
+    return stream<T, W, CENTER>(c);
   if (wide && c.hidden <= 1024 * VEC * FORWARD_PACKS) return launch_forward<T, W, VEC, FORWARD_PACKS, CENTER>(c);
   if (c.hidden <= 1024 * SINGLES) return launch_forward<T, W, 1, SINGLES, CENTER>(c);
   long_row_norm_kernel<T, W, CENTER><<<static_cast<unsigned>(c.rows), 1024, 0, c.stream>>>(
@@ -398,11 +998,13 @@ int launch_grad(const NormCall& c) {
 }
 
 template <typename T, typename W, bool CENTER>
-int gradient(const NormCall& c) {
+int gradient(NormCall& c) {
   constexpr int VEC = 16 / sizeof(T);
   const bool wide = c.hidden % VEC == 0 && c.x_stride % VEC == 0 && c.grad_stride % VEC == 0 && aligned_to(c.x, 16) &&
                     aligned_to(c.grad, 16) && aligned_to(c.y, 16) && aligned_to(c.weight, 16);
-  if (wide && c.hidden <= GRAD_THREADS * VEC * GRAD_PACKS) {
+  if (wide && c.hidden > 32 * VEC * FORWARD_PACKS && c.hidden <= 32 * LONGEST<T>) {
+    if (int rc = stream_grad<T, W, CENTER>(c)) return rc;
+  } else if (wide && c.hidden <= GRAD_THREADS * VEC * GRAD_PACKS) {
     if (int rc = launch_grad<T, W, VEC, GRAD_PACKS, CENTER>(c)) return rc;
   } else if (c.hidden <= GRAD_THREADS * SINGLES) {
     if (int rc = launch_grad<T, W, 1, SINGLES, CENTER>(c)) return rc;
@@ -430,12 +1032,12 @@ int gradient(const NormCall& c) {
 }
 
 template <typename T, typename W>
-int run(const NormCall& c, bool center, bool backward) {
+int run(NormCall& c, bool center, bool backward) {
   if (backward) return center ? gradient<T, W, true>(c) : gradient<T, W, false>(c);
   return center ? forward<T, W, true>(c) : forward<T, W, false>(c);
 }
 
-int run(const NormCall& c, int dtype, int affine_dtype, bool center, bool backward) {
+int run(NormCall& c, int dtype, int affine_dtype, bool center, bool backward) {
   if (dtype == HMC_DTYPE_F32) return run<float, float>(c, center, backward);
   if (dtype == HMC_DTYPE_BF16)
     return affine_dtype == HMC_DTYPE_F32 ? run<__nv_bfloat16, float>(c, center, backward)
