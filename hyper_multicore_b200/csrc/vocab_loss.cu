@@ -41,6 +41,9 @@ constexpr int HALF = TILE / 2;  // rows of A and columns of B that a CTA loads
 constexpr int STAGE_BYTES = 2 * A_TILE_BYTES;
 constexpr int STAGES = 6;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * STORE_STAGE_BYTES + 1024 + 256;
+constexpr int MAX_PARTS = 16;  // of a tile that is cut along k
+constexpr int MIN_PART = 8;    // k-blocks of a part, at the least
+constexpr int PROMOTE = 8;     // k-blocks that add up inside the tensor core before the sum goes to FP32 registers (STATS)
 constexpr int BAND = 8;  // tile rows that are walked together: 8 x 9 tiles in flight share their operands in L2
 
 enum Product { STATS, PROBS, GRAD_HIDDEN, GRAD_WEIGHT };
@@ -65,21 +68,58 @@ struct Params {
   __nv_bfloat16* out;         // GRAD_HIDDEN
   const int* slots;           // GRAD_WEIGHT: [vocab] row of word_sums, or -1
   const float* word_sums;     // GRAD_WEIGHT: [rows, n]
+  float* part_sums;           // GRAD_HIDDEN: [parts][TILE][TILE] of the tiles that are cut
   int* status;
 };
 
-// Tiles in bands of BAND tile rows, a band's columns one after the other.
+// A unit of work: a tile and its range of k-blocks. Part -1 is the whole of it.
+struct Unit {
+  int mi, ni, part;
+  int kb0, kb1;
+};
+
+// Tiles in bands of BAND tile rows, a band's columns one after the other. With `split`, the tiles that would leave pairs
+// idle in the last wave are cut along k: into as many parts as shorten that wave most, counted with a hundredth of a tile's
+// time per part for what they write, at most two parts per pair (4 tiles of 32 wide and k 32000 on 74 pairs: one part each in
+// 166 us, 9 in 29 us).
 struct Walker {
-  int mt, nt;
-  __device__ Walker(int m, int n) : mt((m + TILE - 1) / TILE), nt((n + TILE - 1) / TILE) {}
-  __device__ bool get(long long idx, int& mi, int& ni) const {
-    if (idx >= static_cast<long long>(mt) * nt) return false;
+  int mt, nt, kiters, parts;
+  long long whole, units;
+  __device__ Walker(int m, int n, int k, int pairs, bool split)
+      : mt((m + TILE - 1) / TILE), nt((n + TILE - 1) / TILE), kiters((k + BK - 1) / BK), parts(1) {
+    const long long tiles = static_cast<long long>(mt) * nt;
+    whole = tiles;
+    if (split) {
+      const int rest = static_cast<int>(tiles % pairs);
+      float best = 1.0f;
+      for (int s = 2; s <= MAX_PARTS && rest > 0 && rest * s <= 2 * pairs && s * MIN_PART <= kiters; ++s) {
+        const float cost = static_cast<float>((rest * s + pairs - 1) / pairs) / static_cast<float>(s) + 0.01f * static_cast<float>(s);
+        if (cost < best) best = cost, parts = s;
+      }
+      if (parts > 1) whole = tiles - rest;
+    }
+    units = whole + (tiles - whole) * parts;
+  }
+  __device__ void tile(long long idx, int& mi, int& ni) const {
     const long long per_band = static_cast<long long>(BAND) * nt;
     const int band = static_cast<int>(idx / per_band);
     const int local = static_cast<int>(idx - band * per_band);
     const int high = min(BAND, mt - band * BAND);
     mi = band * BAND + local % high;
     ni = local / high;
+  }
+  __device__ bool get(long long idx, Unit& u) const {
+    if (idx >= units) return false;
+    u.part = -1, u.kb0 = 0, u.kb1 = kiters;
+    if (idx >= whole) {
+      const int cut = static_cast<int>(idx - whole);
+      u.part = cut % parts;
+      u.kb0 = static_cast<int>(static_cast<long long>(kiters) * u.part / parts);
+      u.kb1 = static_cast<int>(static_cast<long long>(kiters) * (u.part + 1) / parts);
+      u.part = cut;  // where its sums go
+      idx = whole + cut / parts;
+    }
+    tile(idx, u.mi, u.ni);
     return true;
   }
 };
@@ -87,40 +127,29 @@ struct Walker {
 __device__ __forceinline__ float shifted_exp(float v, float top) { return __expf(v - top); }
 
 // Maximum and sum of exponentials of one row's 128 columns; the target's logit where it lies among them.
-__device__ __forceinline__ void epilogue_stats(const Params& p, uint32_t taddr, int row, bool row_ok, int col, int half_tile) {
-  const int label = row_ok ? p.labels[row] : -1;
-  float top = -INFINITY, sum = 0.0f;
-#pragma unroll 1
-  for (int c = 0; c < HALF; c += 32) {
-    if (col + c >= p.n) break;
-    __syncwarp();
-    uint32_t raw[32];
-    tmem_ld_32x32(taddr + c, raw);
-    tmem_ld_wait();
-    float high = top;
-    if (col + c + 32 > p.n) {
+__device__ __forceinline__ void epilogue_stats(const Params& p, float (&v)[HALF], int row, int col, int half_tile) {
+  const int label = p.labels[row] - col;
+  if (col + HALF > p.n) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col + c + j >= p.n) raw[j] = __float_as_uint(-INFINITY);
-    }
-#pragma unroll
-    for (int j = 0; j < 32; ++j) high = fmaxf(high, __uint_as_float(raw[j]));
-    const float shift = high == -INFINITY ? 0.0f : high;  // nothing but -inf so far: exp(-inf - 0), not exp(-inf + inf)
-    float add = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) add += shifted_exp(__uint_as_float(raw[j]), shift);
-    sum = sum * shifted_exp(top, shift) + add;
-    top = high;
-    const int at = label - (col + c);
-    if (at >= 0 && at < 32) {
-      float own = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j == at) own = __uint_as_float(raw[j]);
-      p.target_logit[row] = own;
-    }
+    for (int j = 0; j < HALF; ++j)
+      if (col + j >= p.n) v[j] = -INFINITY;
   }
-  if (row_ok) p.partial[half_tile * p.pitch + row] = make_float2(top, sum);
+  if (label >= 0 && label < HALF) {
+    float own = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HALF; ++j)
+      if (j == label) own = v[j];
+    p.target_logit[row] = own;
+  }
+  float high[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int j = 4; j < HALF; ++j) high[j & 3] = fmaxf(high[j & 3], v[j]);
+  const float top = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+  const float shift = top == -INFINITY ? 0.0f : top;  // nothing but -inf: exp(-inf - 0), not exp(-inf + inf)
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < HALF; ++j) sum[j & 3] += shifted_exp(v[j], shift);
+  p.partial[half_tile * p.pitch + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
 }
 
 // 32 x 32 values leave as one BF16 box through shared memory; two boxes per warp in flight.
@@ -167,14 +196,38 @@ __device__ __forceinline__ void epilogue_probs(const Params& p, const CUtensorMa
   }
 }
 
+// Eight columns of a row of dx from this piece's sums: added to those of earlier pieces, and with the last piece the target's
+// row on top, scaled, rounded and stored at the token's place.
+__device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int col, float (&v)[8], float scale) {
+  float* sums = p.sums + static_cast<long long>(row) * p.n + col;
+  if (p.add) {
+    const float4 a = *reinterpret_cast<const float4*>(sums), b = *reinterpret_cast<const float4*>(sums + 4);
+    v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+  }
+  if (!p.last) {
+    *reinterpret_cast<float4*>(sums) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(sums + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    return;
+  }
+  const int label = p.labels[row];
+  if (label >= 0) {
+    const float coef = p.coef[row];
+    const uint4 w = ld_16(p.head + label * p.head_stride + col);
+    const uint32_t parts[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack_bf16x2(parts[e]);
+      v[2 * e] += coef * f.x;
+      v[2 * e + 1] += coef * f.y;
+    }
+  }
+  st_16(p.out + static_cast<long long>(p.row_of[row]) * p.n + col,
+        make_uint4(pack_bf16x2(v[0] * scale, v[1] * scale), pack_bf16x2(v[2] * scale, v[3] * scale),
+                   pack_bf16x2(v[4] * scale, v[5] * scale), pack_bf16x2(v[6] * scale, v[7] * scale)));
+}
+
 __device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t taddr, int row, bool row_ok, int col) {
   const float scale = *p.scale;
-  const float coef = row_ok ? p.coef[row] : 0.0f;
-  const int label = row_ok ? p.labels[row] : -1;
-  const long long token = row_ok ? p.row_of[row] : 0;
-  float* sums = p.sums + static_cast<long long>(row) * p.n + col;
-  const __nv_bfloat16* word = p.head + (label >= 0 ? label : 0) * p.head_stride + col;
-  __nv_bfloat16* dst = p.out + token * p.n + col;
 #pragma unroll 1
   for (int c = 0; c < HALF; c += 32) {
     if (col + c >= p.n) break;
@@ -188,29 +241,47 @@ __device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t t
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(raw[j + e]);
-      if (p.add) {
-        const float4 a = *reinterpret_cast<const float4*>(sums + c + j), b = *reinterpret_cast<const float4*>(sums + c + j + 4);
-        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
-      }
-      if (!p.last) {
-        *reinterpret_cast<float4*>(sums + c + j) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(sums + c + j + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        continue;
-      }
-      if (label >= 0) {
-        const uint4 w = ld_16(word + c + j);
-        const uint32_t parts[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack_bf16x2(parts[e]);
-          v[2 * e] += coef * f.x;
-          v[2 * e + 1] += coef * f.y;
-        }
-      }
-      st_16(dst + c + j, make_uint4(pack_bf16x2(v[0] * scale, v[1] * scale), pack_bf16x2(v[2] * scale, v[3] * scale),
-                                    pack_bf16x2(v[4] * scale, v[5] * scale), pack_bf16x2(v[6] * scale, v[7] * scale)));
+      finish_grad_hidden(p, row, col + c + j, v, scale);
     }
   }
+}
+
+// A part of a tile that is cut along k: its sums as they are.
+__device__ __forceinline__ void epilogue_part(const Params& p, uint32_t taddr, int part, int row_in_tile, bool row_ok, int half) {
+  float* dst = p.part_sums + (static_cast<long long>(part) * TILE + row_in_tile) * TILE + half * HALF;
+#pragma unroll 1
+  for (int c = 0; c < HALF; c += 32) {
+    __syncwarp();
+    uint32_t raw[32];
+    tmem_ld_32x32(taddr + c, raw);
+    tmem_ld_wait();
+    if (row_ok) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) st_16(dst + c + j, make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3]));
+    }
+  }
+}
+
+// The tiles that were cut: their parts in order, eight columns per thread, eight rows per block.
+__global__ void __launch_bounds__(256) join_parts_kernel(Params p, int pairs) {
+  p.m = *p.count;
+  const Walker walker(p.m, p.n, p.k, pairs, true);
+  const long long tile = walker.whole + blockIdx.y;
+  if (walker.parts == 1 || tile >= static_cast<long long>(walker.mt) * walker.nt) return;
+  int mi, ni;
+  walker.tile(tile, mi, ni);
+  const int in_tile = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int row = mi * TILE + in_tile, col = ni * TILE + (threadIdx.x & 31) * 8;
+  if (row >= p.m || col >= p.n) return;
+  const float* src = p.part_sums + ((static_cast<long long>(blockIdx.y) * walker.parts * TILE + in_tile) * TILE) + (threadIdx.x & 31) * 8;
+  float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = 0; s < walker.parts; ++s) {
+    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+    v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+    src += TILE * TILE;
+  }
+  finish_grad_hidden(p, row, col, v, *p.scale);
 }
 
 __device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
@@ -254,6 +325,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                  const __grid_constant__ CUtensorMap tm_c, Params p) {
   constexpr int A_MAJOR = KIND == GRAD_WEIGHT ? HMC_MAJOR_MN : HMC_MAJOR_K;
   constexpr int B_MAJOR = KIND == GRAD_WEIGHT || KIND == GRAD_HIDDEN ? HMC_MAJOR_MN : HMC_MAJOR_K;
+  constexpr int CHAIN = PROMOTE;  // STATS only
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* store_stage = smem + STAGES * STAGE_BYTES;
@@ -298,9 +370,9 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   const int count = *p.count;
   if (KIND == GRAD_WEIGHT) p.k = count;
   else p.m = count;
-  const int kiters = (p.k + BK - 1) / BK;
-  const Walker walker(p.m, p.n);
-  int mi, ni;
+  const Walker walker(p.m, p.n, p.k, static_cast<int>(pairs), KIND == GRAD_HIDDEN);
+  const int kiters = walker.kiters;
+  Unit u;
 
   if (warp == 0) {
     // ======================================================================== TMA producer (both CTAs)
@@ -308,10 +380,10 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (long long idx = pair; ok && walker.get(idx, mi, ni); idx += pairs) {
-        const int m0 = mi * TILE + static_cast<int>(rank) * HALF;
-        const int n0 = ni * TILE + static_cast<int>(rank) * HALF;
-        for (int kb = 0; kb < kiters; ++kb) {
+      for (long long idx = pair; ok && walker.get(idx, u); idx += pairs) {
+        const int m0 = u.mi * TILE + static_cast<int>(rank) * HALF;
+        const int n0 = u.ni * TILE + static_cast<int>(rank) * HALF;
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
             report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 0, stage, kb);
             ok = false;
@@ -353,43 +425,47 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       constexpr uint32_t B_LBO = B_MAJOR == HMC_MAJOR_MN ? CHUNK_BYTES : 16;
       constexpr uint32_t A_KSTEP = A_MAJOR == HMC_MAJOR_MN ? (16 * 128) >> 4 : 32 >> 4;
       constexpr uint32_t B_KSTEP = B_MAJOR == HMC_MAJOR_MN ? (16 * 128) >> 4 : 32 >> 4;
-      for (long long idx = pair; ok && walker.get(idx, mi, ni); idx += pairs) {
-        if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
-          if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 1, acc, 0);
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * TILE);
-        for (int kb = 0; kb < kiters; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, abort_word, PIPE_BUDGET_NS)) {
-            if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 2, stage, kb);
+      for (long long idx = pair; ok && walker.get(idx, u); idx += pairs) {
+        // one accumulator per unit, or per CHAIN k-blocks of it
+        for (int first = u.kb0; ok && first < u.kb1; first += KIND == STATS ? CHAIN : u.kb1 - u.kb0) {
+          const int end = KIND == STATS ? min(u.kb1, first + CHAIN) : u.kb1;
+          if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
+            if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 1, acc, 0);
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          if (lane == 0) {
-            uint8_t* a_src = smem + stage * STAGE_BYTES;
-            uint64_t da = make_smem_desc(smem_u32(a_src), A_LBO, 1024, SWIZZLE_128B);
-            uint64_t db = make_smem_desc(smem_u32(a_src + A_TILE_BYTES), B_LBO, 1024, SWIZZLE_128B);
-#pragma unroll
-            for (int ks = 0; ks < BK / 16; ++ks) {
-              umma_bf16_pair(tmem_d, da, db, idesc, (kb > 0 || ks > 0) ? 1u : 0u);
-              da += A_KSTEP;
-              db += B_KSTEP;
+          const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * TILE);
+          for (int kb = first; kb < end; ++kb) {
+            if (!mbar_wait(&full_bar[stage], phase, abort_word, PIPE_BUDGET_NS)) {
+              if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 2, stage, kb);
+              ok = false;
+              break;
             }
-            umma_commit_pair(&empty_bar[stage]);  // frees the slot in both CTAs
-            if (kb == kiters - 1) umma_commit_pair(&acc_full_bar[acc]);
+            tc_fence_after_sync();
+            if (lane == 0) {
+              uint8_t* a_src = smem + stage * STAGE_BYTES;
+              uint64_t da = make_smem_desc(smem_u32(a_src), A_LBO, 1024, SWIZZLE_128B);
+              uint64_t db = make_smem_desc(smem_u32(a_src + A_TILE_BYTES), B_LBO, 1024, SWIZZLE_128B);
+#pragma unroll
+              for (int ks = 0; ks < BK / 16; ++ks) {
+                umma_bf16_pair(tmem_d, da, db, idesc, (kb > first || ks > 0) ? 1u : 0u);
+                da += A_KSTEP;
+                db += B_KSTEP;
+              }
+              umma_commit_pair(&empty_bar[stage]);  // frees the slot in both CTAs
+              if (kb == end - 1) umma_commit_pair(&acc_full_bar[acc]);
+            }
+            __syncwarp();
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-          __syncwarp();
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
+          if (++acc == ACC_STAGES) {
+            acc = 0;
+            acc_phase ^= 1u;
           }
-        }
-        if (++acc == ACC_STAGES) {
-          acc = 0;
-          acc_phase ^= 1u;
         }
       }
     }
@@ -403,35 +479,67 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     uint8_t* my_stage = store_stage + (warp - 2) * STORE_STAGE_BYTES;
     unsigned issued = 0;
     const uint32_t leader_acc_empty = map_to_cta(smem_u32(acc_empty_bar), 0);
-    for (long long idx = pair; ok && walker.get(idx, mi, ni); idx += pairs) {
-      const int first_row = mi * TILE + static_cast<int>(rank) * HALF + quarter * 32;
-      const int row = first_row + lane;
-      const bool row_ok = row < p.m;
-      const int col = ni * TILE + half * HALF;
-      if (kiters == 0) {  // no token counts: the weight's gradient is zero
-        if (KIND == GRAD_WEIGHT) epilogue_grad_weight(p, &tm_c, 0, my_stage, issued, first_row, row, row_ok, col, lane, true);
-        continue;
-      }
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * HALF);
+    auto filled = [&]() {  // the next accumulator, once its MMAs are done
       if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_word, PIPE_BUDGET_NS)) {
         if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 3, acc, 0);
         ok = false;
-        break;
       }
       tc_fence_after_sync();
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * TILE + half * HALF);
-      if (KIND == STATS) epilogue_stats(p, taddr, row, row_ok, col, 2 * ni + half);
-      if (KIND == PROBS) epilogue_probs(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane);
-      if (KIND == GRAD_HIDDEN) epilogue_grad_hidden(p, taddr, row, row_ok, col);
-      if (KIND == GRAD_WEIGHT)
-        epilogue_grad_weight(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane, false);
+      return ok;
+    };
+    auto release = [&]() {  // the issuer lives in the leader: its barrier from either CTA
       tc_fence_before_sync();
       __syncwarp();
-      // the MMA issuer lives in the leader: signal its barrier from either CTA
       if (lane == 0) mbar_arrive_cluster(leader_acc_empty + static_cast<uint32_t>(acc) * 8u);
       if (++acc == ACC_STAGES) {
         acc = 0;
         acc_phase ^= 1u;
       }
+    };
+    for (long long idx = pair; ok && walker.get(idx, u); idx += pairs) {
+      const int in_tile = static_cast<int>(rank) * HALF + quarter * 32;
+      const int first_row = u.mi * TILE + in_tile;
+      const int row = first_row + lane;
+      const bool row_ok = row < p.m;
+      const int col = u.ni * TILE + half * HALF;
+      if (kiters == 0) {  // no token counts: the weight's gradient is zero
+        if (KIND == GRAD_WEIGHT) epilogue_grad_weight(p, &tm_c, 0, my_stage, issued, first_row, row, row_ok, col, lane, true);
+        continue;
+      }
+      if (KIND == STATS) {
+        // The tensor core's sums lose about half a step per addition, always towards zero: over a whole row of 4096 that is
+        // 2.5e-6 of the loss against 5e-7 in FP32. So PROMOTE k-blocks at a time are added up in registers.
+        float v[HALF];
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) v[j] = 0.0f;
+        for (int first = 0; first < kiters; first += CHAIN) {
+          if (!filled()) break;
+          const uint32_t taddr = lane_base + static_cast<uint32_t>(acc * TILE);
+#pragma unroll
+          for (int c = 0; c < HALF; c += 32) {
+            uint32_t raw[32];
+            tmem_ld_32x32(taddr + c, raw);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[c + j] += __uint_as_float(raw[j]);
+          }
+          release();
+        }
+        if (ok && row_ok) epilogue_stats(p, v, row, col, 2 * u.ni + half);
+        __syncwarp();
+        continue;
+      }
+      if (!filled()) break;
+      const uint32_t taddr = lane_base + static_cast<uint32_t>(acc * TILE);
+      if (KIND == PROBS) epilogue_probs(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane);
+      if (KIND == GRAD_HIDDEN) {
+        if (u.part >= 0) epilogue_part(p, taddr, u.part, in_tile + lane, row_ok, half);
+        else epilogue_grad_hidden(p, taddr, row, row_ok, col);
+      }
+      if (KIND == GRAD_WEIGHT)
+        epilogue_grad_weight(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane, false);
+      release();
     }
     if (issued > 0 && lane == 0) bulk_wait_all();  // this thread's stores are in global memory
   }
@@ -446,8 +554,252 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   }
 }
 
+// ------------------------------------------------------------------------------------------- few tokens
+// Up to 128 tokens: the weight's rows take the M side of the tile and the tokens N = 32, 64 or 128 columns, so that the tensor
+// cores do a fraction of a 256 x 256 tile's work beside the one pass over the weight, which is the bound (scoring of 16
+// tokens of 4096 over 131072 words: 1.07 GB). An accumulator row is a word: the sums over words run across the lanes of a warp.
+template <int N>
+struct Few {
+  static constexpr int B_BYTES = N / 2 * 128;                  // tokens' k-block that a CTA loads
+  static constexpr int STAGE = A_TILE_BYTES + B_BYTES;
+  static constexpr int STAGES = N == 32 ? 12 : N == 64 ? 10 : 8;
+  static constexpr int SMEM = STAGES * STAGE + 1024 + 512;
+  static constexpr int WARPS = N == 32 ? 4 : 8;                // epilogue: 32 columns at least per warp
+  static constexpr int COLS = N * 4 / WARPS;                   // columns per warp
+  static constexpr int THREADS = 64 + 32 * WARPS;
+};
+
+// The reduction over a warp's lanes of each of C columns (halving: a lane hands half of its columns to its partner and
+// takes the partner's values of the other half); column lane * (C / 32) + i ends in out[i].
+template <int C, bool MAX>
+__device__ __forceinline__ void reduce_columns(const float (&v)[C], float (&out)[C / 32], int lane) {
+  float w[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) w[i] = v[i];
+#pragma unroll
+  for (int s = 0; s < 5; ++s) {
+    const int half = C >> (s + 1);
+    const bool upper = (lane & (16 >> s)) != 0;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float keep = upper ? w[i + half] : w[i], send = upper ? w[i] : w[i + half];
+      const float other = __shfl_xor_sync(0xffffffffu, send, 16 >> s);
+      w[i] = MAX ? fmaxf(keep, other) : keep + other;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C / 32; ++i) out[i] = w[i];
+}
+
+template <int N>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Few<N>::THREADS, 1)
+few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_constant__ CUtensorMap tm_tokens, int vocab, int kiters,
+                  const int* __restrict__ count, const int* __restrict__ labels, float2* __restrict__ partial, long long pitch,
+                  float* __restrict__ target_logit, int* status) {
+  using F = Few<N>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::STAGES * F::STAGE);
+  uint64_t* full_bar = bars;                             // leader only: the loads of both CTAs
+  uint64_t* empty_bar = bars + F::STAGES;                // one set per CTA
+  uint64_t* acc_full_bar = bars + 2 * F::STAGES;         // one set per CTA
+  uint64_t* acc_empty_bar = acc_full_bar + ACC_STAGES;   // leader only
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty_bar + ACC_STAGES);
+  volatile int* abort_word = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = (vocab + TILE - 1) / TILE;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < F::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int s = 0; s < ACC_STAGES; ++s) {
+      mbar_init(&acc_full_bar[s], 1);
+      mbar_init(&acc_empty_bar[s], 2 * F::WARPS);  // every epilogue warp of both CTAs
+    }
+    *abort_word = 0;
+    mbar_fence_init();
+    prefetch_tensormap(&tm_words);
+    prefetch_tensormap(&tm_tokens);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA signal
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const int rows = *count;
+  const int last = rows > 0 ? tiles : 0;  // no token counts: nothing to do
+
+  if (warp == 0) {
+    // ======================================================================== TMA producer (both CTAs)
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < last; t += pairs) {
+        const int word = t * TILE + static_cast<int>(rank) * HALF;
+        for (int kb = 0; kb < kiters; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
+            report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 0, stage, kb);
+            ok = false;
+            break;
+          }
+          uint8_t* a_dst = smem + stage * F::STAGE;
+          // the leader's barrier counts the bytes of both CTAs
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * F::STAGE);
+          tma_load_2d_pair(a_dst, &tm_words, &full_bar[stage], kb * BK, word);
+          tma_load_2d_pair(a_dst + A_TILE_BYTES, &tm_tokens, &full_bar[stage], kb * BK, static_cast<int>(rank) * (N / 2));
+          if (++stage == F::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ======================================================================== MMA issuer (leader only)
+    if (rank == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      constexpr uint32_t idesc = make_idesc_f32acc(1u, TILE, N, HMC_MAJOR_K, HMC_MAJOR_K);
+      for (int t = pair; ok && t < last; t += pairs) {
+        for (int first = 0; ok && first < kiters; first += PROMOTE) {
+          const int end = min(kiters, first + PROMOTE);
+          if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
+            if (lane == 0) report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 1, acc, 0);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          for (int kb = first; kb < end; ++kb) {
+            if (!mbar_wait(&full_bar[stage], phase, abort_word, PIPE_BUDGET_NS)) {
+              if (lane == 0) report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 2, stage, kb);
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            if (lane == 0) {
+              uint8_t* a_src = smem + stage * F::STAGE;
+              uint64_t da = make_smem_desc(smem_u32(a_src), 16, 1024, SWIZZLE_128B);
+              uint64_t db = make_smem_desc(smem_u32(a_src + A_TILE_BYTES), 16, 1024, SWIZZLE_128B);
+#pragma unroll
+              for (int ks = 0; ks < BK / 16; ++ks) {
+                umma_bf16_pair(tmem_base + static_cast<uint32_t>(acc * N), da, db, idesc, (kb > first || ks > 0) ? 1u : 0u);
+                da += 32 >> 4;
+                db += 32 >> 4;
+              }
+              umma_commit_pair(&empty_bar[stage]);  // frees the slot in both CTAs
+              if (kb == end - 1) umma_commit_pair(&acc_full_bar[acc]);
+            }
+            __syncwarp();
+            if (++stage == F::STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          if (++acc == ACC_STAGES) {
+            acc = 0;
+            acc_phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else {
+    // ======================================================================== epilogue (both CTAs)
+    constexpr int C = F::COLS, OWN = C / 32;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    const int quarter = warp & 3;
+    const int col = (warp - 2) / 4 * C;  // this warp's first token
+    const uint32_t leader_acc_empty = map_to_cta(smem_u32(acc_empty_bar), 0);
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(col);
+    float top[OWN], sum[OWN];  // of column lane * OWN + i over this warp's words so far
+    int label[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      top[i] = -INFINITY, sum[i] = 0.0f;
+      const int token = col + lane * OWN + i;
+      label[i] = token < rows ? labels[token] : -1;
+    }
+    for (int t = pair; ok && t < last; t += pairs) {
+      float v[C];
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] = 0.0f;
+      for (int first = 0; first < kiters; first += PROMOTE) {
+        if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_word, PIPE_BUDGET_NS)) {
+          if (lane == 0) report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 3, acc, 0);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < C; c += 32) {
+          uint32_t raw[32];
+          tmem_ld_32x32(lane_base + static_cast<uint32_t>(acc * N + c), raw);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[c + j] += __uint_as_float(raw[j]);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(leader_acc_empty + static_cast<uint32_t>(acc) * 8u);
+        if (++acc == ACC_STAGES) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      const int word = t * TILE + static_cast<int>(rank) * HALF + quarter * 32 + lane;
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        if (word >= vocab) v[j] = -INFINITY;
+        if (__shfl_sync(0xffffffffu, label[j % OWN], j / OWN) == word) target_logit[col + j] = v[j];
+      }
+      float high[OWN], part[OWN];
+      reduce_columns<C, true>(v, high, lane);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) high[i] = fmaxf(high[i], top[i]);
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const float most = __shfl_sync(0xffffffffu, high[j % OWN], j / OWN);
+        v[j] = shifted_exp(v[j], most == -INFINITY ? 0.0f : most);
+      }
+      reduce_columns<C, false>(v, part, lane);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        sum[i] = sum[i] * shifted_exp(top[i], high[i] == -INFINITY ? 0.0f : high[i]) + part[i];
+        top[i] = high[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int token = col + lane * OWN + i;
+      if (token < rows) partial[(static_cast<long long>(blockIdx.x) * 4 + quarter) * pitch + token] = make_float2(top[i], sum[i]);
+    }
+  }
+
+  // Teardown: no CTA may leave while its partner can still reach into its shared memory or TMEM.
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
 // ------------------------------------------------------------------------------------------- packing
-constexpr int PACK_TOKENS = 32;  // tokens per block
+constexpr int PACK_TOKENS = 8;  // tokens per block, one per warp
 constexpr int PACK_THREADS = 256;
 
 struct Targets {
@@ -486,12 +838,12 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
   for (long long i = threadIdx.x; i < first; i += PACK_THREADS) before += targets.at(i) != targets.ignored;
   before = block_count(before);
   if (threadIdx.x < 32) {
-    const long long i = first + threadIdx.x;
+    const long long i = threadIdx.x < PACK_TOKENS ? first + threadIdx.x : tokens;
     const long long target = i < tokens ? targets.at(i) : targets.ignored;
     const bool counts = i < tokens && target != targets.ignored;
     const unsigned mask = __ballot_sync(0xffffffffu, counts);
     const int at = before + __popc(mask & ((1u << threadIdx.x) - 1u));
-    place[threadIdx.x] = counts ? at : -1;
+    if (threadIdx.x < PACK_TOKENS) place[threadIdx.x] = counts ? at : -1;
     if (i < tokens) position[i] = counts ? at : -1;
     if (counts) {
       row_of[at] = static_cast<int>(i);
@@ -502,13 +854,14 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
   }
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int t = warp; t < PACK_TOKENS; t += PACK_THREADS / 32) {
-    if (place[t] < 0) continue;
-    const __nv_bfloat16* src = x + (first + t) * x_stride;
-    __nv_bfloat16* dst = packed + static_cast<long long>(place[t]) * hidden;
+  if (place[warp] >= 0) {
+    const __nv_bfloat16* src = x + (first + warp) * x_stride;
+    __nv_bfloat16* dst = packed + static_cast<long long>(place[warp]) * hidden;
     if (vector) {
-      for (int c = lane * 8; c < hidden; c += 256) st_16(dst + c, ld_16(src + c));
+#pragma unroll 8
+      for (int c = lane * 8; c < hidden; c += 256) st_16(dst + c, ld_nc_16(src + c));
     } else {
+#pragma unroll 8
       for (int c = lane; c < hidden; c += 32) dst[c] = src[c];
     }
   }
@@ -540,11 +893,19 @@ __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __
   const bool ok = row < *count;
   float top = -INFINITY, sum = 0.0f;
   if (ok) {
-    // without a branch per part, so that several loads are in flight
-    for (int i = threadIdx.y; i < parts; i += JOIN_SLICES) {
-      const float2 part = partial[i * pitch + row];
-      const float high = fmaxf(top, part.x), shift = high == -INFINITY ? 0.0f : high;
-      sum = sum * shifted_exp(top, shift) + part.y * shifted_exp(part.x, shift);
+    constexpr int AHEAD = 4;  // parts loaded together
+    for (int i = threadIdx.y; i < parts; i += AHEAD * JOIN_SLICES) {
+      float2 part[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a)
+        part[a] = i + a * JOIN_SLICES < parts ? partial[(i + a * JOIN_SLICES) * pitch + row] : make_float2(-INFINITY, 0.0f);
+      float high = top;
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) high = fmaxf(high, part[a].x);
+      const float shift = high == -INFINITY ? 0.0f : high;
+      sum *= shifted_exp(top, shift);
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) sum += part[a].y * shifted_exp(part[a].x, shift);
       top = high;
     }
   }
@@ -607,9 +968,30 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
   }
 }
 
-// word_sums[first row of a word] = sum of coef_i x_i over the rows with that word as target, in their order. A block per row and
-// 1024 columns; rows that are not the first of their word have nothing to do.
-constexpr int WORD_THREADS = 128;
+// The sum of coef_i x_i over the rows that have a word as target, in their order, in slices of WORD_SLICE rows of a word:
+// every row that is the first of a slice adds up its slice, into word_sums at its own row. (One block for all rows of a word
+// took 390 us for 8192 tokens drawn by a power law: the commonest word had 480 of them.)
+constexpr int WORD_THREADS = 256;
+constexpr int WORD_SLICE = 32;
+
+// Number of set `match`es in the block; place: those before this thread's.
+__device__ __forceinline__ int matches(bool match, int& place) {
+  __shared__ int found[WORD_THREADS / 32];
+  const unsigned mask = __ballot_sync(0xffffffffu, match);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) found[warp] = __popc(mask);
+  __syncthreads();
+  int total = 0;
+  place = __popc(mask & ((1u << lane) - 1u));
+#pragma unroll
+  for (int w = 0; w < WORD_THREADS / 32; ++w) {
+    place += w < warp ? found[w] : 0;
+    total += found[w];
+  }
+  __syncthreads();
+  return total;
+}
+
 __global__ void __launch_bounds__(WORD_THREADS) word_sums_kernel(const __nv_bfloat16* __restrict__ packed, int hidden,
                                                                  const int* __restrict__ count,
                                                                  const int* __restrict__ labels,
@@ -617,54 +999,94 @@ __global__ void __launch_bounds__(WORD_THREADS) word_sums_kernel(const __nv_bflo
                                                                  const unsigned* __restrict__ slots,
                                                                  const int* __restrict__ members,
                                                                  float* __restrict__ word_sums) {
-  __shared__ int found[WORD_THREADS];
-  __shared__ int warp_found[WORD_THREADS / 32];
+  __shared__ int slice[WORD_SLICE];
+  const int rows = *count;
+  const int row = blockIdx.x;
+  if (row >= rows) return;
+  const int label = labels[row];
+  if (label < 0) return;
+  const int first = static_cast<int>(slots[label]);
+  const int all = members[label] + 1;
+  int place, before = 0;
+  if (row != first) {
+    if (all <= WORD_SLICE) return;
+    for (int base = first; base < row; base += WORD_THREADS) {  // rows of this word before this one
+      const int at = base + threadIdx.x;
+      before += matches(at < row && labels[at] == label, place);
+    }
+    if (before % WORD_SLICE != 0) return;
+  }
+  const int want = min(WORD_SLICE, all - before);
+  if (threadIdx.x == 0) slice[0] = row;
+  int have = 1;
+  for (int base = row + 1; have < want && base < rows; base += WORD_THREADS) {
+    const int at = base + threadIdx.x;
+    const bool match = at < rows && labels[at] == label;
+    const int found = matches(match, place);
+    if (match && have + place < want) slice[have + place] = at;
+    have += found;
+  }
+  __syncthreads();
+  const int n = min(have, want);
+  for (int col = threadIdx.x * 8; col < hidden; col += WORD_THREADS * 8) {
+    float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const int from = slice[i];
+      const float c = coef[from];
+      const uint4 q = ld_16(packed + static_cast<long long>(from) * hidden + col);
+      const uint32_t parts[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack_bf16x2(parts[e]);
+        sum[2 * e] += c * f.x;
+        sum[2 * e + 1] += c * f.y;
+      }
+    }
+    float* dst = word_sums + static_cast<long long>(row) * hidden + col;
+    *reinterpret_cast<float4*>(dst) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    *reinterpret_cast<float4*>(dst + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+  }
+}
+
+// The slices of a word in their order, into the first one's place.
+__global__ void __launch_bounds__(WORD_THREADS) word_slices_kernel(int hidden, const int* __restrict__ count,
+                                                                   const int* __restrict__ labels,
+                                                                   const unsigned* __restrict__ slots,
+                                                                   const int* __restrict__ members,
+                                                                   float* __restrict__ word_sums) {
+  __shared__ int starts[WORD_THREADS];
   const int rows = *count;
   const int row = blockIdx.x;
   if (row >= rows) return;
   const int label = labels[row];
   if (label < 0 || slots[label] != static_cast<unsigned>(row)) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col = (blockIdx.y * WORD_THREADS + threadIdx.x) * 8;
-  const bool col_ok = col < hidden;
-  float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  int left = members[label] + 1;
-  for (int base = row; left > 0 && base < rows; base += WORD_THREADS) {
+  const int all = members[label] + 1;
+  if (all <= WORD_SLICE) return;
+  const int col = (blockIdx.y * WORD_THREADS + threadIdx.x) * 4;
+  float* mine = word_sums + static_cast<long long>(row) * hidden + col;
+  float4 sum = col < hidden ? *reinterpret_cast<const float4*>(mine) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  int seen = 1;
+  for (int base = row + 1; seen < all && base < rows; base += WORD_THREADS) {
     const int at = base + threadIdx.x;
     const bool match = at < rows && labels[at] == label;
-    const unsigned mask = __ballot_sync(0xffffffffu, match);
-    if (lane == 0) warp_found[warp] = __popc(mask);
+    int place;
+    const int found = matches(match, place);
+    // slices start at every WORD_SLICE-th row of the word
+    const int from = (seen + WORD_SLICE - 1) / WORD_SLICE, to = (seen + found + WORD_SLICE - 1) / WORD_SLICE;
+    if (match && (seen + place) % WORD_SLICE == 0) starts[(seen + place) / WORD_SLICE - from] = at;
     __syncthreads();
-    int place = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < WORD_THREADS / 32; ++w) {
-      if (w < warp) place += warp_found[w];
-      total += warp_found[w];
-    }
-    if (match) found[place + __popc(mask & ((1u << lane) - 1u))] = at;
-    __syncthreads();
-    if (col_ok) {
+    if (col < hidden) {
 #pragma unroll 4
-      for (int i = 0; i < total; ++i) {
-        const int from = found[i];
-        const float c = coef[from];
-        const uint4 q = ld_16(packed + static_cast<long long>(from) * hidden + col);
-        const uint32_t parts[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack_bf16x2(parts[e]);
-          sum[2 * e] += c * f.x;
-          sum[2 * e + 1] += c * f.y;
-        }
+      for (int i = 0; i < to - from; ++i) {
+        const float4 q = *reinterpret_cast<const float4*>(word_sums + static_cast<long long>(starts[i]) * hidden + col);
+        sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
       }
     }
-    left -= total;
+    seen += found;
     __syncthreads();
   }
-  if (!col_ok) return;
-  float* dst = word_sums + static_cast<long long>(row) * hidden + col;
-  *reinterpret_cast<float4*>(dst) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-  *reinterpret_cast<float4*>(dst + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+  if (col < hidden) *reinterpret_cast<float4*>(mine) = sum;
 }
 
 __global__ void __launch_bounds__(128) zero_ignored_kernel(const int* __restrict__ position, int hidden,
@@ -718,13 +1140,20 @@ int map_store(CUtensorMap* map, const void* base, long long width, long long row
 
 long long tiles_of(long long v) { return (v + TILE - 1) / TILE; }
 
+// Tiles of a launch that may be cut along k, and the sums they leave: see Walker.
+long long cut_tiles(long long tiles) {
+  const long long pairs = sm_count() / 2;
+  return tiles < pairs ? tiles : pairs - 1;
+}
+
 template <Product KIND>
 int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const Params& p, long long tiles,
                    cudaStream_t stream) {
   static PerDeviceFlag configured{};
   if (int rc = allow_dynamic_smem(head_gemm_kernel<KIND>, SMEM_BYTES, configured)) return rc;
   const long long most = sm_count() / 2;
-  const int grid = static_cast<int>(2 * (tiles < most ? tiles : most));
+  // a product that is cut along k may have more units than tiles
+  const int grid = static_cast<int>(2 * (KIND == GRAD_HIDDEN || tiles > most ? most : tiles));
   head_gemm_kernel<KIND><<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(a, b, c, p);
   HMC_LAUNCH_OK();
   return 0;
@@ -752,6 +1181,28 @@ struct State {
   }
 };
 
+constexpr long long FEW_TOKENS = 128;
+
+// Parts that a launch over `vocab` words leaves per token: one per epilogue warp and column, or two per tile.
+long long few_parts(long long vocab) {
+  const long long pairs = sm_count() / 2, tiles = tiles_of(vocab);
+  return 8 * (tiles < pairs ? tiles : pairs);
+}
+
+template <int N>
+int launch_few(const CUtensorMap& words, const State& st, long long hidden, long long tokens, const Params& p, int* parts,
+               cudaStream_t stream) {
+  CUtensorMap rows;
+  if (int rc = make_map(&rows, st.packed, hidden, tokens, hidden, BK, N / 2, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  static PerDeviceFlag configured{};
+  if (int rc = allow_dynamic_smem(few_tokens_kernel<N>, Few<N>::SMEM, configured)) return rc;
+  *parts = static_cast<int>(few_parts(p.n));
+  few_tokens_kernel<N><<<*parts / 4, Few<N>::THREADS, Few<N>::SMEM, stream>>>(words, rows, p.n, (p.k + BK - 1) / BK, p.count, p.labels,
+                                                                          p.partial, p.pitch, p.target_logit, p.status);
+  HMC_LAUNCH_OK();
+  return 0;
+}
+
 // A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size.
 constexpr long long PIECE_BYTES = 512ll << 20;
 long long piece_words(long long tokens, long long vocab) {
@@ -762,7 +1213,7 @@ long long piece_words(long long tokens, long long vocab) {
 }
 
 struct GradSpace {
-  float *scale, *weights, *coef, *word_sums, *sums;
+  float *scale, *weights, *coef, *word_sums, *sums, *part_sums;
   unsigned* slots;
   int* members;
   __nv_bfloat16* probs;
@@ -783,6 +1234,7 @@ struct GradSpace {
     slot_bytes = reinterpret_cast<char*>(members) - reinterpret_cast<char*>(slots) + 4 * vocab;
     word_sums = reinterpret_cast<float*>(take(4 * tokens * hidden));
     sums = piece < vocab ? reinterpret_cast<float*>(take(4 * tokens * hidden)) : nullptr;
+    part_sums = reinterpret_cast<float*>(take(2ll * (sm_count() / 2) * TILE * TILE * 4));
     probs = reinterpret_cast<__nv_bfloat16*>(take(2 * tokens * piece));
     bytes = at;
   }
@@ -812,7 +1264,10 @@ extern "C" int64_t hmc_vocab_loss_state_bytes(int64_t tokens, int64_t hidden) {
 
 extern "C" int64_t hmc_vocab_loss_workspace_bytes(int64_t tokens, int64_t vocab) {
   using namespace hmc;
-  return tokens > 0 && vocab > 0 ? up256(4 * tokens) + 2 * tiles_of(vocab) * tokens * 8 : 0;
+  if (tokens <= 0 || vocab <= 0) return 0;
+  // of the most parts that any smaller call leaves too
+  const long long parts = 2 * tiles_of(vocab) > few_parts(vocab) ? 2 * tiles_of(vocab) : few_parts(vocab);
+  return up256(4 * tokens) + parts * tokens * 8;
 }
 
 extern "C" int64_t hmc_vocab_loss_grad_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab) {
@@ -846,11 +1301,20 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
   p.n = static_cast<int>(vocab), p.k = static_cast<int>(hidden);
   p.count = st.count, p.labels = st.labels, p.partial = partial, p.pitch = tokens, p.target_logit = target_logit, p.status = status;
   CUtensorMap a, b;
-  if (int rc = map_k_major(&a, st.packed, hidden, tokens, hidden)) return rc;
   if (int rc = map_k_major(&b, weight, hidden, vocab, weight_stride)) return rc;
-  if (int rc = launch_product<STATS>(a, b, a, p, tiles_of(tokens) * tiles_of(vocab), s)) return rc;
+  int parts = 0;
+  if (tokens <= FEW_TOKENS) {
+    const int rc = tokens <= 32   ? launch_few<32>(b, st, hidden, tokens, p, &parts, s)
+                   : tokens <= 64 ? launch_few<64>(b, st, hidden, tokens, p, &parts, s)
+                                  : launch_few<128>(b, st, hidden, tokens, p, &parts, s);
+    if (rc != 0) return rc;
+  } else {
+    if (int rc = map_k_major(&a, st.packed, hidden, tokens, hidden)) return rc;
+    if (int rc = launch_product<STATS>(a, b, a, p, tiles_of(tokens) * tiles_of(vocab), s)) return rc;
+    parts = static_cast<int>(2 * tiles_of(vocab));
+  }
   join_kernel<<<static_cast<unsigned>((tokens + 31) / 32), dim3(32, JOIN_SLICES), 0, s>>>(
-      partial, tokens, static_cast<int>(2 * tiles_of(vocab)), st.count, st.labels, st.row_of, target_logit, st.lse, st.losses,
+      partial, tokens, parts, st.count, st.labels, st.row_of, target_logit, st.lse, st.losses,
       token_loss);
   HMC_LAUNCH_OK();
   if (reduction != HMC_REDUCE_NONE) {
@@ -884,9 +1348,14 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
       grad_weight != nullptr ? w.slots : nullptr, w.members);
   HMC_LAUNCH_OK();
   if (grad_weight != nullptr) {
-    const dim3 grid(static_cast<unsigned>(tokens), (width / 8 + WORD_THREADS - 1) / WORD_THREADS);
-    word_sums_kernel<<<grid, WORD_THREADS, 0, s>>>(st.packed, width, st.count, st.labels, w.coef, w.slots, w.members, w.word_sums);
+    word_sums_kernel<<<static_cast<unsigned>(tokens), WORD_THREADS, 0, s>>>(st.packed, width, st.count, st.labels, w.coef,
+                                                                           w.slots, w.members, w.word_sums);
     HMC_LAUNCH_OK();
+    if (tokens > WORD_SLICE) {
+      const dim3 grid(static_cast<unsigned>(tokens), (width / 4 + WORD_THREADS - 1) / WORD_THREADS);
+      word_slices_kernel<<<grid, WORD_THREADS, 0, s>>>(width, st.count, st.labels, w.slots, w.members, w.word_sums);
+      HMC_LAUNCH_OK();
+    }
   }
   if (grad_hidden != nullptr) {
     zero_ignored_kernel<<<static_cast<unsigned>(tokens), 128, 0, s>>>(st.position, width, static_cast<__nv_bfloat16*>(grad_hidden));
@@ -916,7 +1385,11 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
       p.sums = w.sums, p.add = first > 0, p.last = first + words == vocab;
       p.head = static_cast<const __nv_bfloat16*>(weight), p.head_stride = weight_stride;
       p.out = static_cast<__nv_bfloat16*>(grad_hidden);
-      if (int rc = launch_product<GRAD_HIDDEN>(probs_k, head_mn, probs_k, p, tiles_of(tokens) * tiles_of(width), s)) return rc;
+      p.part_sums = w.part_sums;
+      const long long tiles = tiles_of(tokens) * tiles_of(width);
+      if (int rc = launch_product<GRAD_HIDDEN>(probs_k, head_mn, probs_k, p, tiles, s)) return rc;
+      join_parts_kernel<<<dim3(TILE / 8, static_cast<unsigned>(cut_tiles(tiles))), 256, 0, s>>>(p, sm_count() / 2);
+      HMC_LAUNCH_OK();
     }
     if (grad_weight != nullptr) {
       CUtensorMap grad_store;
