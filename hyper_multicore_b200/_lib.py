@@ -463,15 +463,22 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)  # pylint: disable=protected-access
 
 
+_FUNCTIONS: dict = {}
+
+
 def launch(name: str, device: torch.device, *args) -> None:
     """Call an entry point with torch's current stream on ``device`` as its last argument. The device guard costs several
     microseconds, more than the rest of the call, so it is left out where ``device`` is the current one already."""
-    function = getattr(load(), name)
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(function(*args, stream_ptr(device)))
+    function = _FUNCTIONS.get(name)
+    if function is None:
+        function = _FUNCTIONS[name] = getattr(load(), name)
+    if device.index is None or device.index == torch._C._cuda_getDevice():  # pylint: disable=protected-access
+        code = function(*args, stream_ptr(device))
     else:
         with torch.cuda.device(device):
-            check(function(*args, stream_ptr(device)))
+            code = function(*args, stream_ptr(device))
+    if code != 0:
+        check(code)
 
 
 def new_status(device: torch.device) -> torch.Tensor:

@@ -7,6 +7,7 @@ checks, and enqueues on torch's current stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -756,39 +757,50 @@ def mx_pack_weight_scale(scale: torch.Tensor, axis: int, experts: int, m: int, n
 
 
 # ------------------------------------------------------------------------------- norms and the vocabulary
+@functools.lru_cache(maxsize=256)
+def _size(name: str, *extents: int) -> int:
+    """What a ``..._bytes`` entry point says; it depends on the extents alone."""
+    return getattr(_lib.load(), name)(*extents)
+
+
 def row_norm(x, weight, bias, *, center: bool, eps: float, keep: bool):
     """Layer norm (``center``) or RMSNorm of the rows of ``x`` [T, H] (rows any distance apart, values adjacent).
 
-    Returns (y [T, H], mean [T] | None, rstd [T] | None); the statistics, FP32, only with ``keep``.
+    Returns (y [T, H], stats | None): with ``keep`` the FP32 statistics, rstd [T] behind mean [T] where there is one.
     """
     device = _require_cuda(x, weight, bias)
     rows, hidden = x.shape
-    y = torch.empty((rows, hidden), dtype=x.dtype, device=device)
-    mean = rstd = None
+    dtype = x.dtype
+    y = torch.empty((rows, hidden), dtype=dtype, device=device)
+    stats = mean = rstd = None
     if keep:
-        stats = torch.empty((2 if center else 1, rows), dtype=torch.float32, device=device)
-        mean, rstd = (stats[0], stats[1]) if center else (None, stats[0])
-    affine = weight if weight is not None else bias
-    _call("hmc_row_norm", device, x.data_ptr(), x.stride(0), rows, hidden, _lib.HMC_DTYPE[x.dtype], _lib.ptr(weight),
-          _lib.ptr(bias), _lib.HMC_DTYPE[x.dtype if affine is None else affine.dtype], int(center), eps, y.data_ptr(),
-          _lib.ptr(mean), _lib.ptr(rstd))
-    return y, mean, rstd
+        stats = torch.empty(2 * rows if center else rows, dtype=torch.float32, device=device)
+        rstd = stats.data_ptr()
+        if center:
+            mean, rstd = rstd, rstd + 4 * rows
+    affine = dtype if weight is None and bias is None else bias.dtype if weight is None else weight.dtype
+    _call("hmc_row_norm", device, x.data_ptr(), x.stride(0), rows, hidden, _lib.HMC_DTYPE[dtype], _lib.ptr(weight), _lib.ptr(bias),
+          _lib.HMC_DTYPE[affine], center, eps, y.data_ptr(), mean, rstd)
+    return y, stats
 
 
-def row_norm_grad(grad, x, weight, mean, rstd, *, affine_dtype, need_x: bool, need_weight: bool, need_bias: bool):
-    """Gradients of ``row_norm`` (``mean`` None: RMSNorm): (grad_x [T, H], grad_weight [H], grad_bias [H]), None where not needed."""
-    device = _require_cuda(grad, x, weight, mean, rstd)
+def row_norm_grad(grad, x, weight, stats, *, center: bool, affine_dtype, need_x: bool, need_weight: bool, need_bias: bool):
+    """Gradients of ``row_norm``: (grad_x [T, H], grad_weight [H], grad_bias [H]), None where not needed."""
+    device = _require_cuda(grad, x, weight, stats)
     rows, hidden = x.shape
     grad_x = torch.empty((rows, hidden), dtype=x.dtype, device=device) if need_x else None
     grad_weight = torch.empty(hidden, dtype=affine_dtype, device=device) if need_weight else None
     grad_bias = torch.empty(hidden, dtype=affine_dtype, device=device) if need_bias else None
     need, workspace = 0, None
     if need_weight or need_bias:
-        need = _lib.load().hmc_row_norm_grad_workspace_bytes(rows, hidden)
+        need = _size("hmc_row_norm_grad_workspace_bytes", rows, hidden)
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    rstd, mean = stats.data_ptr(), None
+    if center:
+        mean, rstd = rstd, rstd + 4 * rows
     _call("hmc_row_norm_grad", device, x.data_ptr(), x.stride(0), grad.data_ptr(), grad.stride(0), rows, hidden,
-          _lib.HMC_DTYPE[x.dtype], _lib.ptr(weight), _lib.HMC_DTYPE[affine_dtype], int(mean is not None), _lib.ptr(mean),
-          _lib.ptr(rstd), _lib.ptr(grad_x), _lib.ptr(grad_weight), _lib.ptr(grad_bias), _lib.ptr(workspace), need)
+          _lib.HMC_DTYPE[x.dtype], _lib.ptr(weight), _lib.HMC_DTYPE[affine_dtype], center, mean, rstd, _lib.ptr(grad_x),
+          _lib.ptr(grad_weight), _lib.ptr(grad_bias), _lib.ptr(workspace), need)
     return grad_x, grad_weight, grad_bias
 
 
@@ -796,13 +808,12 @@ def vocab_loss(x, weight, targets, *, ignore_index: int, reduction: str, status=
     """Cross entropy of ``x`` [T, H] against ``weight`` [V, H] and ``targets`` [T]: (loss [T] or [], state for the gradient)."""
     device = _require_cuda(x, weight, targets)
     (tokens, hidden), vocab = x.shape, weight.shape[0]
-    lib = _lib.load()
     loss = torch.empty((tokens,) if reduction == "none" else (), dtype=torch.float32, device=device)
-    state = torch.empty(lib.hmc_vocab_loss_state_bytes(tokens, hidden), dtype=torch.uint8, device=device)
-    need = lib.hmc_vocab_loss_workspace_bytes(tokens, vocab)
+    state = torch.empty(_size("hmc_vocab_loss_state_bytes", tokens, hidden), dtype=torch.uint8, device=device)
+    need = _size("hmc_vocab_loss_workspace_bytes", tokens, vocab)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _call("hmc_vocab_loss", device, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), targets.data_ptr(),
-          int(targets.dtype == torch.int64), tokens, hidden, vocab, ignore_index, _lib.HMC_REDUCE[reduction], state.data_ptr(),
+          targets.dtype == torch.int64, tokens, hidden, vocab, ignore_index, _lib.HMC_REDUCE[reduction], state.data_ptr(),
           loss.data_ptr(), workspace.data_ptr(), need, _lib.ptr(status))
     return loss, state
 
@@ -813,7 +824,7 @@ def vocab_loss_grad(grad_loss, state, weight, tokens: int, *, reduction: str, ne
     vocab, hidden = weight.shape
     grad_hidden = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=device) if need_hidden else None
     grad_weight = torch.empty((vocab, hidden), dtype=torch.bfloat16, device=device) if need_weight else None
-    need = _lib.load().hmc_vocab_loss_grad_workspace_bytes(tokens, hidden, vocab)
+    need = _size("hmc_vocab_loss_grad_workspace_bytes", tokens, hidden, vocab)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _call("hmc_vocab_loss_grad", device, state.data_ptr(), weight.data_ptr(), weight.stride(0), tokens, hidden, vocab,
           _lib.HMC_REDUCE[reduction], grad_loss.data_ptr(), _lib.ptr(grad_hidden), _lib.ptr(grad_weight), workspace.data_ptr(),

@@ -2,19 +2,35 @@
 
 from __future__ import annotations
 
+from collections.abc import Callable
+
 import torch
+from torch.autograd.function import once_differentiable
+
+_functorch = torch._C._functorch  # pylint: disable=protected-access
 
 
 def as_rows(tensor: torch.Tensor, width: int) -> torch.Tensor:
     """``tensor`` [..., width] as [rows, width] with adjacent values; rows may lie any distance apart, so that a slice of a
     wider buffer and a broadcast row are read in place."""
-    rows = tensor.resolve_neg().reshape(-1, width)
+    if tensor.is_neg():
+        tensor = tensor.resolve_neg()
+    rows = tensor if tensor.ndim == 2 else tensor.reshape(-1, width)
     return rows if width == 1 or rows.stride(1) == 1 else rows.contiguous()
 
 
 def plain_grad(grad: torch.Tensor, what: str) -> torch.Tensor:
-    """``grad`` as memory a kernel can read; a gradient batched by vmap (``is_grads_batched``) is refused."""
-    functorch = torch._C._functorch  # pylint: disable=protected-access
-    if functorch.is_legacy_batchedtensor(grad) or functorch.is_functorch_wrapped_tensor(grad):
+    """``grad``; one that is batched by vmap (``is_grads_batched``) and so no memory of its own is refused."""
+    if _functorch.is_legacy_batchedtensor(grad) or _functorch.is_functorch_wrapped_tensor(grad):
         raise RuntimeError(f"{what} does not take gradients batched by vmap (is_grads_batched); call its backward once each")
-    return grad.resolve_neg()
+    return grad
+
+
+def first_order(backward: Callable) -> Callable:
+    """``once_differentiable`` that costs nothing where no graph of the gradient is recorded."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run

@@ -9,13 +9,25 @@ import math
 from typing import Any
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib, kernels
-from ._rows import as_rows, plain_grad
+from ._rows import as_rows, first_order, plain_grad
+
+
+def _fits(hidden, weight, targets, ignore_index, reduction) -> bool:
+    """All of ``_validate`` in one expression, which builds no message; that one then says what is wrong."""
+    return (type(hidden) is torch.Tensor and hidden.is_cuda and hidden.ndim > 0 and hidden.dtype == torch.bfloat16
+            and isinstance(weight, torch.Tensor) and weight.ndim == 2 and weight.dtype == torch.bfloat16
+            and hidden.shape[-1] == weight.shape[1] and weight.shape[1] % 8 == 0 and 0 < weight.shape[1] < 1 << 30
+            and 0 < weight.shape[0] < (1 << 31) - 256 and weight.device == hidden.device
+            and isinstance(targets, torch.Tensor) and targets.dtype in (torch.int64, torch.int32)
+            and targets.shape == hidden.shape[:-1] and targets.device == hidden.device and targets.numel() < (1 << 31) - 256
+            and type(ignore_index) is int and -(1 << 63) <= ignore_index < 1 << 63 and reduction in _lib.HMC_REDUCE)
 
 
 def _validate(hidden, weight, targets, ignore_index, reduction) -> None:
+    if _fits(hidden, weight, targets, ignore_index, reduction):
+        return
     for name, tensor in (("hidden", hidden), ("weight", weight), ("targets", targets)):
         if not isinstance(tensor, torch.Tensor):
             raise TypeError(f"{name} must be a Tensor.")
@@ -44,7 +56,8 @@ def _validate(hidden, weight, targets, ignore_index, reduction) -> None:
 
 def _weight_rows(weight: torch.Tensor) -> torch.Tensor:
     """The weight in place where its rows are adjacent values that start on 16-byte boundaries, a copy otherwise."""
-    weight = weight.resolve_neg()
+    if weight.is_neg():
+        weight = weight.resolve_neg()
     one_row = weight.shape[0] == 1
     if (weight.stride(1) == 1 and (one_row or (weight.stride(0) % 8 == 0 and weight.stride(0) >= weight.shape[1]))
             and weight.data_ptr() % 16 == 0):
@@ -73,13 +86,13 @@ class _CrossEntropyFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad_loss):  # pylint: disable=arguments-differ
         state, weight = ctx.saved_tensors
         if ctx.tokens == 0:
             return (torch.empty((0, weight.shape[1]), dtype=torch.bfloat16, device=weight.device),
                     torch.zeros(weight.shape, dtype=torch.bfloat16, device=weight.device), None, None, None)
-        grad = plain_grad(grad_loss, "MegaCrossEntropy's backward").contiguous()
+        grad = plain_grad(grad_loss, "MegaCrossEntropy's backward").resolve_neg().contiguous()
         grad_hidden, grad_weight = kernels.vocab_loss_grad(grad, state, weight, ctx.tokens, reduction=ctx.reduction,
                                                            need_hidden=ctx.needs_input_grad[0], need_weight=ctx.needs_input_grad[1])
         return grad_hidden, grad_weight, None, None, None
@@ -97,14 +110,13 @@ def mega_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torc
     the gradients are BF16. The backward pass takes scratch of up to 512 MiB for probabilities and of up to 8 bytes per element of ``hidden``.
     """
     _validate(hidden, weight, targets, ignore_index, reduction)
-    shape = targets.shape
     rows = as_rows(hidden, weight.shape[1])
-    flat = targets.reshape(-1).contiguous()
+    flat = targets if targets.ndim == 1 and targets.is_contiguous() else targets.reshape(-1).contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         loss = _CrossEntropyFunction.apply(rows, weight, flat, ignore_index, reduction)
     else:
         loss = _forward(rows, _weight_rows(weight), flat, ignore_index, reduction)[0]
-    return loss.view(shape) if reduction == "none" else loss
+    return loss.view(targets.shape) if reduction == "none" and targets.ndim != 1 else loss
 
 
 class MegaCrossEntropy(torch.nn.Module):

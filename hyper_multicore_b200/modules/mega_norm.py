@@ -10,13 +10,29 @@ import math
 from typing import Any
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib, kernels
-from ._rows import as_rows, plain_grad
+from ._rows import as_rows, first_order, plain_grad
+
+
+def _fits(x, weight, bias, eps) -> bool:
+    """All of ``_validate`` in one expression, which builds no message; that one then says what is wrong."""
+    if type(x) is not torch.Tensor or not x.is_cuda or x.ndim == 0 or type(eps) is not float or not 0.0 <= eps < math.inf:
+        return False
+    shape, dtype, device = x.shape, x.dtype, x.device
+    hidden = shape[-1]
+    if not (1 <= hidden <= _lib.HMC_NORM_MAX_HIDDEN and x.numel() < hidden << 31 and dtype in _lib.HMC_DTYPE):
+        return False
+    for parameter in (weight, bias):
+        if parameter is not None and not (isinstance(parameter, torch.Tensor) and parameter.shape == shape[-1:]
+                                          and parameter.dtype in (dtype, torch.float32) and parameter.device == device):
+            return False
+    return weight is None or bias is None or weight.dtype == bias.dtype
 
 
 def _validate(x, weight, bias, eps) -> None:
+    if _fits(x, weight, bias, eps):
+        return
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a Tensor.")
     if x.dtype not in _lib.HMC_DTYPE:
@@ -47,36 +63,47 @@ def _validate(x, weight, bias, eps) -> None:
 
 
 class _RowNormFunction(torch.autograd.Function):
-    """Norm of [T, H] rows with its matching backward; first order."""
+    """Norm of rows with its matching backward; first order."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, center, eps):  # pylint: disable=arguments-differ
-        rows = as_rows(x, x.shape[-1])
-        w, b = (None if p is None else p.contiguous() for p in (weight, bias))
-        y, mean, rstd = kernels.row_norm(rows, w, b, center=center, eps=eps, keep=True)
-        ctx.save_for_backward(rows, w, mean, rstd)
-        ctx.shape = x.shape
-        ctx.affine_dtype = next((p.dtype for p in (weight, bias) if p is not None), x.dtype)
-        return y.view(x.shape)
+        y, rows, weight, bias, stats = _forward(x, weight, bias, center, eps, True)
+        ctx.save_for_backward(rows, weight, stats)
+        ctx.center, ctx.shape = center, x.shape
+        ctx.affine_dtype = x.dtype if weight is None and bias is None else bias.dtype if weight is None else weight.dtype
+        return y
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad):  # pylint: disable=arguments-differ
-        rows, weight, mean, rstd = ctx.saved_tensors
-        grad_rows = as_rows(plain_grad(grad, "a row norm's backward"), rows.shape[1])
+        rows, weight, stats = ctx.saved_tensors
         need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
+        grad = as_rows(plain_grad(grad, "a row norm's backward"), rows.shape[1])
         grad_x, grad_weight, grad_bias = kernels.row_norm_grad(
-            grad_rows, rows, weight, mean, rstd, affine_dtype=ctx.affine_dtype, need_x=need_x, need_weight=need_weight,
+            grad, rows, weight, stats, center=ctx.center, affine_dtype=ctx.affine_dtype, need_x=need_x, need_weight=need_weight,
             need_bias=need_bias)
-        return grad_x.view(ctx.shape) if need_x else None, grad_weight, grad_bias, None, None
+        if need_x and len(ctx.shape) != 2:
+            grad_x = grad_x.view(ctx.shape)
+        return grad_x, grad_weight, grad_bias, None, None
+
+
+def _forward(x, weight, bias, center, eps, keep):
+    """(y, x as rows, parameters as the kernel reads them, statistics)"""
+    rows = as_rows(x, x.shape[-1])
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    y, stats = kernels.row_norm(rows, weight, bias, center=center, eps=eps, keep=keep)
+    return y if x.ndim == 2 else y.view(x.shape), rows, weight, bias, stats
 
 
 def _norm(x, weight, bias, center, eps):
     _validate(x, weight, bias, eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _RowNormFunction.apply(x, weight, bias, center, float(eps))
-    w, b = (None if p is None else p.contiguous() for p in (weight, bias))
-    return kernels.row_norm(as_rows(x, x.shape[-1]), w, b, center=center, eps=float(eps), keep=False)[0].view(x.shape)
+    return _forward(x, weight, bias, center, float(eps), False)[0]
 
 
 def mega_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
