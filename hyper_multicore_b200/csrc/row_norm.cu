@@ -168,96 +168,6 @@ __global__ void __launch_bounds__(1024) long_row_norm_kernel(const T* __restrict
   }
 }
 
-// Gradient: a block walks the rows blockIdx.x, + gridDim.x, ...; its threads own columns, so that the parameters'
-// gradients stay in registers over all its rows and x and dy are read once. `partial_*` are [gridDim.x, hidden] in FP32.
-template <typename T, typename W, int VEC, int NV, bool CENTER>
-__global__ void __launch_bounds__(512) row_norm_grad_kernel(const T* __restrict__ x, long long x_stride,
-                                                            const T* __restrict__ grad, long long grad_stride, long long rows,
-                                                            int hidden, const W* __restrict__ weight,
-                                                            const float* __restrict__ mean_in,
-                                                            const float* __restrict__ rstd_in, T* __restrict__ grad_x,
-                                                            float* __restrict__ partial_weight,
-                                                            float* __restrict__ partial_bias) {
-  __shared__ float slots[2][2 * MAX_WARPS];
-  const int warps = blockDim.x >> 5;
-  const int packs = hidden / VEC;
-  const float scale = 1.0f / static_cast<float>(hidden);
-  Pack<W, VEC> w[NV];
-  float sum_weight[NV][VEC], sum_bias[CENTER ? NV : 1][VEC];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int at = j * blockDim.x + threadIdx.x;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[j].v[e] = narrow<W>(1.0f);
-      sum_weight[j][e] = 0.0f;
-      if (CENTER) sum_bias[j][e] = 0.0f;
-    }
-    if (at < packs && weight != nullptr) w[j] = load_pack<W, VEC>(weight + static_cast<long long>(at) * VEC);
-  }
-  int turn = 0;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
-    Pack<T, VEC> in[NV], dy[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int at = j * blockDim.x + threadIdx.x;
-      if (at < packs) {
-        in[j] = load_pack<T, VEC>(x + row * x_stride + static_cast<long long>(at) * VEC);
-        dy[j] = load_pack<T, VEC>(grad + row * grad_stride + static_cast<long long>(at) * VEC);
-      }
-    }
-    const float mean = CENTER ? mean_in[row] : 0.0f;
-    const float rstd = rstd_in[row];
-    float sums[2] = {0.0f, 0.0f};  // of g * u and of g
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (j * blockDim.x + threadIdx.x < packs) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float d = widen(dy[j].v[e]), u = (widen(in[j].v[e]) - mean) * rstd, g = d * widen(w[j].v[e]);
-          sums[0] += g * u;
-          sum_weight[j][e] += d * u;
-          if (CENTER) {
-            sums[1] += g;
-            sum_bias[j][e] += d;
-          }
-        }
-      }
-    row_sum(sums, slots[turn], warps);
-    const float along = sums[0] * scale, offset = sums[1] * scale;
-    if (grad_x != nullptr) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int at = j * blockDim.x + threadIdx.x;
-        if (at < packs) {
-          Pack<T, VEC> out;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float u = (widen(in[j].v[e]) - mean) * rstd, g = widen(dy[j].v[e]) * widen(w[j].v[e]);
-            float v = g - u * along;
-            if (CENTER) v -= offset;
-            out.v[e] = narrow<T>(v * rstd);
-          }
-          store_pack<T, VEC>(grad_x + row * hidden + static_cast<long long>(at) * VEC, out);
-        }
-      }
-    }
-  }
-  if (partial_weight == nullptr) return;
-  const long long base = static_cast<long long>(blockIdx.x) * hidden;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int at = j * blockDim.x + threadIdx.x;
-    if (at < packs) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        partial_weight[base + static_cast<long long>(at) * VEC + e] = sum_weight[j][e];
-        if (CENTER) partial_bias[base + static_cast<long long>(at) * VEC + e] = sum_bias[j][e];
-      }
-    }
-  }
-}
-
 // ------------------------------------------------------------------------------------------- many rows
 // 16 bytes of T as FP32 pairs: the arithmetic of the kernels below takes two values per instruction, because counted in
 // single ones it is longer than the memory's time (34 instructions per value in a first version, 123 us for 16384 rows of
@@ -339,24 +249,24 @@ __device__ __forceinline__ float2 madd2(float2 a, float2 b, float2 c) {
 constexpr int STREAM_THREADS = 512;
 constexpr int STREAM_WARPS = STREAM_THREADS / 32;
 
-// row_sum for at most STREAM_WARPS warps: every thread reads the slots four at a time, the unused ones are zero.
-template <int N>
+// row_sum for at most WARPS warps: every thread reads the slots four at a time, the unused ones are zero.
+template <int WARPS = STREAM_WARPS, int N>
 __device__ __forceinline__ void block_sum(float (&v)[N], float* slots) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
   if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) slots[i * STREAM_WARPS + (threadIdx.x >> 5)] = v[i];
+    for (int i = 0; i < N; ++i) slots[i * WARPS + (threadIdx.x >> 5)] = v[i];
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    float4 q[STREAM_WARPS / 4];
+    float4 q[WARPS / 4];
 #pragma unroll
-    for (int w = 0; w < STREAM_WARPS / 4; ++w) q[w] = reinterpret_cast<const float4*>(slots + i * STREAM_WARPS)[w];
+    for (int w = 0; w < WARPS / 4; ++w) q[w] = reinterpret_cast<const float4*>(slots + i * WARPS)[w];
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < STREAM_WARPS / 4; ++w) sum += (q[w].x + q[w].y) + (q[w].z + q[w].w);
+    for (int w = 0; w < WARPS / 4; ++w) sum += (q[w].x + q[w].y) + (q[w].z + q[w].w);
     v[i] = sum;
   }
 }
@@ -465,161 +375,13 @@ stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
   }
 }
 
-// The gradient over the same ring, ROWS rows of x and dy per stage. Threads own columns: the parameters' gradients stay in
-// registers over all rows of a block, so that x and dy are read once. So do g and u of the ROWS rows between the reduction
-// and dx: widening the packs a second time made a row cost 29 instructions per value (163 us for 16384 rows of 7168).
-template <typename T, typename W, int NV, int ROWS, int PITCH, bool CENTER>
-__global__ void __launch_bounds__(PITCH, STREAM_THREADS / PITCH)
-stream_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
-                        long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
-                        const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
-                        float* __restrict__ partial_bias) {
-  extern __shared__ uint4 ring_raw[];
-  constexpr int stages = GRAD_STAGES, SUMS = CENTER ? 2 * ROWS : ROWS;
-  __shared__ __align__(16) float slots[2][SUMS * STREAM_WARPS];
-  constexpr int PAIRS = Quad<T>::PAIRS, VEC = 2 * PAIRS;
-  constexpr int WIDTH = NV * PITCH;  // known at compile time: offsets in the ring cost no arithmetic
-  const int threads = blockDim.x;
-  const int packs = hidden / VEC;
-  const float scale = 1.0f / static_cast<float>(hidden);
-  uint4* ring = ring_raw + threadIdx.x;  // [stage][row][x, dy][NV][PITCH]
-  for (int i = threadIdx.x; i < SUMS * STREAM_WARPS; i += threads) slots[0][i] = slots[1][i] = 0.0f;
-  bool here[NV];
-  constexpr int QUADS = PAIRS / Quad<W>::PAIRS;  // 16-byte pieces of a pack's parameters, kept as they are
-  uint4 params[NV][QUADS];
-  float2 sum_weight[NV][PAIRS], sum_bias[CENTER ? NV : 1][PAIRS];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int at = j * threads + threadIdx.x;
-    here[j] = at < packs;
-#pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
-      sum_weight[j][i] = both(0.0f);
-      if (CENTER) sum_bias[j][i] = both(0.0f);
-    }
-    float2 ones[Quad<W>::PAIRS];
-#pragma unroll
-    for (int i = 0; i < Quad<W>::PAIRS; ++i) ones[i] = both(1.0f);
-#pragma unroll
-    for (int i = 0; i < QUADS; ++i)
-      params[j][i] = here[j] && weight != nullptr ? ld_16(weight + at * VEC + i * 2 * Quad<W>::PAIRS) : Quad<W>::narrow(ones);
-  }
-  const T *mine_x = x + threadIdx.x * VEC, *mine_grad = grad + threadIdx.x * VEC;
-  auto fetch = [&](long long first, int stage) {
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-      if (first + r < rows) {
-        const T *a = mine_x + (first + r) * x_stride, *d = mine_grad + (first + r) * grad_stride;
-        uint4* dst = ring + (stage * ROWS + r) * 2 * WIDTH;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if (here[j]) {
-            copy_async_16(dst + j * PITCH, a + j * threads * VEC);
-            copy_async_16(dst + WIDTH + j * PITCH, d + j * threads * VEC);
-          }
-      }
-    copy_async_commit();
-  };
-  const long long step = static_cast<long long>(ROWS) * gridDim.x;
-  for (int s = 0; s < stages - 1; ++s) fetch(ROWS * static_cast<long long>(blockIdx.x) + s * step, s);
-  __syncthreads();  // the slots are zero
-  int stage = 0, last = stages - 1, turn = 0;
-  float next_mean[ROWS], next_rstd[ROWS];
-  auto stats = [&](long long first) {  // a row that does not exist has scale 0 and adds nothing
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      next_mean[r] = CENTER && first + r < rows ? mean_in[first + r] : 0.0f;
-      next_rstd[r] = first + r < rows ? rstd_in[first + r] : 0.0f;
-    }
-  };
-  stats(ROWS * static_cast<long long>(blockIdx.x));
-  for (long long first = ROWS * static_cast<long long>(blockIdx.x); first < rows; first += step, turn ^= 1) {
-    float mean[ROWS], rstd[ROWS];
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) mean[r] = next_mean[r], rstd[r] = next_rstd[r];
-    stats(first + step);
-    fetch(first + (stages - 1) * step, last);
-    copy_async_wait<stages - 1>();
-    float2 u[ROWS][NV][PAIRS], g[ROWS][NV][PAIRS];
-    float2 along[ROWS], total[ROWS];  // sums of g u and of g
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) along[r] = total[r] = both(0.0f);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float2 w[PAIRS];
-#pragma unroll
-      for (int i = 0; i < QUADS; ++i) Quad<W>::widen(params[j][i], w + i * Quad<W>::PAIRS);
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const uint4* src = ring + ((stage * ROWS + r) * 2 * WIDTH + j * PITCH);
-        uint4 in = make_uint4(0, 0, 0, 0), dy = in;
-        if (here[j] && (r == 0 || first + r < rows)) in = src[0], dy = src[WIDTH];
-        Quad<T>::widen(in, u[r][j]);
-        Quad<T>::widen(dy, g[r][j]);
-#pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-          float2 &a = u[r][j][i], &d = g[r][j][i];
-          if (CENTER) a = add2(a, both(-mean[r]));
-          a = times2(a, both(rstd[r]));
-          sum_weight[j][i] = madd2(d, a, sum_weight[j][i]);
-          if (CENTER) sum_bias[j][i] = add2(sum_bias[j][i], d);
-          d = times2(d, w[i]);
-          along[r] = madd2(d, a, along[r]);
-          if (CENTER) total[r] = add2(total[r], d);
-        }
-      }
-    }
-    float sums[SUMS];
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      sums[r] = along[r].x + along[r].y;
-      if (CENTER) sums[ROWS + r] = total[r].x + total[r].y;
-    }
-    block_sum(sums, slots[turn]);
-    if (grad_x != nullptr) {
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        if (r > 0 && first + r >= rows) break;
-        T* dst = grad_x + (first + r) * hidden + threadIdx.x * VEC;
-        const float2 by = both(rstd[r]), back = both(-sums[r] * scale * rstd[r]);
-        const float2 offset = CENTER ? both(-sums[ROWS + r] * scale * rstd[r]) : both(0.0f);
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if (here[j]) {
-#pragma unroll
-            for (int i = 0; i < PAIRS; ++i) {
-              const float2 v = CENTER ? madd2(g[r][j][i], by, offset) : times2(g[r][j][i], by);
-              g[r][j][i] = madd2(u[r][j][i], back, v);
-            }
-            st_16(dst + j * threads * VEC, Quad<T>::narrow(g[r][j]));
-          }
-      }
-    }
-    last = stage;
-    if (++stage == stages) stage = 0;
-  }
-  if (partial_weight == nullptr) return;
-  const long long base = static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if (here[j]) {
-#pragma unroll
-      for (int i = 0; i < PAIRS; i += 2) {
-        const long long at = base + j * threads * VEC + 2 * i;
-        *reinterpret_cast<float4*>(partial_weight + at) =
-            make_float4(sum_weight[j][i].x, sum_weight[j][i].y, sum_weight[j][i + 1].x, sum_weight[j][i + 1].y);
-        if (CENTER)
-          *reinterpret_cast<float4*>(partial_bias + at) =
-              make_float4(sum_bias[j][i].x, sum_bias[j][i].y, sum_bias[j][i + 1].x, sum_bias[j][i + 1].y);
-      }
-    }
-}
-
-// The same for rows whose u and g do not fit the registers of two blocks per SM beside the sums: one row at a time, which is
-// widened again from the ring behind the reduction. More instructions, but 28 instead of 14 warps to issue them.
-constexpr int WIDE_THREADS = 448;
-template <typename T, typename W, int NV, bool CENTER>
-__global__ void __launch_bounds__(WIDE_THREADS, 2)
+// The gradient over the same ring, x and dy per stage. Threads own columns: the parameters' gradients stay in registers over
+// all rows of a block, so that x and dy are read once. Behind the reduction a row is widened again from the ring: kept in
+// registers its g and u would leave room for 14 warps per SM instead of 28 (16384 rows, layer norm, BF16: 2048 wide 67 against
+// 45 us, 4096 100 against 83, 7168 203 against 144).
+constexpr int WIDE_THREADS = 448;  // a row of 7168
+template <typename T, typename W, int NV, int PITCH, bool CENTER>
+__global__ void __launch_bounds__(PITCH, 2 * WIDE_THREADS / PITCH > 0 ? 2 * WIDE_THREADS / PITCH : 1)
 stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
                         long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
                         const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
@@ -628,7 +390,7 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
   constexpr int stages = GRAD_STAGES, SUMS = CENTER ? 2 : 1;
   __shared__ __align__(16) float slots[2][SUMS * STREAM_WARPS];
   constexpr int PAIRS = Quad<T>::PAIRS, VEC = 2 * PAIRS;
-  constexpr int PITCH = WIDE_THREADS, WIDTH = NV * PITCH;  // known at compile time: offsets in the ring cost no arithmetic
+  constexpr int WIDTH = NV * PITCH;  // known at compile time: offsets in the ring cost no arithmetic
   const int threads = blockDim.x;
   const int packs = hidden / VEC;
   const float scale = 1.0f / static_cast<float>(hidden);
@@ -753,6 +515,435 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
     }
 }
 
+// The gradient of the longest rows that stream, 32 values per thread and one block per SM: g and u stay in registers between the
+// reduction and dx.
+template <typename T, typename W, int NV, int PITCH, bool CENTER>
+__global__ void __launch_bounds__(PITCH)
+stream_longest_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
+                        long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
+                        const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
+                        float* __restrict__ partial_bias) {
+  extern __shared__ uint4 ring_raw[];
+  constexpr int stages = GRAD_STAGES, SUMS = CENTER ? 2 : 1;
+  __shared__ __align__(16) float slots[2][SUMS * STREAM_WARPS];
+  constexpr int PAIRS = Quad<T>::PAIRS, VEC = 2 * PAIRS;
+  constexpr int WIDTH = NV * PITCH;  // known at compile time: offsets in the ring cost no arithmetic
+  const int threads = blockDim.x;
+  const int packs = hidden / VEC;
+  const float scale = 1.0f / static_cast<float>(hidden);
+  uint4* ring = ring_raw + threadIdx.x;  // [stage][x, dy][NV][PITCH]
+  for (int i = threadIdx.x; i < SUMS * STREAM_WARPS; i += threads) slots[0][i] = slots[1][i] = 0.0f;
+  bool here[NV];
+  constexpr int QUADS = PAIRS / Quad<W>::PAIRS;  // 16-byte pieces of a pack's parameters, kept as they are
+  uint4 params[NV][QUADS];
+  float2 sum_weight[NV][PAIRS], sum_bias[CENTER ? NV : 1][PAIRS];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int at = j * threads + threadIdx.x;
+    here[j] = at < packs;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      sum_weight[j][i] = both(0.0f);
+      if (CENTER) sum_bias[j][i] = both(0.0f);
+    }
+    float2 ones[Quad<W>::PAIRS];
+#pragma unroll
+    for (int i = 0; i < Quad<W>::PAIRS; ++i) ones[i] = both(1.0f);
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i)
+      params[j][i] = here[j] && weight != nullptr ? ld_16(weight + at * VEC + i * 2 * Quad<W>::PAIRS) : Quad<W>::narrow(ones);
+  }
+  const T *mine_x = x + threadIdx.x * VEC, *mine_grad = grad + threadIdx.x * VEC;
+  auto fetch = [&](long long row, int stage) {
+    if (row < rows) {
+      const T *a = mine_x + row * x_stride, *d = mine_grad + row * grad_stride;
+      uint4* dst = ring + stage * 2 * WIDTH;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (here[j]) {
+          copy_async_16(dst + j * PITCH, a + j * threads * VEC);
+          copy_async_16(dst + WIDTH + j * PITCH, d + j * threads * VEC);
+        }
+    }
+    copy_async_commit();
+  };
+  for (int s = 0; s < stages - 1; ++s) fetch(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  __syncthreads();  // the slots are zero
+  int stage = 0, last = stages - 1, turn = 0;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    const float mean = CENTER ? mean_in[row] : 0.0f, rstd = rstd_in[row];
+    fetch(row + static_cast<long long>(stages - 1) * gridDim.x, last);
+    copy_async_wait<stages - 1>();
+    float2 u[NV][PAIRS], g[NV][PAIRS];
+    float2 along = both(0.0f), total = both(0.0f);  // sums of g u and of g
+    const uint4* src = ring + stage * 2 * WIDTH;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+        float2 w[PAIRS];
+#pragma unroll
+        for (int i = 0; i < QUADS; ++i) Quad<W>::widen(params[j][i], w + i * Quad<W>::PAIRS);
+        Quad<T>::widen(src[j * PITCH], u[j]);
+        Quad<T>::widen(src[WIDTH + j * PITCH], g[j]);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          float2 &a = u[j][i], &d = g[j][i];
+          if (CENTER) a = add2(a, both(-mean));
+          a = times2(a, both(rstd));
+          sum_weight[j][i] = madd2(d, a, sum_weight[j][i]);
+          if (CENTER) sum_bias[j][i] = add2(sum_bias[j][i], d);
+          d = times2(d, w[i]);
+          along = madd2(d, a, along);
+          if (CENTER) total = add2(total, d);
+        }
+      }
+    float sums[SUMS];
+    sums[0] = along.x + along.y;
+    if (CENTER) sums[SUMS - 1] = total.x + total.y;
+    block_sum(sums, slots[turn]);
+    if (grad_x != nullptr) {
+      T* dst = grad_x + row * hidden + threadIdx.x * VEC;
+      const float2 back = both(-sums[0] * scale * rstd), offset = both(CENTER ? -sums[SUMS - 1] * scale * rstd : 0.0f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (here[j]) {
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) {
+            const float2 v = CENTER ? madd2(g[j][i], both(rstd), offset) : times2(g[j][i], both(rstd));
+            g[j][i] = madd2(u[j][i], back, v);
+          }
+          st_16(dst + j * threads * VEC, Quad<T>::narrow(g[j]));
+        }
+    }
+    last = stage;
+    if (++stage == stages) stage = 0;
+  }
+  if (partial_weight == nullptr) return;
+  const long long base = static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (here[j]) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; i += 2) {
+        const long long at = base + j * threads * VEC + 2 * i;
+        *reinterpret_cast<float4*>(partial_weight + at) =
+            make_float4(sum_weight[j][i].x, sum_weight[j][i].y, sum_weight[j][i + 1].x, sum_weight[j][i + 1].y);
+        if (CENTER)
+          *reinterpret_cast<float4*>(partial_bias + at) =
+              make_float4(sum_bias[j][i].x, sum_bias[j][i].y, sum_bias[j][i + 1].x, sum_bias[j][i + 1].y);
+      }
+    }
+}
+
+// Rows that start on no 16-byte boundary, or are no multiple of 16 bytes, of a tensor that starts on one. A ring again, but of
+// windows: the 16-byte pieces that hold a row, copied by whichever thread, so that a barrier stands before their use. The
+// first piece may begin with the end of the row before (the first row of all begins on its boundary), the last one ends
+// with the row. VEC = 1 or 2 values per access behind that. (Straight from memory, two bytes at a time, too little was under
+// way: 237 us for 16384 rows of 5003 BF16 against 50 us of traffic.)
+constexpr int WINDOW_WARPS = 16;
+constexpr int WINDOW_MOST = 8192;  // values of a row
+constexpr int WINDOW_STAGES = 6;
+
+__device__ __forceinline__ void copy_async_part(void* smem_dst, const void* src, int bytes) {  // 16 bytes, zeros behind `bytes`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem_dst))),
+               "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void window_fetch(uint8_t* dst, const void* row, int bytes) {
+  const uintptr_t start = reinterpret_cast<uintptr_t>(row), end = start + bytes;
+  for (uintptr_t at = (start & ~static_cast<uintptr_t>(15)) + threadIdx.x * 16; at < end; at += blockDim.x * 16) {
+    const int valid = end - at < 16 ? static_cast<int>(end - at) : 16;
+    copy_async_part(dst + (at - (start & ~static_cast<uintptr_t>(15))), reinterpret_cast<const void*>(at), valid);
+  }
+}
+__device__ __forceinline__ int window_shift(const void* row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15); }
+__device__ __forceinline__ void window_wait(int pending) {
+  switch (pending) {
+    case 1: copy_async_wait<1>(); break;
+    case 2: copy_async_wait<2>(); break;
+    case 3: copy_async_wait<3>(); break;
+    case 4: copy_async_wait<4>(); break;
+    default: copy_async_wait<5>(); break;
+  }
+}
+
+template <typename T, typename W, int VEC, int NV, bool CENTER>
+__global__ void __launch_bounds__(32 * WINDOW_WARPS)
+window_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, int hidden, const W* __restrict__ weight,
+                   const W* __restrict__ bias, float eps, T* __restrict__ y, float* __restrict__ mean_out,
+                   float* __restrict__ rstd_out, int stages, int window) {
+  extern __shared__ uint4 ring_raw[];
+  __shared__ __align__(16) float slots[2][WINDOW_WARPS];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(ring_raw);
+  const int threads = blockDim.x, packs = hidden / VEC, bytes = hidden * static_cast<int>(sizeof(T));
+  const float scale = 1.0f / static_cast<float>(hidden);
+  if (threadIdx.x < WINDOW_WARPS) slots[0][threadIdx.x] = slots[1][threadIdx.x] = 0.0f;
+  bool here[NV];
+  float w[NV][VEC], b[CENTER ? NV : 1][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int at = j * threads + threadIdx.x;
+    here[j] = at < packs;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      w[j][e] = here[j] && weight != nullptr ? widen(weight[at * VEC + e]) : 1.0f;
+      if (CENTER) b[j][e] = here[j] && bias != nullptr ? widen(bias[at * VEC + e]) : 0.0f;
+    }
+  }
+  auto fetch = [&](long long row, int stage) {
+    if (row < rows) window_fetch(ring + stage * window, x + row * x_stride, bytes);
+    copy_async_commit();
+  };
+  for (int s = 0; s < stages - 1; ++s) fetch(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  int stage = 0, last = stages - 1, turn = 0;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    // the stage that is filled now was read before a barrier of the row before
+    fetch(row + static_cast<long long>(stages - 1) * gridDim.x, last);
+    window_wait(stages - 1);
+    __syncthreads();
+    const T* src = reinterpret_cast<const T*>(ring + stage * window + window_shift(x + row * x_stride)) + threadIdx.x * VEC;
+    float v[NV][VEC];
+    float sum[1] = {0.0f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[j][e] = 0.0f;
+      if (here[j]) {
+        const Pack<T, VEC> in = load_pack<T, VEC>(src + j * threads * VEC);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          v[j][e] = widen(in.v[e]);
+          sum[0] += v[j][e];
+        }
+      }
+    }
+    float mean = 0.0f;
+    if (CENTER) {
+      block_sum<WINDOW_WARPS>(sum, slots[turn]);
+      turn ^= 1;
+      mean = sum[0] * scale;
+    }
+    float square[1] = {0.0f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (CENTER) v[j][e] = here[j] ? v[j][e] - mean : 0.0f;
+        square[0] += v[j][e] * v[j][e];
+      }
+    block_sum<WINDOW_WARPS>(square, slots[turn]);
+    turn ^= 1;
+    const float rstd = rsqrtf(square[0] * scale + eps);
+    T* dst = y + row * hidden + threadIdx.x * VEC;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float u = v[j][e] * rstd;
+          out.v[e] = narrow<T>(CENTER ? u * w[j][e] + b[j][e] : u * w[j][e]);
+        }
+        store_pack<T, VEC>(dst + j * threads * VEC, out);
+      }
+    if (threadIdx.x == 0 && rstd_out != nullptr) {
+      if (CENTER) mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    last = stage;
+    if (++stage == stages) stage = 0;
+  }
+}
+
+template <typename T, typename W, int VEC, int NV, bool CENTER>
+__global__ void __launch_bounds__(32 * WINDOW_WARPS)
+window_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
+                        long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
+                        const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
+                        float* __restrict__ partial_bias, int stages, int window) {
+  extern __shared__ uint4 ring_raw[];
+  __shared__ __align__(16) float slots[2][2 * WINDOW_WARPS];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(ring_raw);  // [stage][x, dy]
+  const int threads = blockDim.x, packs = hidden / VEC, bytes = hidden * static_cast<int>(sizeof(T));
+  const float scale = 1.0f / static_cast<float>(hidden);
+  for (int i = threadIdx.x; i < 2 * WINDOW_WARPS; i += threads) slots[0][i] = slots[1][i] = 0.0f;
+  bool here[NV];
+  float w[NV][VEC], sum_weight[NV][VEC], sum_bias[CENTER ? NV : 1][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int at = j * threads + threadIdx.x;
+    here[j] = at < packs;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      w[j][e] = here[j] && weight != nullptr ? widen(weight[at * VEC + e]) : 1.0f;
+      sum_weight[j][e] = 0.0f;
+      if (CENTER) sum_bias[j][e] = 0.0f;
+    }
+  }
+  auto fetch = [&](long long row, int stage) {
+    if (row < rows) {
+      window_fetch(ring + 2 * stage * window, x + row * x_stride, bytes);
+      window_fetch(ring + (2 * stage + 1) * window, grad + row * grad_stride, bytes);
+    }
+    copy_async_commit();
+  };
+  for (int s = 0; s < stages - 1; ++s) fetch(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  int stage = 0, last = stages - 1, turn = 0;
+  float next_mean = CENTER && blockIdx.x < rows ? mean_in[blockIdx.x] : 0.0f;
+  float next_rstd = blockIdx.x < rows ? rstd_in[blockIdx.x] : 0.0f;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
+    const long long next = row + gridDim.x;
+    if (next < rows) {
+      if (CENTER) next_mean = mean_in[next];
+      next_rstd = rstd_in[next];
+    }
+    fetch(row + static_cast<long long>(stages - 1) * gridDim.x, last);
+    window_wait(stages - 1);
+    __syncthreads();
+    const uint8_t* at = ring + 2 * stage * window;
+    const T* a = reinterpret_cast<const T*>(at + window_shift(x + row * x_stride)) + threadIdx.x * VEC;
+    const T* d = reinterpret_cast<const T*>(at + window + window_shift(grad + row * grad_stride)) + threadIdx.x * VEC;
+    float u[NV][VEC], g[NV][VEC];
+    float sums[2] = {0.0f, 0.0f};  // of g * u and of g
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+        const Pack<T, VEC> in = load_pack<T, VEC>(a + j * threads * VEC), dy = load_pack<T, VEC>(d + j * threads * VEC);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float dv = widen(dy.v[e]);
+          u[j][e] = (widen(in.v[e]) - mean) * rstd;
+          sum_weight[j][e] += dv * u[j][e];
+          if (CENTER) sum_bias[j][e] += dv;
+          g[j][e] = dv * w[j][e];
+          sums[0] += g[j][e] * u[j][e];
+          sums[1] += g[j][e];
+        }
+      }
+    block_sum<WINDOW_WARPS>(sums, slots[turn]);
+    last = stage;
+    if (++stage == stages) stage = 0;
+    if (grad_x == nullptr) continue;
+    const float along = sums[0] * scale, offset = CENTER ? sums[1] * scale : 0.0f;
+    T* dst = grad_x + row * hidden + threadIdx.x * VEC;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out.v[e] = narrow<T>((g[j][e] - u[j][e] * along - offset) * rstd);
+        store_pack<T, VEC>(dst + j * threads * VEC, out);
+      }
+  }
+  if (partial_weight == nullptr) return;
+  const long long base = static_cast<long long>(blockIdx.x) * hidden;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (here[j]) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const long long at = base + (j * threads + static_cast<int>(threadIdx.x)) * VEC + e;
+        partial_weight[at] = sum_weight[j][e];
+        if (CENTER) partial_bias[at] = sum_bias[j][e];
+      }
+    }
+}
+
+// Short rows: a warp per row, no barrier per row, the next row's loads under way. The warps of a block join their sums over
+// rows one after the other in shared memory.
+constexpr int SHORT_WARPS = 8;
+
+template <typename T, typename W, int VEC, int NV, bool CENTER>
+__global__ void __launch_bounds__(32 * SHORT_WARPS, 2)
+short_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
+                       long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
+                       const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
+                       float* __restrict__ partial_bias) {
+  __shared__ float joined[2][32 * VEC * NV];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, packs = hidden / VEC;
+  const float scale = 1.0f / static_cast<float>(hidden);
+  bool here[NV];
+  float w[NV][VEC], sum_weight[NV][VEC], sum_bias[CENTER ? NV : 1][VEC];
+  Pack<T, VEC> next_x[NV], next_grad[NV];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch = [&](long long row) {
+    const T *a = x + row * x_stride + lane * VEC, *d = grad + row * grad_stride + lane * VEC;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+        next_x[j] = load_pack<T, VEC>(a + j * 32 * VEC);
+        next_grad[j] = load_pack<T, VEC>(d + j * 32 * VEC);
+      }
+    if (CENTER) next_mean = mean_in[row];
+    next_rstd = rstd_in[row];
+  };
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int at = j * 32 + lane;
+    here[j] = at < packs;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      next_x[j].v[e] = next_grad[j].v[e] = narrow<T>(0.0f);
+      w[j][e] = here[j] && weight != nullptr ? widen(weight[at * VEC + e]) : 1.0f;
+      sum_weight[j][e] = 0.0f;
+      if (CENTER) sum_bias[j][e] = 0.0f;
+    }
+  }
+  const long long step = static_cast<long long>(gridDim.x) * SHORT_WARPS;
+  const long long first = static_cast<long long>(blockIdx.x) * SHORT_WARPS + warp;
+  if (first < rows) fetch(first);
+  for (long long row = first; row < rows; row += step) {
+    const float mean = next_mean, rstd = next_rstd;
+    float u[NV][VEC], g[NV][VEC];
+    float along = 0.0f, total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = widen(next_grad[j].v[e]);
+        u[j][e] = (widen(next_x[j].v[e]) - mean) * rstd;
+        sum_weight[j][e] += d * u[j][e];
+        if (CENTER) sum_bias[j][e] += d;
+        g[j][e] = d * w[j][e];
+        along += g[j][e] * u[j][e];
+        if (CENTER) total += g[j][e];
+      }
+    if (row + step < rows) fetch(row + step);
+    if (grad_x == nullptr) continue;
+    along = warp_sum(along) * scale;
+    total = CENTER ? warp_sum(total) * scale : 0.0f;
+    T* dst = grad_x + row * hidden + lane * VEC;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (here[j]) {
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out.v[e] = narrow<T>((g[j][e] - u[j][e] * along - total) * rstd);
+        store_pack<T, VEC>(dst + j * 32 * VEC, out);
+      }
+  }
+  if (partial_weight == nullptr) return;
+  for (int turn = 0; turn < SHORT_WARPS; ++turn) {
+    if (turn == warp) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int at = (j * 32 + lane) * VEC + e;
+          joined[0][at] = (turn > 0 ? joined[0][at] : 0.0f) + sum_weight[j][e];
+          if (CENTER) joined[1][at] = (turn > 0 ? joined[1][at] : 0.0f) + sum_bias[j][e];
+        }
+    }
+    __syncthreads();
+  }
+  const long long base = static_cast<long long>(blockIdx.x) * hidden;
+  for (int c = threadIdx.x; c < hidden; c += 32 * SHORT_WARPS) {
+    partial_weight[base + c] = joined[0][c];
+    if (CENTER) partial_bias[base + c] = joined[1][c];
+  }
+}
+
 // Rows too long for a block's registers: dx by one block per row, the parameters' partial sums by columns.
 template <typename T, typename W, bool CENTER>
 __global__ void __launch_bounds__(1024) long_row_norm_grad_kernel(const T* __restrict__ x, long long x_stride,
@@ -833,9 +1024,6 @@ bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
 constexpr int FORWARD_PACKS = 4;  // packs of 16 bytes per thread and row
-constexpr int GRAD_PACKS = 2;
-constexpr int SINGLES = 8;        // values per thread where rows start on no 16-byte boundary
-constexpr int GRAD_THREADS = 512;
 
 struct NormCall {
   const void *x, *grad, *weight, *bias;
@@ -849,10 +1037,10 @@ struct NormCall {
   cudaStream_t stream;
 };
 
-// Blocks of the gradient kernels: two per SM at most, each with partial sums of its own.
-constexpr int GRAD_BLOCKS = 2;
-long long grad_parts(long long rows) {
-  const long long most = static_cast<long long>(GRAD_BLOCKS) * sm_count();
+// Blocks of the gradient kernels per SM at most, each with partial sums of its own: fewer of long rows.
+int grad_blocks(long long hidden) { return hidden <= 1024 ? 8 : hidden <= 2048 ? 6 : hidden <= 4096 ? 3 : 2; }
+long long grad_parts(long long rows, long long hidden) {
+  const long long most = static_cast<long long>(grad_blocks(hidden)) * sm_count();
   return rows < most ? rows : most;
 }
 
@@ -874,7 +1062,7 @@ constexpr int STREAM_SHARED = SM_SHARED - 2048;  // beside the reductions' slots
 
 // Blocks of `threads` threads with `bytes` of shared memory that an SM holds of a kernel; asked once per block size.
 struct Residency {
-  int blocks[HMC_MAX_DEVICES][STREAM_WARPS + 1];
+  int blocks[HMC_MAX_DEVICES][WINDOW_WARPS + 1];
 };
 template <typename Kernel>
 int resident_blocks(Kernel kernel, int threads, int bytes, Residency& known, int* blocks) {
@@ -882,7 +1070,7 @@ int resident_blocks(Kernel kernel, int threads, int bytes, Residency& known, int
   HMC_CUDA_OK(cudaGetDevice(&dev));
   int* slot = dev < HMC_MAX_DEVICES ? &known.blocks[dev][threads / 32] : nullptr;
   if (slot == nullptr || *slot == 0) {
-    HMC_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SHARED));
+    if (bytes > 0) HMC_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SHARED));
     int found = 0;
     HMC_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&found, kernel, threads, bytes));
     if (found < 1) found = 1;
@@ -921,18 +1109,15 @@ int stream(const NormCall& c) {
   return packs <= 512 ? launch_stream<T, W, 2, CENTER>(c) : launch_stream<T, W, 4, CENTER>(c);
 }
 
-template <typename T, typename W, int NV, int ROWS, int PITCH, bool CENTER>
-int launch_stream_grad(NormCall& c) {
+template <typename T, typename W, int NV, int PITCH, bool CENTER>
+int launch_longest_grad(NormCall& c) {
   constexpr int VEC = 16 / sizeof(T);
   const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
-  const int bytes = GRAD_STAGES * ROWS * 2 * NV * PITCH * 16;
-  static Residency known{};
-  auto kernel = stream_norm_grad_kernel<T, W, NV, ROWS, PITCH, CENTER>;
-  int blocks = 0;
-  if (int rc = resident_blocks(kernel, threads, bytes, known, &blocks)) return rc;
-  if (blocks > GRAD_BLOCKS) blocks = GRAD_BLOCKS;
-  const long long most = static_cast<long long>(blocks) * sm_count(), pieces = (c.rows + ROWS - 1) / ROWS;
-  c.parts = static_cast<int>(pieces < most ? pieces : most);
+  constexpr int bytes = GRAD_STAGES * 2 * NV * PITCH * 16;
+  static PerDeviceFlag configured{};
+  auto kernel = stream_longest_grad_kernel<T, W, NV, PITCH, CENTER>;
+  if (int rc = allow_dynamic_smem(kernel, bytes, configured)) return rc;
+  c.parts = static_cast<int>(c.rows < sm_count() ? c.rows : sm_count());
   kernel<<<static_cast<unsigned>(c.parts), threads, bytes, c.stream>>>(
       static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
       static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias);
@@ -940,16 +1125,16 @@ int launch_stream_grad(NormCall& c) {
   return 0;
 }
 
-template <typename T, typename W, int NV, bool CENTER>
+template <typename T, typename W, int NV, int PITCH, bool CENTER>
 int launch_wide_grad(NormCall& c) {
   constexpr int VEC = 16 / sizeof(T);
   const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
-  const int bytes = NV * WIDE_THREADS * (GRAD_STAGES * 2 * 16 + VEC * 4);
+  const int bytes = NV * PITCH * (GRAD_STAGES * 2 * 16 + VEC * 4);
   static Residency known{};
-  auto kernel = stream_wide_grad_kernel<T, W, NV, CENTER>;
+  auto kernel = stream_wide_grad_kernel<T, W, NV, PITCH, CENTER>;
   int blocks = 0;
   if (int rc = resident_blocks(kernel, threads, bytes, known, &blocks)) return rc;
-  if (blocks > GRAD_BLOCKS) blocks = GRAD_BLOCKS;
+  if (blocks > grad_blocks(c.hidden)) blocks = grad_blocks(c.hidden);
   const long long most = static_cast<long long>(blocks) * sm_count();
   c.parts = static_cast<int>(c.rows < most ? c.rows : most);
   kernel<<<static_cast<unsigned>(c.parts), threads, bytes, c.stream>>>(
@@ -966,9 +1151,45 @@ constexpr int LONGEST = sizeof(T) == 4 ? 288 : STREAM_THREADS;
 template <typename T, typename W, bool CENTER>
 int stream_grad(NormCall& c) {
   constexpr int NV = sizeof(T) == 4 ? 4 : 2;  // 16 values per thread
-  if (c.hidden <= 16 * 256) return launch_stream_grad<T, W, NV, 2, 256, CENTER>(c);
-  if (c.hidden <= 16 * WIDE_THREADS) return launch_wide_grad<T, W, NV, CENTER>(c);
-  return launch_stream_grad<T, W, 2 * NV, 1, LONGEST<T>, CENTER>(c);
+  if (c.hidden <= 16 * 64) return launch_wide_grad<T, W, NV, 64, CENTER>(c);
+  if (c.hidden <= 16 * 128) return launch_wide_grad<T, W, NV, 128, CENTER>(c);
+  if (c.hidden <= 16 * 256) return launch_wide_grad<T, W, NV, 256, CENTER>(c);
+  if (c.hidden <= 16 * WIDE_THREADS) return launch_wide_grad<T, W, NV, WIDE_THREADS, CENTER>(c);
+  if (c.hidden <= 16 * STREAM_THREADS) return launch_wide_grad<T, W, NV, STREAM_THREADS, CENTER>(c);
+  return launch_longest_grad<T, W, 2 * NV, LONGEST<T>, CENTER>(c);
+}
+
+// Windows of a row in a ring of `each` of them per stage.
+struct WindowRing {
+  int window, stages, bytes;
+  WindowRing(long long row_bytes, int each) {
+    window = static_cast<int>((row_bytes + 15 + 15) / 16 * 16);
+    stages = STREAM_SHARED / (each * window);
+    if (stages > WINDOW_STAGES) stages = WINDOW_STAGES;
+    bytes = stages * each * window;
+  }
+};
+
+template <typename T, typename W, int VEC, int NV, bool CENTER>
+int launch_window(const NormCall& c) {
+  const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
+  const WindowRing ring(c.hidden * sizeof(T), 1);
+  static Residency known{};
+  auto kernel = window_norm_kernel<T, W, VEC, NV, CENTER>;
+  int blocks = 0;
+  if (int rc = resident_blocks(kernel, threads, ring.bytes, known, &blocks)) return rc;
+  const long long most = static_cast<long long>(blocks) * sm_count();
+  kernel<<<static_cast<unsigned>(c.rows < most ? c.rows : most), threads, ring.bytes, c.stream>>>(
+      static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
+      c.eps, static_cast<T*>(c.y), c.mean, c.rstd, ring.stages, ring.window);
+  HMC_LAUNCH_OK();
+  return 0;
+}
+
+template <typename T, typename W, int VEC, bool CENTER>
+int window(const NormCall& c) {
+  if (c.hidden <= 2048) return launch_window<T, W, VEC, 8 / VEC, CENTER>(c);
+  return launch_window<T, W, VEC, 16 / VEC, CENTER>(c);
 }
 
 template <typename T, typename W, bool CENTER>
@@ -979,7 +1200,11 @@ int forward(const NormCall& c) {
   if (wide && c.rows > 2ll * sm_count() && c.hidden > 32 * VEC * FORWARD_PACKS && c.hidden <= STREAM_THREADS * VEC * FORWARD_PACKS)
     return stream<T, W, CENTER>(c);
   if (wide && c.hidden <= 1024 * VEC * FORWARD_PACKS) return launch_forward<T, W, VEC, FORWARD_PACKS, CENTER>(c);
-  if (c.hidden <= 1024 * SINGLES) return launch_forward<T, W, 1, SINGLES, CENTER>(c);
+  const bool pairs = c.hidden % 2 == 0 && c.x_stride % 2 == 0 && aligned_to(c.x, 2 * sizeof(T)) && aligned_to(c.y, 2 * sizeof(T)) &&
+                     aligned_to(c.weight, 2 * sizeof(W)) && aligned_to(c.bias, 2 * sizeof(W));
+  if (c.hidden <= 32 * 16)
+    return pairs ? launch_forward<T, W, 2, 8, CENTER>(c) : launch_forward<T, W, 1, 16, CENTER>(c);
+  if (aligned_to(c.x, 16) && c.hidden <= WINDOW_MOST) return pairs ? window<T, W, 2, CENTER>(c) : window<T, W, 1, CENTER>(c);
   long_row_norm_kernel<T, W, CENTER><<<static_cast<unsigned>(c.rows), 1024, 0, c.stream>>>(
       static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
       c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
@@ -988,13 +1213,44 @@ int forward(const NormCall& c) {
 }
 
 template <typename T, typename W, int VEC, int NV, bool CENTER>
-int launch_grad(const NormCall& c) {
+int launch_window_grad(NormCall& c) {
   const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
-  row_norm_grad_kernel<T, W, VEC, NV, CENTER><<<static_cast<unsigned>(c.parts), threads, 0, c.stream>>>(
+  const WindowRing ring(c.hidden * sizeof(T), 2);
+  static Residency known{};
+  auto kernel = window_norm_grad_kernel<T, W, VEC, NV, CENTER>;
+  int blocks = 0;
+  if (int rc = resident_blocks(kernel, threads, ring.bytes, known, &blocks)) return rc;
+  if (blocks > grad_blocks(c.hidden)) blocks = grad_blocks(c.hidden);
+  const long long most = static_cast<long long>(blocks) * sm_count();
+  c.parts = static_cast<int>(c.rows < most ? c.rows : most);
+  kernel<<<static_cast<unsigned>(c.parts), threads, ring.bytes, c.stream>>>(
+      static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
+      static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias, ring.stages,
+      ring.window);
+  HMC_LAUNCH_OK();
+  return 0;
+}
+
+template <typename T, typename W, int VEC, int NV, bool CENTER>
+int launch_short_grad(NormCall& c) {
+  static Residency known{};
+  int blocks = 0;
+  if (int rc = resident_blocks(short_norm_grad_kernel<T, W, VEC, NV, CENTER>, 32 * SHORT_WARPS, 0, known, &blocks)) return rc;
+  if (blocks > 4) blocks = 4;  // 32 warps
+  const long long most = static_cast<long long>(blocks) * sm_count();
+  const long long pieces = (c.rows + SHORT_WARPS - 1) / SHORT_WARPS;
+  c.parts = static_cast<int>(pieces < most ? pieces : most);
+  short_norm_grad_kernel<T, W, VEC, NV, CENTER><<<static_cast<unsigned>(c.parts), 32 * SHORT_WARPS, 0, c.stream>>>(
       static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
       static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias);
   HMC_LAUNCH_OK();
   return 0;
+}
+
+template <typename T, typename W, int VEC, bool CENTER>
+int window_grad(NormCall& c) {
+  if (c.hidden <= 2048) return launch_window_grad<T, W, VEC, 8 / VEC, CENTER>(c);
+  return launch_window_grad<T, W, VEC, 16 / VEC, CENTER>(c);
 }
 
 template <typename T, typename W, bool CENTER>
@@ -1002,12 +1258,19 @@ int gradient(NormCall& c) {
   constexpr int VEC = 16 / sizeof(T);
   const bool wide = c.hidden % VEC == 0 && c.x_stride % VEC == 0 && c.grad_stride % VEC == 0 && aligned_to(c.x, 16) &&
                     aligned_to(c.grad, 16) && aligned_to(c.y, 16) && aligned_to(c.weight, 16);
-  if (wide && c.hidden > 32 * VEC * FORWARD_PACKS && c.hidden <= 32 * LONGEST<T>) {
-    if (int rc = stream_grad<T, W, CENTER>(c)) return rc;
-  } else if (wide && c.hidden <= GRAD_THREADS * VEC * GRAD_PACKS) {
-    if (int rc = launch_grad<T, W, VEC, GRAD_PACKS, CENTER>(c)) return rc;
-  } else if (c.hidden <= GRAD_THREADS * SINGLES) {
-    if (int rc = launch_grad<T, W, 1, SINGLES, CENTER>(c)) return rc;
+  const bool pairs = c.hidden % 2 == 0 && c.x_stride % 2 == 0 && c.grad_stride % 2 == 0 && aligned_to(c.x, 2 * sizeof(T)) &&
+                     aligned_to(c.grad, 2 * sizeof(T)) && aligned_to(c.y, 2 * sizeof(T));
+  int rc = 0;
+  if (wide && c.hidden <= 32 * VEC) {
+    rc = launch_short_grad<T, W, VEC, 1, CENTER>(c);
+  } else if (wide && c.hidden <= 32 * VEC * 2) {
+    rc = launch_short_grad<T, W, VEC, 2, CENTER>(c);
+  } else if (wide && c.hidden <= 32 * LONGEST<T>) {
+    rc = stream_grad<T, W, CENTER>(c);
+  } else if (c.hidden <= 32 * 16) {
+    rc = pairs ? launch_short_grad<T, W, 2, 8, CENTER>(c) : launch_short_grad<T, W, 1, 16, CENTER>(c);
+  } else if (aligned_to(c.x, 16) && aligned_to(c.grad, 16) && c.hidden <= WINDOW_MOST) {
+    rc = pairs ? window_grad<T, W, 2, CENTER>(c) : window_grad<T, W, 1, CENTER>(c);
   } else {
     if (c.y != nullptr) {
       long_row_norm_grad_kernel<T, W, CENTER><<<static_cast<unsigned>(c.rows), 1024, 0, c.stream>>>(
@@ -1023,6 +1286,7 @@ int gradient(NormCall& c) {
       HMC_LAUNCH_OK();
     }
   }
+  if (rc != 0) return rc;
   if (c.partial_weight != nullptr) {
     param_grad_kernel<W><<<(c.hidden + 31) / 32, dim3(32, FINISH_SLICES), 0, c.stream>>>(
         c.partial_weight, c.partial_bias, c.parts, c.hidden, static_cast<W*>(c.grad_weight), static_cast<W*>(c.grad_bias));
@@ -1080,7 +1344,7 @@ extern "C" int hmc_row_norm(const void* x, int64_t x_stride, int64_t rows, int64
 
 extern "C" int64_t hmc_row_norm_grad_workspace_bytes(int64_t rows, int64_t hidden) {
   if (rows <= 0 || hidden <= 0) return 0;
-  return 2 * hmc::grad_parts(rows) * hidden * static_cast<int64_t>(sizeof(float));
+  return 2 * hmc::grad_parts(rows, hidden) * hidden * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int hmc_row_norm_grad(const void* x, int64_t x_stride, const void* grad, int64_t grad_stride, int64_t rows,
@@ -1109,7 +1373,7 @@ extern "C" int hmc_row_norm_grad(const void* x, int64_t x_stride, const void* gr
   NormCall c{};
   c.x = x, c.x_stride = x_stride, c.grad = grad, c.grad_stride = grad_stride, c.rows = rows;
   c.hidden = static_cast<int>(hidden), c.weight = weight, c.mean_in = mean, c.rstd_in = rstd, c.y = grad_x;
-  c.grad_weight = grad_weight, c.grad_bias = grad_bias, c.parts = static_cast<int>(grad_parts(rows)), c.stream = s;
+  c.grad_weight = grad_weight, c.grad_bias = grad_bias, c.parts = static_cast<int>(grad_parts(rows, hidden)), c.stream = s;
   if (params) {
     c.partial_weight = static_cast<float*>(workspace);
     c.partial_bias = c.partial_weight + static_cast<long long>(c.parts) * hidden;

@@ -44,7 +44,7 @@ constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * STORE_STAGE_BYTES 
 constexpr int MAX_PARTS = 16;  // of a tile that is cut along k
 constexpr int MIN_PART = 8;    // k-blocks of a part, at the least
 constexpr int PROMOTE = 8;     // k-blocks that add up inside the tensor core before the sum goes to FP32 registers (STATS)
-constexpr int BAND = 8;  // tile rows that are walked together: 8 x 9 tiles in flight share their operands in L2
+constexpr int BAND = 16; // tile rows that are walked together, so that a band's rows stay in L2 while the weight passes by (8, 16, 32: 29987, 29527, 31442 us for a training step of 8192 x 4096 x 131072)
 
 enum Product { STATS, PROBS, GRAD_HIDDEN, GRAD_WEIGHT };
 
