@@ -88,6 +88,27 @@ static inline int allow_dynamic_smem(Kernel kernel, int bytes, PerDeviceFlag& fl
   return 0;
 }
 
+// A kernel that may start while the one before it in the stream still runs: blocks are placed as soon as the other's have all
+// started and room is left, and wait in chain_wait() until it has completed and its writes are visible. Every kernel launched
+// this way calls chain_wait() before its first access to memory that another launch touches, so that completion
+// carries over from launch to launch.
+#ifdef __CUDACC__
+template <typename... Formal, typename... Actual>
+static inline int launch_chained(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Actual... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid, config.blockDim = block, config.dynamicSmemBytes = smem, config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute, config.numAttrs = 1;
+  HMC_CUDA_OK(cudaLaunchKernelEx(&config, kernel, static_cast<Formal>(args)...));
+  count_launch();
+  return 0;
+}
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
+
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---------------------------------------------------------------------------------------------

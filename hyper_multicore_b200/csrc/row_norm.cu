@@ -499,6 +499,7 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
     if (++stage == stages) stage = 0;
   }
   if (partial_weight == nullptr) return;
+  chain_next();
   const long long base = static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -619,6 +620,7 @@ stream_longest_grad_kernel(const T* __restrict__ x, long long x_stride, const T*
     if (++stage == stages) stage = 0;
   }
   if (partial_weight == nullptr) return;
+  chain_next();
   const long long base = static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -837,6 +839,7 @@ window_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
       }
   }
   if (partial_weight == nullptr) return;
+  chain_next();
   const long long base = static_cast<long long>(blockIdx.x) * hidden;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -924,6 +927,7 @@ short_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __r
       }
   }
   if (partial_weight == nullptr) return;
+  chain_next();
   for (int turn = 0; turn < SHORT_WARPS; ++turn) {
     if (turn == warp) {
 #pragma unroll
@@ -999,6 +1003,7 @@ __global__ void __launch_bounds__(32 * FINISH_SLICES) param_grad_kernel(const fl
                                                                         int hidden, W* __restrict__ grad_weight,
                                                                         W* __restrict__ grad_bias) {
   __shared__ float sums[2][FINISH_SLICES][32];
+  chain_wait();
   const int c = blockIdx.x * 32 + threadIdx.x;
   float w = 0.0f, b = 0.0f;
   if (c < hidden) {
@@ -1288,9 +1293,8 @@ int gradient(NormCall& c) {
   }
   if (rc != 0) return rc;
   if (c.partial_weight != nullptr) {
-    param_grad_kernel<W><<<(c.hidden + 31) / 32, dim3(32, FINISH_SLICES), 0, c.stream>>>(
-        c.partial_weight, c.partial_bias, c.parts, c.hidden, static_cast<W*>(c.grad_weight), static_cast<W*>(c.grad_bias));
-    HMC_LAUNCH_OK();
+    return launch_chained(param_grad_kernel<W>, dim3((c.hidden + 31) / 32), dim3(32, FINISH_SLICES), 0, c.stream, c.partial_weight,
+                          c.partial_bias, c.parts, c.hidden, static_cast<W*>(c.grad_weight), static_cast<W*>(c.grad_bias));
   }
   return 0;
 }

@@ -153,7 +153,7 @@ __device__ __forceinline__ void epilogue_stats(const Params& p, float (&v)[HALF]
 }
 
 // 32 x 32 values leave as one BF16 box through shared memory; two boxes per warp in flight.
-__device__ __forceinline__ void store_box(const CUtensorMap* tm, uint8_t* stage, unsigned& issued, const float (&v)[32], int col,
+__device__ __forceinline__ void store_box(const CUtensorMap* tm, uint8_t* stage, unsigned& issued, const float* v, int col,
                                           int row, int lane) {
   uint8_t* box = stage + (issued & 1) * (STORE_STAGE_BYTES / 2);
   if (issued > 1) {
@@ -175,30 +175,46 @@ __device__ __forceinline__ void store_box(const CUtensorMap* tm, uint8_t* stage,
   ++issued;
 }
 
+// 64 columns of the accumulator row of each lane: two loads under way at a time.
+__device__ __forceinline__ void load_columns(uint32_t taddr, float (&v)[64]) {
+  uint32_t lo[32], hi[32];
+  __syncwarp();
+  tmem_ld_32x32(taddr, lo);
+  tmem_ld_32x32(taddr + 32, hi);
+  tmem_ld_wait();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(lo[j]), v[32 + j] = __uint_as_float(hi[j]);
+}
+
 // p of one row's 128 columns times the row's gradient, the target's entry left out.
 __device__ __forceinline__ void epilogue_probs(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
                                                unsigned& issued, int first_row, int row, bool row_ok, int col, int lane) {
   const float lse = row_ok ? p.lse[row] : 0.0f;
   const float weight = row_ok ? p.weights[row] : 0.0f;
-  const int label = row_ok ? p.labels[row] - p.first_word : -1;
+  const int label = row_ok ? p.labels[row] - p.first_word - col : -1;
 #pragma unroll 1
-  for (int c = 0; c < HALF; c += 32) {
+  for (int c = 0; c < HALF; c += 64) {
     if (col + c >= p.n) break;
-    __syncwarp();
-    uint32_t raw[32];
-    tmem_ld_32x32(taddr + c, raw);
-    tmem_ld_wait();
-    float v[32];
+    float v[64];
+    load_columns(taddr + c, v);
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      v[j] = row_ok && col + c + j != label ? shifted_exp(__uint_as_float(raw[j]), lse) * weight : 0.0f;
-    store_box(tm, stage, issued, v, col + c, first_row, lane);
+    for (int j = 0; j < 64; ++j) v[j] = row_ok ? shifted_exp(v[j], lse) * weight : 0.0f;
+    const int own = label - c;
+    if (own >= 0 && own < 64) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j)
+        if (j == own) v[j] = 0.0f;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 64; h += 32)
+      if (col + c + h < p.n) store_box(tm, stage, issued, v + h, col + c + h, first_row, lane);
   }
 }
 
 // Eight columns of a row of dx from this piece's sums: added to those of earlier pieces, and with the last piece the target's
 // row on top, scaled, rounded and stored at the token's place.
-__device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int col, float (&v)[8], float scale) {
+__device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int col, float* v, float scale) {
   float* sums = p.sums + static_cast<long long>(row) * p.n + col;
   if (p.add) {
     const float4 a = *reinterpret_cast<const float4*>(sums), b = *reinterpret_cast<const float4*>(sums + 4);
@@ -229,19 +245,14 @@ __device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int
 __device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t taddr, int row, bool row_ok, int col) {
   const float scale = *p.scale;
 #pragma unroll 1
-  for (int c = 0; c < HALF; c += 32) {
+  for (int c = 0; c < HALF; c += 64) {
     if (col + c >= p.n) break;
-    __syncwarp();
-    uint32_t raw[32];
-    tmem_ld_32x32(taddr + c, raw);
-    tmem_ld_wait();
+    float v[64];
+    load_columns(taddr + c, v);
+    if (row_ok) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (!row_ok || col + c + j >= p.n) continue;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(raw[j + e]);
-      finish_grad_hidden(p, row, col + c + j, v, scale);
+      for (int j = 0; j < 64; j += 8)
+        if (col + c + j < p.n) finish_grad_hidden(p, row, col + c + j, v + j, scale);
     }
   }
 }
@@ -250,20 +261,20 @@ __device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t t
 __device__ __forceinline__ void epilogue_part(const Params& p, uint32_t taddr, int part, int row_in_tile, bool row_ok, int half) {
   float* dst = p.part_sums + (static_cast<long long>(part) * TILE + row_in_tile) * TILE + half * HALF;
 #pragma unroll 1
-  for (int c = 0; c < HALF; c += 32) {
-    __syncwarp();
-    uint32_t raw[32];
-    tmem_ld_32x32(taddr + c, raw);
-    tmem_ld_wait();
+  for (int c = 0; c < HALF; c += 64) {
+    float v[64];
+    load_columns(taddr + c, v);
     if (row_ok) {
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) st_16(dst + c + j, make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3]));
+      for (int j = 0; j < 64; j += 4) *reinterpret_cast<float4*>(dst + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
     }
   }
 }
 
 // The tiles that were cut: their parts in order, eight columns per thread, eight rows per block.
 __global__ void __launch_bounds__(256) join_parts_kernel(Params p, int pairs) {
+  chain_wait();
+  chain_next();
   p.m = *p.count;
   const Walker walker(p.m, p.n, p.k, pairs, true);
   const long long tile = walker.whole + blockIdx.y;
@@ -291,31 +302,29 @@ __device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUte
   const int slot = row_ok ? p.slots[p.first_word + row] : -1;
   const float* more = p.word_sums + static_cast<long long>(slot >= 0 ? slot : 0) * p.n + col;
 #pragma unroll 1
-  for (int c = 0; c < HALF; c += 32) {
+  for (int c = 0; c < HALF; c += 64) {
     if (col + c >= p.n) break;
-    __syncwarp();
-    float v[32];
+    float v[64];
     if (empty) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+      for (int j = 0; j < 64; ++j) v[j] = 0.0f;
     } else {
-      uint32_t raw[32];
-      tmem_ld_32x32(taddr + c, raw);
-      tmem_ld_wait();
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+      load_columns(taddr + c, v);
       if (slot >= 0) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
+        for (int j = 0; j < 64; j += 4)
           if (col + c + j < p.n) {
             const float4 a = *reinterpret_cast<const float4*>(more + c + j);
             v[j] += a.x, v[j + 1] += a.y, v[j + 2] += a.z, v[j + 3] += a.w;
           }
       }
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= scale;
+      for (int j = 0; j < 64; ++j) v[j] *= scale;
     }
-    store_box(tm, stage, issued, v, col + c, first_row, lane);
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 64; h += 32)
+      if (col + c + h < p.n) store_box(tm, stage, issued, v + h, col + c + h, first_row, lane);
   }
 }
 
@@ -366,6 +375,8 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA signal
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  chain_wait();
+  chain_next();
 
   const int count = *p.count;
   if (KIND == GRAD_WEIGHT) p.k = count;
@@ -633,6 +644,8 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
   cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA signal
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  chain_wait();
+  chain_next();
   const int rows = *count;
   const int last = rows > 0 ? tiles : 0;  // no token counts: nothing to do
 
@@ -833,6 +846,7 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
                                                                  __nv_bfloat16* __restrict__ packed,
                                                                  float* __restrict__ token_loss) {
   __shared__ int place[PACK_TOKENS];
+  chain_next();  // the first of its chain
   const long long first = static_cast<long long>(blockIdx.x) * PACK_TOKENS;
   int before = 0;
   for (long long i = threadIdx.x; i < first; i += PACK_THREADS) before += targets.at(i) != targets.ignored;
@@ -889,6 +903,8 @@ __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __
                                                                 float* __restrict__ lse, float* __restrict__ losses,
                                                                 float* __restrict__ token_loss) {
   __shared__ float2 sums[JOIN_SLICES][33];
+  chain_wait();
+  chain_next();
   const int row = blockIdx.x * 32 + threadIdx.x;
   const bool ok = row < *count;
   float top = -INFINITY, sum = 0.0f;
@@ -928,6 +944,7 @@ __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __
 __global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ losses, const int* __restrict__ count, int mean,
                                                       float* __restrict__ loss) {
   __shared__ float slots[32];
+  chain_wait();
   const int rows = *count;
   float v = 0.0f;
   for (int i = threadIdx.x; i < rows; i += blockDim.x) v += losses[i];
@@ -948,6 +965,7 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
                                                         float* __restrict__ weights, float* __restrict__ coef,
                                                         float* __restrict__ scale, unsigned* __restrict__ slots,
                                                         int* __restrict__ members) {
+  chain_next();  // the first of its chain
   const int rows = *count;
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i == 0) {
@@ -992,17 +1010,24 @@ __device__ __forceinline__ int matches(bool match, int& place) {
   return total;
 }
 
-__global__ void __launch_bounds__(WORD_THREADS) word_sums_kernel(const __nv_bfloat16* __restrict__ packed, int hidden,
-                                                                 const int* __restrict__ count,
-                                                                 const int* __restrict__ labels,
-                                                                 const float* __restrict__ coef,
-                                                                 const unsigned* __restrict__ slots,
-                                                                 const int* __restrict__ members,
-                                                                 float* __restrict__ word_sums) {
+// Beside that, the rows of grad_hidden of the tokens that do not count (a block per token, too). Either may be absent.
+__global__ void __launch_bounds__(WORD_THREADS) token_rows_kernel(const __nv_bfloat16* __restrict__ packed, int hidden,
+                                                                  const int* __restrict__ count, const int* __restrict__ labels,
+                                                                  const float* __restrict__ coef,
+                                                                  const unsigned* __restrict__ slots,
+                                                                  const int* __restrict__ members, float* __restrict__ word_sums,
+                                                                  const int* __restrict__ position,
+                                                                  __nv_bfloat16* __restrict__ grad_hidden) {
   __shared__ int slice[WORD_SLICE];
+  chain_wait();
+  chain_next();
   const int rows = *count;
   const int row = blockIdx.x;
-  if (row >= rows) return;
+  if (grad_hidden != nullptr && position[row] < 0) {
+    for (int c = threadIdx.x * 8; c < hidden; c += WORD_THREADS * 8)
+      st_16(grad_hidden + static_cast<long long>(row) * hidden + c, make_uint4(0, 0, 0, 0));
+  }
+  if (word_sums == nullptr || row >= rows) return;
   const int label = labels[row];
   if (label < 0) return;
   const int first = static_cast<int>(slots[label]);
@@ -1056,6 +1081,8 @@ __global__ void __launch_bounds__(WORD_THREADS) word_slices_kernel(int hidden, c
                                                                    const int* __restrict__ members,
                                                                    float* __restrict__ word_sums) {
   __shared__ int starts[WORD_THREADS];
+  chain_wait();
+  chain_next();
   const int rows = *count;
   const int row = blockIdx.x;
   if (row >= rows) return;
@@ -1087,13 +1114,6 @@ __global__ void __launch_bounds__(WORD_THREADS) word_slices_kernel(int hidden, c
     __syncthreads();
   }
   if (col < hidden) *reinterpret_cast<float4*>(mine) = sum;
-}
-
-__global__ void __launch_bounds__(128) zero_ignored_kernel(const int* __restrict__ position, int hidden,
-                                                           __nv_bfloat16* __restrict__ grad_hidden) {
-  const long long token = blockIdx.x;
-  if (position[token] >= 0) return;
-  for (int c = threadIdx.x * 8; c < hidden; c += 128 * 8) st_16(grad_hidden + token * hidden + c, make_uint4(0, 0, 0, 0));
 }
 
 // ------------------------------------------------------------------------------------------- host
@@ -1154,9 +1174,7 @@ int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   const long long most = sm_count() / 2;
   // a product that is cut along k may have more units than tiles
   const int grid = static_cast<int>(2 * (KIND == GRAD_HIDDEN || tiles > most ? most : tiles));
-  head_gemm_kernel<KIND><<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(a, b, c, p);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(head_gemm_kernel<KIND>, dim3(grid), dim3(NUM_THREADS), SMEM_BYTES, stream, a, b, c, p);
 }
 
 long long up256(long long bytes) { return (bytes + 255) / 256 * 256; }
@@ -1197,10 +1215,8 @@ int launch_few(const CUtensorMap& words, const State& st, long long hidden, long
   static PerDeviceFlag configured{};
   if (int rc = allow_dynamic_smem(few_tokens_kernel<N>, Few<N>::SMEM, configured)) return rc;
   *parts = static_cast<int>(few_parts(p.n));
-  few_tokens_kernel<N><<<*parts / 4, Few<N>::THREADS, Few<N>::SMEM, stream>>>(words, rows, p.n, (p.k + BK - 1) / BK, p.count, p.labels,
-                                                                          p.partial, p.pitch, p.target_logit, p.status);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(few_tokens_kernel<N>, dim3(*parts / 4), dim3(Few<N>::THREADS), Few<N>::SMEM, stream, words, rows, p.n,
+                        (p.k + BK - 1) / BK, p.count, p.labels, p.partial, p.pitch, p.target_logit, p.status);
 }
 
 // A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size.
@@ -1313,15 +1329,11 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
     if (int rc = launch_product<STATS>(a, b, a, p, tiles_of(tokens) * tiles_of(vocab), s)) return rc;
     parts = static_cast<int>(2 * tiles_of(vocab));
   }
-  join_kernel<<<static_cast<unsigned>((tokens + 31) / 32), dim3(32, JOIN_SLICES), 0, s>>>(
-      partial, tokens, parts, st.count, st.labels, st.row_of, target_logit, st.lse, st.losses,
-      token_loss);
-  HMC_LAUNCH_OK();
-  if (reduction != HMC_REDUCE_NONE) {
-    reduce_kernel<<<1, 1024, 0, s>>>(st.losses, st.count, reduction == HMC_REDUCE_MEAN, loss);
-    HMC_LAUNCH_OK();
-  }
-  return 0;
+  if (int rc = launch_chained(join_kernel, dim3(static_cast<unsigned>((tokens + 31) / 32)), dim3(32, JOIN_SLICES), 0, s, partial, tokens,
+                              parts, st.count, st.labels, st.row_of, target_logit, st.lse, st.losses, token_loss))
+    return rc;
+  if (reduction == HMC_REDUCE_NONE) return 0;
+  return launch_chained(reduce_kernel, dim3(1), dim3(1024), 0, s, st.losses, st.count, reduction == HMC_REDUCE_MEAN, loss);
 }
 
 extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_t weight_stride, int64_t tokens, int64_t hidden,
@@ -1347,19 +1359,16 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
       grad_loss, reduction, st.count, st.labels, st.row_of, st.losses, w.weights, w.coef, w.scale,
       grad_weight != nullptr ? w.slots : nullptr, w.members);
   HMC_LAUNCH_OK();
-  if (grad_weight != nullptr) {
-    word_sums_kernel<<<static_cast<unsigned>(tokens), WORD_THREADS, 0, s>>>(st.packed, width, st.count, st.labels, w.coef,
-                                                                           w.slots, w.members, w.word_sums);
-    HMC_LAUNCH_OK();
-    if (tokens > WORD_SLICE) {
-      const dim3 grid(static_cast<unsigned>(tokens), (width / 4 + WORD_THREADS - 1) / WORD_THREADS);
-      word_slices_kernel<<<grid, WORD_THREADS, 0, s>>>(width, st.count, st.labels, w.slots, w.members, w.word_sums);
-      HMC_LAUNCH_OK();
-    }
-  }
-  if (grad_hidden != nullptr) {
-    zero_ignored_kernel<<<static_cast<unsigned>(tokens), 128, 0, s>>>(st.position, width, static_cast<__nv_bfloat16*>(grad_hidden));
-    HMC_LAUNCH_OK();
+  float* word_sums = grad_weight != nullptr ? w.word_sums : nullptr;
+  if (int rc = launch_chained(token_rows_kernel, dim3(static_cast<unsigned>(tokens)), dim3(WORD_THREADS), 0, s, st.packed, width, st.count,
+                              st.labels, w.coef, w.slots, w.members, word_sums, st.position,
+                              static_cast<__nv_bfloat16*>(grad_hidden)))
+    return rc;
+  if (grad_weight != nullptr && tokens > WORD_SLICE) {
+    const dim3 grid(static_cast<unsigned>(tokens), (width / 4 + WORD_THREADS - 1) / WORD_THREADS);
+    if (int rc = launch_chained(word_slices_kernel, grid, dim3(WORD_THREADS), 0, s, width, st.count, st.labels, w.slots, w.members,
+                                w.word_sums))
+      return rc;
   }
 
   Params base{};
@@ -1388,8 +1397,9 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
       p.part_sums = w.part_sums;
       const long long tiles = tiles_of(tokens) * tiles_of(width);
       if (int rc = launch_product<GRAD_HIDDEN>(probs_k, head_mn, probs_k, p, tiles, s)) return rc;
-      join_parts_kernel<<<dim3(TILE / 8, static_cast<unsigned>(cut_tiles(tiles))), 256, 0, s>>>(p, sm_count() / 2);
-      HMC_LAUNCH_OK();
+      if (int rc = launch_chained(join_parts_kernel, dim3(TILE / 8, static_cast<unsigned>(cut_tiles(tiles))), dim3(256), 0, s, p,
+                                  sm_count() / 2))
+        return rc;
     }
     if (grad_weight != nullptr) {
       CUtensorMap grad_store;
