@@ -940,20 +940,23 @@ __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __
   if (token_loss != nullptr) token_loss[row_of[row]] = loss;
 }
 
-// Sum (or mean) of the packed rows' losses by one block, in a fixed order.
+// Sum (or mean) of the packed rows' losses by one block, in a fixed order; in FP64, since a thread's share may be long.
 __global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ losses, const int* __restrict__ count, int mean,
                                                       float* __restrict__ loss) {
-  __shared__ float slots[32];
+  __shared__ double slots[32];
   chain_wait();
   const int rows = *count;
-  float v = 0.0f;
-  for (int i = threadIdx.x; i < rows; i += blockDim.x) v += losses[i];
-  v = warp_sum(v);
+  double v = 0.0;
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) v += static_cast<double>(losses[i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x >= 32) return;
-  v = warp_sum(slots[threadIdx.x]);
-  if (threadIdx.x == 0) *loss = mean ? v / static_cast<float>(rows) : v;  // no row: the mean is NaN
+  v = slots[threadIdx.x];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (threadIdx.x == 0) *loss = static_cast<float>(mean ? v / rows : v);  // no row: the mean is NaN
 }
 
 // ------------------------------------------------------------------------------------------- gradient

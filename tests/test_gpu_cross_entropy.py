@@ -277,6 +277,76 @@ def test_rows_of_the_output_are_written_and_nothing_else():
     assert (gx[70:] == 3).all() and (gw[300:] == 3).all() and (space[need:] == 0x5A).all()
 
 
+@pytest.mark.parametrize("tokens,hidden,vocab", [(70, 4096, 530_000), (530_000, 4096, 200)])
+def test_offsets_beyond_31_bits(tokens, hidden, vocab):
+    """A weight, and packed rows, of more than 2^31 values: the far end against the definition."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    weight = torch.randn(vocab, hidden, generator=g, device="cuda", dtype=torch.bfloat16).mul_(hidden ** -0.5)
+    x = torch.randn(1000, hidden, generator=g, device="cuda", dtype=torch.bfloat16).repeat(tokens // 1000 + 1, 1)[:tokens]
+    targets = torch.randint(0, vocab, (tokens,), generator=g, device="cuda")
+    targets[-1] = vocab - 1
+    loss, grad_x, grad_w = run(x, weight, targets, "none")
+    rows = slice(max(0, tokens - 300), tokens)
+    logits = x[rows].double() @ weight.double().t() if vocab < 1000 else torch.cat(
+        [x[rows].double() @ w.double().t() for w in weight.split(65536)], 1)
+    p = torch.softmax(logits, 1)
+    want = torch.logsumexp(logits, 1) - logits.gather(1, targets[rows].unsqueeze(1)).squeeze(1)
+    assert (loss[rows].double() - want).abs().max() <= 2.0 ** -14  # E = 256 * 2^-22 * 64 at the most, twice
+    p.scatter_add_(1, targets[rows].unsqueeze(1), torch.full_like(want, -1).unsqueeze(1))
+    far = sum(p[:, i:i + 65536] @ weight[i:i + 65536].double() for i in range(0, vocab, 65536))
+    assert (grad_x[rows].double() - far).norm() <= HALF * far.norm()
+    if tokens < 1000:  # a row of the weight's gradient needs every token
+        tail = p[:, -500:].t() @ x.double()
+        assert (grad_w[-500:].double() - tail).norm() <= HALF * tail.norm()
+    else:
+        whole = torch.zeros(vocab, hidden, dtype=torch.float64, device="cuda")
+        for at in range(0, tokens, 50_000):
+            part = slice(at, min(tokens, at + 50_000))
+            q = torch.softmax(x[part].double() @ weight.double().t(), 1)
+            q.scatter_add_(1, targets[part].unsqueeze(1), torch.full((q.shape[0], 1), -1.0, dtype=torch.float64, device="cuda"))
+            whole += q.t() @ x[part].double()
+        assert (grad_w.double() - whole).norm() <= HALF * whole.norm()
+
+
+def test_calls_from_two_threads_on_two_streams():
+    import threading
+
+    cases = [make(300, 128, 2000, ignored=0.2, seed=s) for s in (21, 22)]
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = run(*cases[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for mine, expected in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(mine, expected))
+
+
+def test_backward_twice_over_one_forward():
+    from hyper_multicore_b200 import mega_cross_entropy
+
+    x, weight, targets = make(100, 64, 700, ignored=0.2, seed=23)
+    a, b = x.detach().requires_grad_(True), weight.detach().requires_grad_(True)
+    loss = mega_cross_entropy(a, b, targets)
+    first = torch.autograd.grad(loss, (a, b), retain_graph=True)
+    second = torch.autograd.grad(loss, (a, b))
+    assert all(torch.equal(p, q) for p, q in zip(first, second))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss = mega_cross_entropy(a, b, targets)
+        with torch.no_grad():
+            b.mul_(2)
+        torch.autograd.grad(loss, b)
+
+
 def test_second_derivatives_and_batched_gradients_are_refused():
     from hyper_multicore_b200 import mega_cross_entropy
 

@@ -76,7 +76,8 @@ def run(x, weight, bias, grad, center, eps=1e-6):
 TYPES = [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
          (torch.float16, torch.float32), (torch.float32, torch.float32)]
 SIZES = [(1, 1), (3, 7), (5, 8), (700, 40), (2, 64), (33, 1000), (17, 1001), (1, 1024), (6, 1032), (300, 2560), (3, 4096),
-         (5, 4097), (9, 7168), (2, 8192), (3, 9000), (2, 33000)]
+         (5, 4097), (9, 7168), (2, 8192), (3, 9000),
+         (2, 16384), (2, 33000)]
 
 
 @pytest.mark.parametrize("center", [True, False])
@@ -91,8 +92,12 @@ def test_norm_and_gradients_match_the_definition(tokens, hidden, dtype, affine, 
 
 
 @pytest.mark.parametrize("center", [True, False])
-def test_many_rows_and_their_parameter_gradients(center):
-    x, weight, bias, grad = make(5000, 768, torch.bfloat16, torch.float32, center, seed=3)
+@pytest.mark.parametrize("tokens,hidden,dtype", [
+    (5000, 768, torch.bfloat16), (3000, 300, torch.bfloat16), (1501, 1001, torch.bfloat16), (1501, 1002, torch.float16),
+    (777, 3001, torch.float32), (900, 1536, torch.float16), (700, 3584, torch.bfloat16), (600, 5120, torch.float32),
+    (601, 8192, torch.bfloat16), (320, 12288, torch.bfloat16), (320, 9216, torch.float32), (500, 6145, torch.bfloat16)])
+def test_many_rows_and_their_parameter_gradients(center, tokens, hidden, dtype):
+    x, weight, bias, grad = make(tokens, hidden, dtype, torch.float32, center, seed=3)
     y, grads = run(x, weight, bias, grad, center)
     check(y, grads, x, weight, bias, grad, center, 1e-6)
     again = run(x, weight, bias, grad, center)
@@ -202,6 +207,56 @@ def test_rows_beyond_31_bits_of_elements():
     y, grads = run(x, torch.ones(hidden, device="cuda", dtype=torch.bfloat16), None, x, False)
     for rows in (slice(0, 64), slice(tokens - 64, tokens)):
         check(y[rows], [grads[0][rows], None, None], x[rows], None, None, x[rows], False, 1e-6)
+
+
+@pytest.mark.parametrize("dtype,hidden", [(torch.bfloat16, 2560), (torch.bfloat16, 1001), (torch.bfloat16, 300), (torch.float32, 520)])
+def test_nothing_is_written_behind_the_rows(dtype, hidden):
+    from hyper_multicore_b200 import _lib
+
+    rows, code = 700, _lib.HMC_DTYPE[dtype]
+    x, weight, bias, grad = make(rows, hidden, dtype, dtype, True, seed=hidden)
+    want = run(x, weight, bias, grad, True)
+    y, dx = (torch.full((rows + 3, hidden), 7.0, device="cuda", dtype=dtype) for _ in range(2))
+    mean, rstd = (torch.full((rows + 8,), 7.0, device="cuda") for _ in range(2))
+    dw, db = (torch.full((hidden + 8,), 7.0, device="cuda", dtype=dtype) for _ in range(2))
+    need = _lib.load().hmc_row_norm_grad_workspace_bytes(rows, hidden)
+    space = torch.full((need + 256,), 0x5A, dtype=torch.uint8, device="cuda")
+    _lib.launch("hmc_row_norm", x.device, x.data_ptr(), hidden, rows, hidden, code, weight.data_ptr(), bias.data_ptr(), code, 1,
+                1e-6, y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
+    _lib.launch("hmc_row_norm_grad", x.device, x.data_ptr(), hidden, grad.data_ptr(), hidden, rows, hidden, code, weight.data_ptr(),
+                code, 1, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), space.data_ptr(), need)
+    assert torch.equal(y[:rows], want[0]) and torch.equal(dx[:rows], want[1][0])
+    assert torch.equal(dw[:hidden], want[1][1]) and torch.equal(db[:hidden], want[1][2])
+    for guard in (y[rows:], dx[rows:], mean[rows:], rstd[rows:], dw[hidden:], db[hidden:]):
+        assert (guard == 7).all()
+    assert (space[need:] == 0x5A).all()
+
+
+def test_first_call_of_a_process_may_be_captured():
+    """Shared memory limits and residency are asked for at the first launch of a kernel: that may happen under capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from hyper_multicore_b200 import mega_cross_entropy, mega_layer_norm
+x = torch.randn(700, 2048, device="cuda").bfloat16().requires_grad_(True)
+w = torch.randn(1000, 2048, device="cuda").bfloat16().mul_(0.02).requires_grad_(True)
+t = torch.randint(0, 1000, (700,), device="cuda")
+def step():
+    loss = mega_cross_entropy(mega_layer_norm(x), w, t)
+    return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+torch.autograd.grad((x * 2).sum(), x)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+"""
+    root = Path(__file__).resolve().parent.parent
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
 
 
 def test_other_streams_and_captured_graphs():
