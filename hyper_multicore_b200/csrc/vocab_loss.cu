@@ -43,7 +43,9 @@ constexpr int STAGES = 6;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * STORE_STAGE_BYTES + 1024 + 256;
 constexpr int MAX_PARTS = 16;  // of a tile that is cut along k
 constexpr int MIN_PART = 8;    // k-blocks of a part, at the least
-constexpr int PROMOTE = 8;     // k-blocks that add up inside the tensor core before the sum goes to FP32 registers (STATS)
+// k-blocks that add up inside the tensor core before the sum goes to FP32 registers (STATS, few tokens). The loss of 8192 tokens
+// of 4096 over 131072 words: 8 7.63 ms, 16 7.30, 32 7.22, 64 (all of it) 6.85.
+constexpr int PROMOTE = 32;
 constexpr int BAND = 16; // tile rows that are walked together, so that a band's rows stay in L2 while the weight passes by (8, 16, 32: 29987, 29527, 31442 us for a training step of 8192 x 4096 x 131072)
 
 enum Product { STATS, PROBS, GRAD_HIDDEN, GRAD_WEIGHT };
@@ -58,7 +60,6 @@ struct Params {
   const float* coef;   // [rows] weight * (p_target - 1)
   float2* partial;     // STATS: [2 * n_tiles][pitch] maximum and sum
   long long pitch;
-  float* target_logit;  // STATS
   int first_word;       // PROBS, GRAD_*: first word of the piece
   const int* row_of;    // GRAD_HIDDEN: token of a packed row
   float* sums;          // GRAD_HIDDEN: [rows, n] FP32 sums over pieces, or NULL
@@ -126,7 +127,7 @@ struct Walker {
 
 __device__ __forceinline__ float shifted_exp(float v, float top) { return __expf(v - top); }
 
-// Maximum and sum of exponentials of one row's 128 columns; the target's logit where it lies among them.
+// Maximum and sum of exponentials of one row's 128 columns, without the target's.
 __device__ __forceinline__ void epilogue_stats(const Params& p, float (&v)[HALF], int row, int col, int half_tile) {
   const int label = p.labels[row] - col;
   if (col + HALF > p.n) {
@@ -135,11 +136,9 @@ __device__ __forceinline__ void epilogue_stats(const Params& p, float (&v)[HALF]
       if (col + j >= p.n) v[j] = -INFINITY;
   }
   if (label >= 0 && label < HALF) {
-    float own = 0.0f;
 #pragma unroll
     for (int j = 0; j < HALF; ++j)
-      if (j == label) own = v[j];
-    p.target_logit[row] = own;
+      if (j == label) v[j] = -INFINITY;
   }
   float high[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
@@ -519,8 +518,8 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         continue;
       }
       if (KIND == STATS) {
-        // The tensor core's sums lose about half a step per addition, always towards zero: over a whole row of 4096 that is
-        // 2.5e-6 of the loss against 5e-7 in FP32. So PROMOTE k-blocks at a time are added up in registers.
+        // The tensor core's sums lose about half a step per addition, always towards zero, so PROMOTE k-blocks at a time are
+        // added up in FP32 registers. Reading an accumulator holds up the MMAs into the other one for about 250 cycles.
         float v[HALF];
 #pragma unroll
         for (int j = 0; j < HALF; ++j) v[j] = 0.0f;
@@ -606,7 +605,7 @@ template <int N>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Few<N>::THREADS, 1)
 few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_constant__ CUtensorMap tm_tokens, int vocab, int kiters,
                   const int* __restrict__ count, const int* __restrict__ labels, float2* __restrict__ partial, long long pitch,
-                  float* __restrict__ target_logit, int* status) {
+                  int* status) {
   using F = Few<N>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -644,20 +643,27 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
   cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA signal
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  chain_wait();
+  if (warp != 0) chain_wait();
   chain_next();
-  const int rows = *count;
-  const int last = rows > 0 ? tiles : 0;  // no token counts: nothing to do
 
   if (warp == 0) {
     // ======================================================================== TMA producer (both CTAs)
+    // The weight does not come from this chain of launches: its first pieces are on their way before the tokens are packed.
     if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
+      const int first = pair * TILE + static_cast<int>(rank) * HALF, early = pair < tiles ? min(F::STAGES, kiters) : 0;
+      for (int kb = 0; kb < early; ++kb) {
+        if (rank == 0) mbar_arrive_expect_tx(&full_bar[kb], 2 * F::STAGE);
+        tma_load_2d_pair(smem + kb * F::STAGE, &tm_words, &full_bar[kb], kb * BK, first);
+      }
+      chain_wait();
+      for (int kb = 0; kb < early; ++kb)
+        tma_load_2d_pair(smem + kb * F::STAGE + A_TILE_BYTES, &tm_tokens, &full_bar[kb], kb * BK, static_cast<int>(rank) * (N / 2));
+      int stage = early % F::STAGES;
+      uint32_t phase = early == F::STAGES ? 1 : 0;
       bool ok = true;
-      for (int t = pair; ok && t < last; t += pairs) {
+      for (int t = pair; ok && t < tiles; t += pairs) {
         const int word = t * TILE + static_cast<int>(rank) * HALF;
-        for (int kb = 0; kb < kiters; ++kb) {
+        for (int kb = t == pair ? early : 0; kb < kiters; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
             report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 0, stage, kb);
             ok = false;
@@ -684,7 +690,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
       uint32_t acc_phase = 0;
       bool ok = true;
       constexpr uint32_t idesc = make_idesc_f32acc(1u, TILE, N, HMC_MAJOR_K, HMC_MAJOR_K);
-      for (int t = pair; ok && t < last; t += pairs) {
+      for (int t = pair; ok && t < tiles; t += pairs) {
         for (int first = 0; ok && first < kiters; first += PROMOTE) {
           const int end = min(kiters, first + PROMOTE);
           if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
@@ -736,6 +742,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
     const int col = (warp - 2) / 4 * C;  // this warp's first token
     const uint32_t leader_acc_empty = map_to_cta(smem_u32(acc_empty_bar), 0);
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(col);
+    const int rows = *count;
     float top[OWN], sum[OWN];  // of column lane * OWN + i over this warp's words so far
     int label[OWN];
 #pragma unroll
@@ -744,7 +751,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
       const int token = col + lane * OWN + i;
       label[i] = token < rows ? labels[token] : -1;
     }
-    for (int t = pair; ok && t < last; t += pairs) {
+    for (int t = pair; ok && t < tiles; t += pairs) {
       float v[C];
 #pragma unroll
       for (int j = 0; j < C; ++j) v[j] = 0.0f;
@@ -776,7 +783,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         if (word >= vocab) v[j] = -INFINITY;
-        if (__shfl_sync(0xffffffffu, label[j % OWN], j / OWN) == word) target_logit[col + j] = v[j];
+        if (__shfl_sync(0xffffffffu, label[j % OWN], j / OWN) == word) v[j] = -INFINITY;  // the target is joined in FP32
       }
       float high[OWN], part[OWN];
       reduce_columns<C, true>(v, high, lane);
@@ -837,15 +844,18 @@ __device__ __forceinline__ int block_count(int v) {  // sum over the block, in e
   return v;
 }
 
-// The tokens that count, in their order, as rows without gaps. A block finds its place by counting the targets before
+// The tokens that count, in their order, as rows without gaps, and the logit of each one's target by FP32 multiply-adds: it
+// enters the loss with its whole weight, where an error of the tensor core's sums would show. A block finds its place by counting the targets before
 // its own; the last one writes the number of rows and clears the rows up to the next k-block of a contraction over them.
 __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bfloat16* __restrict__ x, long long x_stride,
                                                                  Targets targets, long long tokens, int hidden, int vector,
                                                                  int* __restrict__ count, int* __restrict__ position,
                                                                  int* __restrict__ row_of, int* __restrict__ labels,
                                                                  __nv_bfloat16* __restrict__ packed,
+                                                                 const __nv_bfloat16* __restrict__ head, long long head_stride,
+                                                                 float* __restrict__ target_logit,
                                                                  float* __restrict__ token_loss) {
-  __shared__ int place[PACK_TOKENS];
+  __shared__ int place[PACK_TOKENS], known[PACK_TOKENS];  // packed row and target of a token, -1: none
   chain_next();  // the first of its chain
   const long long first = static_cast<long long>(blockIdx.x) * PACK_TOKENS;
   int before = 0;
@@ -857,11 +867,12 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
     const bool counts = i < tokens && target != targets.ignored;
     const unsigned mask = __ballot_sync(0xffffffffu, counts);
     const int at = before + __popc(mask & ((1u << threadIdx.x) - 1u));
-    if (threadIdx.x < PACK_TOKENS) place[threadIdx.x] = counts ? at : -1;
+    const int label = counts && target >= 0 && target < targets.vocab ? static_cast<int>(target) : -1;
+    if (threadIdx.x < PACK_TOKENS) place[threadIdx.x] = counts ? at : -1, known[threadIdx.x] = label;
     if (i < tokens) position[i] = counts ? at : -1;
     if (counts) {
       row_of[at] = static_cast<int>(i);
-      labels[at] = target >= 0 && target < targets.vocab ? static_cast<int>(target) : -1;
+      labels[at] = label;
     } else if (i < tokens && token_loss != nullptr) {
       token_loss[i] = 0.0f;
     }
@@ -871,13 +882,29 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
   if (place[warp] >= 0) {
     const __nv_bfloat16* src = x + (first + warp) * x_stride;
     __nv_bfloat16* dst = packed + static_cast<long long>(place[warp]) * hidden;
-    if (vector) {
-#pragma unroll 8
-      for (int c = lane * 8; c < hidden; c += 256) st_16(dst + c, ld_nc_16(src + c));
-    } else {
-#pragma unroll 8
-      for (int c = lane; c < hidden; c += 32) dst[c] = src[c];
+    const __nv_bfloat16* word = known[warp] >= 0 ? head + known[warp] * head_stride : nullptr;
+    float2 dot = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for (int c = lane * 8; c < hidden; c += 256) {
+      uint4 q;
+      if (vector) {
+        q = ld_nc_16(src + c);
+      } else {
+        const uint16_t* bits = reinterpret_cast<const uint16_t*>(src + c);
+        q.x = bits[0] | static_cast<uint32_t>(bits[1]) << 16, q.y = bits[2] | static_cast<uint32_t>(bits[3]) << 16;
+        q.z = bits[4] | static_cast<uint32_t>(bits[5]) << 16, q.w = bits[6] | static_cast<uint32_t>(bits[7]) << 16;
+      }
+      st_16(dst + c, q);
+      if (word != nullptr) {
+        const uint4 w = ld_nc_16(word + c);
+        dot = fma2(unpack_bf16x2(q.x), unpack_bf16x2(w.x), dot);
+        dot = fma2(unpack_bf16x2(q.y), unpack_bf16x2(w.y), dot);
+        dot = fma2(unpack_bf16x2(q.z), unpack_bf16x2(w.z), dot);
+        dot = fma2(unpack_bf16x2(q.w), unpack_bf16x2(w.w), dot);
+      }
     }
+    const float logit = warp_sum(dot.x + dot.y);
+    if (lane == 0) target_logit[place[warp]] = logit;
   }
   if (blockIdx.x != gridDim.x - 1) return;
   int rows = 0;
@@ -929,12 +956,15 @@ __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __
   __syncthreads();
   if (threadIdx.y != 0 || !ok) return;
   for (int s = 1; s < JOIN_SLICES; ++s) top = fmaxf(top, sums[s][threadIdx.x].x);
-  const float shift = top == -INFINITY ? 0.0f : top;
+  // the target's logit joins the others here: loss = log(1 + sum over the others exp(l_j - l_target))
+  const float own = target_logit[row], shift = fmaxf(top, own);
   sum = 0.0f;
   for (int s = 0; s < JOIN_SLICES; ++s) sum += sums[s][threadIdx.x].y * shifted_exp(sums[s][threadIdx.x].x, shift);
-  const float log_sum = logf(sum);
-  // a target outside the vocabulary has no loss: NaN, which no later sum hides
-  const float loss = labels[row] >= 0 ? log_sum + (shift - target_logit[row]) : __int_as_float(0x7fffffff);
+  const float log_sum = own >= top ? log1pf(sum) : logf(sum + shifted_exp(own, shift));
+  float loss = log_sum + (shift - own);
+  // a target outside the vocabulary has no loss, and neither has a row whose largest logit is infinite: NaN, which no
+  // later sum hides
+  if (labels[row] < 0 || isinf(shift)) loss = __int_as_float(0x7fffffff);
   lse[row] = shift + log_sum;
   losses[row] = loss;
   if (token_loss != nullptr) token_loss[row_of[row]] = loss;
@@ -1219,7 +1249,7 @@ int launch_few(const CUtensorMap& words, const State& st, long long hidden, long
   if (int rc = allow_dynamic_smem(few_tokens_kernel<N>, Few<N>::SMEM, configured)) return rc;
   *parts = static_cast<int>(few_parts(p.n));
   return launch_chained(few_tokens_kernel<N>, dim3(*parts / 4), dim3(Few<N>::THREADS), Few<N>::SMEM, stream, words, rows, p.n,
-                        (p.k + BK - 1) / BK, p.count, p.labels, p.partial, p.pitch, p.target_logit, p.status);
+                        (p.k + BK - 1) / BK, p.count, p.labels, p.partial, p.pitch, p.status);
 }
 
 // A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size.
@@ -1313,12 +1343,12 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
   const int vector = aligned16(x) && x_stride % 8 == 0;
   pack_rows_kernel<<<static_cast<unsigned>((tokens + PACK_TOKENS - 1) / PACK_TOKENS), PACK_THREADS, 0, s>>>(
       static_cast<const __nv_bfloat16*>(x), x_stride, given, tokens, static_cast<int>(hidden), vector, st.count, st.position,
-      st.row_of, st.labels, st.packed, token_loss);
+      st.row_of, st.labels, st.packed, static_cast<const __nv_bfloat16*>(weight), weight_stride, target_logit, token_loss);
   HMC_LAUNCH_OK();
 
   Params p{};
   p.n = static_cast<int>(vocab), p.k = static_cast<int>(hidden);
-  p.count = st.count, p.labels = st.labels, p.partial = partial, p.pitch = tokens, p.target_logit = target_logit, p.status = status;
+  p.count = st.count, p.labels = st.labels, p.partial = partial, p.pitch = tokens, p.status = status;
   CUtensorMap a, b;
   if (int rc = map_k_major(&b, weight, hidden, vocab, weight_stride)) return rc;
   int parts = 0;

@@ -763,44 +763,60 @@ def _size(name: str, *extents: int) -> int:
     return getattr(_lib.load(), name)(*extents)
 
 
-def row_norm(x, weight, bias, *, center: bool, eps: float, keep: bool):
+def row_norm(x, weight, bias, center: bool, eps: float, keep: bool, device: torch.device | None = None):
     """Layer norm (``center``) or RMSNorm of the rows of ``x`` [T, H] (rows any distance apart, values adjacent).
 
-    Returns (y [T, H], stats | None): with ``keep`` the FP32 statistics, rstd [T] behind mean [T] where there is one.
+    Returns (y [T, H], stats | None): with ``keep`` the FP32 statistics, rstd [T] behind mean [T] where there is one. A caller
+    that has found all tensors on one CUDA ``device`` passes it.
     """
-    device = _require_cuda(x, weight, bias)
+    if device is None:
+        device = _require_cuda(x, weight, bias)
     rows, hidden = x.shape
     dtype = x.dtype
     y = torch.empty((rows, hidden), dtype=dtype, device=device)
-    stats = mean = rstd = None
+    stats = mean = rstd = w = b = None
     if keep:
         stats = torch.empty(2 * rows if center else rows, dtype=torch.float32, device=device)
         rstd = stats.data_ptr()
         if center:
             mean, rstd = rstd, rstd + 4 * rows
-    affine = dtype if weight is None and bias is None else bias.dtype if weight is None else weight.dtype
-    _call("hmc_row_norm", device, x.data_ptr(), x.stride(0), rows, hidden, _lib.HMC_DTYPE[dtype], _lib.ptr(weight), _lib.ptr(bias),
-          _lib.HMC_DTYPE[affine], center, eps, y.data_ptr(), mean, rstd)
+    affine = dtype
+    if weight is not None:
+        w, affine = weight.data_ptr(), weight.dtype
+    if bias is not None:
+        b, affine = bias.data_ptr(), bias.dtype
+    codes = _lib.HMC_DTYPE
+    _call("hmc_row_norm", device, x.data_ptr(), x.stride(0), rows, hidden, codes[dtype], w, b, codes[affine], center, eps,
+          y.data_ptr(), mean, rstd)
     return y, stats
 
 
-def row_norm_grad(grad, x, weight, stats, *, center: bool, affine_dtype, need_x: bool, need_weight: bool, need_bias: bool):
+def row_norm_grad(grad, x, weight, stats, center: bool, affine_dtype, need_x: bool, need_weight: bool, need_bias: bool):
     """Gradients of ``row_norm``: (grad_x [T, H], grad_weight [H], grad_bias [H]), None where not needed."""
-    device = _require_cuda(grad, x, weight, stats)
+    device = _require_cuda(grad, x)
     rows, hidden = x.shape
-    grad_x = torch.empty((rows, hidden), dtype=x.dtype, device=device) if need_x else None
-    grad_weight = torch.empty(hidden, dtype=affine_dtype, device=device) if need_weight else None
-    grad_bias = torch.empty(hidden, dtype=affine_dtype, device=device) if need_bias else None
-    need, workspace = 0, None
+    dtype = x.dtype
+    need = 0
+    grad_x = grad_weight = grad_bias = workspace = dx = dw = db = space = mean = None
+    if need_x:
+        grad_x = torch.empty((rows, hidden), dtype=dtype, device=device)
+        dx = grad_x.data_ptr()
+    if need_weight:
+        grad_weight = torch.empty(hidden, dtype=affine_dtype, device=device)
+        dw = grad_weight.data_ptr()
+    if need_bias:
+        grad_bias = torch.empty(hidden, dtype=affine_dtype, device=device)
+        db = grad_bias.data_ptr()
     if need_weight or need_bias:
         need = _size("hmc_row_norm_grad_workspace_bytes", rows, hidden)
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    rstd, mean = stats.data_ptr(), None
+        space = workspace.data_ptr()
+    rstd = stats.data_ptr()
     if center:
         mean, rstd = rstd, rstd + 4 * rows
-    _call("hmc_row_norm_grad", device, x.data_ptr(), x.stride(0), grad.data_ptr(), grad.stride(0), rows, hidden,
-          _lib.HMC_DTYPE[x.dtype], _lib.ptr(weight), _lib.HMC_DTYPE[affine_dtype], center, mean, rstd, _lib.ptr(grad_x),
-          _lib.ptr(grad_weight), _lib.ptr(grad_bias), _lib.ptr(workspace), need)
+    codes = _lib.HMC_DTYPE
+    _call("hmc_row_norm_grad", device, x.data_ptr(), x.stride(0), grad.data_ptr(), grad.stride(0), rows, hidden, codes[dtype],
+          None if weight is None else weight.data_ptr(), codes[affine_dtype], center, mean, rstd, dx, dw, db, space, need)
     return grad_x, grad_weight, grad_bias
 
 

@@ -19,20 +19,19 @@ def _fits(x, weight, bias, eps) -> bool:
     """All of ``_validate`` in one expression, which builds no message; that one then says what is wrong."""
     if type(x) is not torch.Tensor or not x.is_cuda or x.ndim == 0 or type(eps) is not float or not 0.0 <= eps < math.inf:
         return False
-    shape, dtype, device = x.shape, x.dtype, x.device
-    hidden = shape[-1]
+    dtype, hidden = x.dtype, x.shape[-1]
     if not (1 <= hidden <= _lib.HMC_NORM_MAX_HIDDEN and x.numel() < hidden << 31 and dtype in _lib.HMC_DTYPE):
         return False
-    for parameter in (weight, bias):
-        if parameter is not None and not (isinstance(parameter, torch.Tensor) and parameter.shape == shape[-1:]
-                                          and parameter.dtype in (dtype, torch.float32) and parameter.device == device):
-            return False
-    return weight is None or bias is None or weight.dtype == bias.dtype
+    if weight is not None and not (isinstance(weight, torch.Tensor) and weight.ndim == 1 and weight.shape[0] == hidden
+                                   and weight.dtype in (dtype, torch.float32) and weight.device == x.device):
+        return False
+    if bias is None:
+        return True
+    return (isinstance(bias, torch.Tensor) and bias.ndim == 1 and bias.shape[0] == hidden and bias.device == x.device
+            and bias.dtype in ((dtype, torch.float32) if weight is None else (weight.dtype,)))
 
 
 def _validate(x, weight, bias, eps) -> None:
-    if _fits(x, weight, bias, eps):
-        return
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a Tensor.")
     if x.dtype not in _lib.HMC_DTYPE:
@@ -79,9 +78,8 @@ class _RowNormFunction(torch.autograd.Function):
         rows, weight, stats = ctx.saved_tensors
         need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
         grad = as_rows(plain_grad(grad, "a row norm's backward"), rows.shape[1])
-        grad_x, grad_weight, grad_bias = kernels.row_norm_grad(
-            grad, rows, weight, stats, center=ctx.center, affine_dtype=ctx.affine_dtype, need_x=need_x, need_weight=need_weight,
-            need_bias=need_bias)
+        grad_x, grad_weight, grad_bias = kernels.row_norm_grad(grad, rows, weight, stats, ctx.center, ctx.affine_dtype, need_x,
+                                                               need_weight, need_bias)
         if need_x and len(ctx.shape) != 2:
             grad_x = grad_x.view(ctx.shape)
         return grad_x, grad_weight, grad_bias, None, None
@@ -94,12 +92,13 @@ def _forward(x, weight, bias, center, eps, keep):
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    y, stats = kernels.row_norm(rows, weight, bias, center=center, eps=eps, keep=keep)
+    y, stats = kernels.row_norm(rows, weight, bias, center, eps, keep, x.device)
     return y if x.ndim == 2 else y.view(x.shape), rows, weight, bias, stats
 
 
 def _norm(x, weight, bias, center, eps):
-    _validate(x, weight, bias, eps)
+    if not _fits(x, weight, bias, eps):
+        _validate(x, weight, bias, eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _RowNormFunction.apply(x, weight, bias, center, float(eps))
