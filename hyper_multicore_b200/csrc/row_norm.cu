@@ -249,26 +249,28 @@ __device__ __forceinline__ float2 madd2(float2 a, float2 b, float2 c) {
 constexpr int STREAM_THREADS = 512;
 constexpr int STREAM_WARPS = STREAM_THREADS / 32;
 
-// row_sum for at most WARPS warps: every thread reads the slots four at a time, the unused ones are zero.
-template <int WARPS = STREAM_WARPS, int N>
-__device__ __forceinline__ void block_sum(float (&v)[N], float* slots) {
+// Sums over a block of at most STREAM_WARPS warps, in an order of their own: the warp's by halving, one slot per warp (the unused
+// ones are zero), and 16 lanes each over the slots. Two calls in a row use different slots, as in row_sum.
+__device__ __forceinline__ float over_16_lanes(float v) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) slots[i * WARPS + (threadIdx.x >> 5)] = v[i];
-  }
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float block_sum(float v, float* slots) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float4 q[WARPS / 4];
-#pragma unroll
-    for (int w = 0; w < WARPS / 4; ++w) q[w] = reinterpret_cast<const float4*>(slots + i * WARPS)[w];
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WARPS / 4; ++w) sum += (q[w].x + q[w].y) + (q[w].z + q[w].w);
-    v[i] = sum;
-  }
+  return over_16_lanes(slots[threadIdx.x & 15]);
+}
+// Of two values at once: the lower 16 lanes take the first, the upper ones the second.
+__device__ __forceinline__ float2 block_sum(float2 v, float* slots) {
+  const bool upper = (threadIdx.x & 16) != 0;
+  float mine = (upper ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+  mine = over_16_lanes(mine);
+  if ((threadIdx.x & 15) == 0) slots[(threadIdx.x & 16) + (threadIdx.x >> 5)] = mine;
+  __syncthreads();
+  mine = over_16_lanes(slots[threadIdx.x & 31]);
+  return make_float2(__shfl_sync(0xffffffffu, mine, 0), __shfl_sync(0xffffffffu, mine, 16));
 }
 
 // A block walks the rows blockIdx.x, + gridDim.x, ... and copies the next ones asynchronously while it works on one: a ring
@@ -305,21 +307,28 @@ stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
     if (here[j] && weight != nullptr) widen_params<W, PAIRS>(weight + at * VEC, w[j]);
     if (CENTER && here[j] && bias != nullptr) widen_params<W, PAIRS>(bias + at * VEC, b[j]);
   }
-  const T* mine = x + threadIdx.x * VEC;
-  auto fetch = [&](long long row, int stage) {
-    if (row < rows) {
-      const T* src = mine + row * x_stride;
+  // rows are counted down in 32 bits and pointers moved on: 64-bit products per row cost more than the row's arithmetic
+  const int step = gridDim.x;
+  const T* src = x + blockIdx.x * x_stride + threadIdx.x * VEC;
+  T* dst = y + static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
+  const long long src_step = step * x_stride, dst_step = static_cast<long long>(step) * hidden;
+  int ahead = blockIdx.x;  // the next row to copy
+  const int end = static_cast<int>(rows);
+  auto fetch = [&](int stage) {
+    if (ahead < end) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (here[j]) copy_async_16(ring + stage * width + j * threads, src + j * threads * VEC);
+      src += src_step;
+      ahead += step;
     }
     copy_async_commit();
   };
-  for (int s = 0; s < stages - 1; ++s) fetch(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  for (int s = 0; s < stages - 1; ++s) fetch(s);
   __syncthreads();  // the slots are zero
-  int stage = 0, last = stages - 1;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    fetch(row + static_cast<long long>(stages - 1) * gridDim.x, last);
+  int stage = 0, last = stages - 1, turn = 0;
+  for (int row = blockIdx.x; row < end; row += step, dst += dst_step) {
+    fetch(last);
     copy_async_wait<stages - 1>();  // the copies of a row are one group
     float2 v[NV][PAIRS];
     float2 part[2] = {both(0.0f), both(0.0f)};
@@ -336,9 +345,8 @@ stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
     float mean = 0.0f;
     if (CENTER) {
       const float2 all = add2(part[0], part[1]);
-      float sum[1] = {all.x + all.y};
-      block_sum(sum, slots[0]);
-      mean = sum[0] * scale;
+      mean = block_sum(all.x + all.y, slots[turn]) * scale;
+      turn ^= 1;
       part[0] = part[1] = both(0.0f);
     }
 #pragma unroll
@@ -351,11 +359,8 @@ stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
         }
       }
     const float2 all = add2(part[0], part[1]);
-    float square[1] = {all.x + all.y};
-    // a centred row has two reductions and so a barrier between two uses of a slot; the others alternate
-    block_sum(square, slots[CENTER ? 1 : (row / gridDim.x) & 1]);
-    const float rstd = rsqrtf(square[0] * scale + eps);
-    T* dst = y + row * hidden + threadIdx.x * VEC;
+    const float rstd = rsqrtf(block_sum(all.x + all.y, slots[turn]) * scale + eps);
+    turn ^= 1;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (here[j]) {
@@ -416,33 +421,40 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
     for (int i = 0; i < PAIRS; i += 2)
       gain[(j * PAIRS + i) / 2 * PITCH] = make_float4(w[i].x, w[i].y, w[i + 1].x, w[i + 1].y);
   }
-  const T *mine_x = x + threadIdx.x * VEC, *mine_grad = grad + threadIdx.x * VEC;
-  auto fetch = [&](long long row, int stage) {
-    if (row < rows) {
-      const T *a = mine_x + row * x_stride, *d = mine_grad + row * grad_stride;
-      uint4* dst = ring + stage * 2 * WIDTH;
+  const int step = gridDim.x, end = static_cast<int>(rows);
+  const T *src_x = x + blockIdx.x * x_stride + threadIdx.x * VEC, *src_grad = grad + blockIdx.x * grad_stride + threadIdx.x * VEC;
+  T* dst = grad_x + static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
+  const long long x_step = step * x_stride, grad_step = step * grad_stride, dst_step = static_cast<long long>(step) * hidden;
+  int ahead = blockIdx.x;  // the next row to copy
+  auto fetch = [&](int stage) {
+    if (ahead < end) {
+      uint4* to = ring + stage * 2 * WIDTH;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (here[j]) {
-          copy_async_16(dst + j * PITCH, a + j * threads * VEC);
-          copy_async_16(dst + WIDTH + j * PITCH, d + j * threads * VEC);
+          copy_async_16(to + j * PITCH, src_x + j * threads * VEC);
+          copy_async_16(to + WIDTH + j * PITCH, src_grad + j * threads * VEC);
         }
+      src_x += x_step, src_grad += grad_step;
+      ahead += step;
     }
     copy_async_commit();
   };
-  for (int s = 0; s < stages - 1; ++s) fetch(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  for (int s = 0; s < stages - 1; ++s) fetch(s);
   __syncthreads();  // the slots are zero
   int stage = 0, last = stages - 1, turn = 0;
-  float next_mean = CENTER && blockIdx.x < rows ? mean_in[blockIdx.x] : 0.0f;
-  float next_rstd = blockIdx.x < rows ? rstd_in[blockIdx.x] : 0.0f;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
-    const float mean = next_mean, rstd = next_rstd;
-    const long long next = row + gridDim.x;
-    if (next < rows) {
-      if (CENTER) next_mean = mean_in[next];
-      next_rstd = rstd_in[next];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto stats = [&](int row) {
+    if (row < end) {
+      if (CENTER) next_mean = mean_in[row];
+      next_rstd = rstd_in[row];
     }
-    fetch(row + static_cast<long long>(stages - 1) * gridDim.x, last);
+  };
+  stats(blockIdx.x);
+  for (int row = blockIdx.x; row < end; row += step, turn ^= 1, dst += dst_step) {
+    const float mean = next_mean, rstd = next_rstd;
+    stats(row + step);
+    fetch(last);
     copy_async_wait<stages - 1>();
     const uint4* src = ring + stage * 2 * WIDTH;
     float2 along = both(0.0f), total = both(0.0f);  // rstd times the sums of g (x - mean) and of g
@@ -473,14 +485,12 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
           if (CENTER) total = add2(total, d[i]);
         }
       }
-    float sums[SUMS];
-    sums[0] = along.x + along.y;
-    if (CENTER) sums[SUMS - 1] = total.x + total.y;
-    block_sum(sums, slots[turn]);
+    float2 sums = make_float2(along.x + along.y, total.x + total.y);
+    if (CENTER) sums = block_sum(sums, slots[turn]);
+    else sums.x = block_sum(sums.x, slots[turn]);
     if (grad_x != nullptr) {
-      T* dst = grad_x + row * hidden + threadIdx.x * VEC;
       // dx = rstd g - (x - mean) rstd^2 mean(g u) - rstd mean(g), u = (x - mean) rstd
-      const float2 back = both(-sums[0] * scale * rstd * rstd), offset = both(CENTER ? -sums[SUMS - 1] * scale : 0.0f);
+      const float2 back = both(-sums.x * scale * rstd * rstd), offset = both(CENTER ? -sums.y * scale : 0.0f);
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (here[j]) {
@@ -598,13 +608,12 @@ stream_longest_grad_kernel(const T* __restrict__ x, long long x_stride, const T*
           if (CENTER) total = add2(total, d);
         }
       }
-    float sums[SUMS];
-    sums[0] = along.x + along.y;
-    if (CENTER) sums[SUMS - 1] = total.x + total.y;
-    block_sum(sums, slots[turn]);
+    float2 sums = make_float2(along.x + along.y, total.x + total.y);
+    if (CENTER) sums = block_sum(sums, slots[turn]);
+    else sums.x = block_sum(sums.x, slots[turn]);
     if (grad_x != nullptr) {
       T* dst = grad_x + row * hidden + threadIdx.x * VEC;
-      const float2 back = both(-sums[0] * scale * rstd), offset = both(CENTER ? -sums[SUMS - 1] * scale * rstd : 0.0f);
+      const float2 back = both(-sums.x * scale * rstd), offset = both(CENTER ? -sums.y * scale * rstd : 0.0f);
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (here[j]) {
@@ -675,7 +684,7 @@ window_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
                    const W* __restrict__ bias, float eps, T* __restrict__ y, float* __restrict__ mean_out,
                    float* __restrict__ rstd_out, int stages, int window) {
   extern __shared__ uint4 ring_raw[];
-  __shared__ __align__(16) float slots[2][WINDOW_WARPS];
+  __shared__ float slots[2][WINDOW_WARPS];
   uint8_t* ring = reinterpret_cast<uint8_t*>(ring_raw);
   const int threads = blockDim.x, packs = hidden / VEC, bytes = hidden * static_cast<int>(sizeof(T));
   const float scale = 1.0f / static_cast<float>(hidden);
@@ -705,7 +714,7 @@ window_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
     __syncthreads();
     const T* src = reinterpret_cast<const T*>(ring + stage * window + window_shift(x + row * x_stride)) + threadIdx.x * VEC;
     float v[NV][VEC];
-    float sum[1] = {0.0f};
+    float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
@@ -715,27 +724,25 @@ window_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           v[j][e] = widen(in.v[e]);
-          sum[0] += v[j][e];
+          sum += v[j][e];
         }
       }
     }
     float mean = 0.0f;
     if (CENTER) {
-      block_sum<WINDOW_WARPS>(sum, slots[turn]);
+      mean = block_sum(sum, slots[turn]) * scale;
       turn ^= 1;
-      mean = sum[0] * scale;
     }
-    float square[1] = {0.0f};
+    float square = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         if (CENTER) v[j][e] = here[j] ? v[j][e] - mean : 0.0f;
-        square[0] += v[j][e] * v[j][e];
+        square += v[j][e] * v[j][e];
       }
-    block_sum<WINDOW_WARPS>(square, slots[turn]);
+    const float rstd = rsqrtf(block_sum(square, slots[turn]) * scale + eps);
     turn ^= 1;
-    const float rstd = rsqrtf(square[0] * scale + eps);
     T* dst = y + row * hidden + threadIdx.x * VEC;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -807,7 +814,7 @@ window_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
     const T* a = reinterpret_cast<const T*>(at + window_shift(x + row * x_stride)) + threadIdx.x * VEC;
     const T* d = reinterpret_cast<const T*>(at + window + window_shift(grad + row * grad_stride)) + threadIdx.x * VEC;
     float u[NV][VEC], g[NV][VEC];
-    float sums[2] = {0.0f, 0.0f};  // of g * u and of g
+    float2 sums = make_float2(0.0f, 0.0f);  // of g * u and of g
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (here[j]) {
@@ -819,15 +826,15 @@ window_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
           sum_weight[j][e] += dv * u[j][e];
           if (CENTER) sum_bias[j][e] += dv;
           g[j][e] = dv * w[j][e];
-          sums[0] += g[j][e] * u[j][e];
-          sums[1] += g[j][e];
+          sums.x += g[j][e] * u[j][e];
+          sums.y += g[j][e];
         }
       }
-    block_sum<WINDOW_WARPS>(sums, slots[turn]);
+    sums = block_sum(sums, slots[turn]);
     last = stage;
     if (++stage == stages) stage = 0;
     if (grad_x == nullptr) continue;
-    const float along = sums[0] * scale, offset = CENTER ? sums[1] * scale : 0.0f;
+    const float along = sums.x * scale, offset = CENTER ? sums.y * scale : 0.0f;
     T* dst = grad_x + row * hidden + threadIdx.x * VEC;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
