@@ -849,7 +849,8 @@ __device__ __forceinline__ int block_count(int v) {  // sum over the block, in e
 // its own; the last one writes the number of rows and clears the rows up to the next k-block of a contraction over them.
 __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bfloat16* __restrict__ x, long long x_stride,
                                                                  Targets targets, long long tokens, int hidden, int vector,
-                                                                 int* __restrict__ count, int* __restrict__ position,
+                                                                 int* __restrict__ count, int* __restrict__ done,
+                                                                 int* __restrict__ position,
                                                                  int* __restrict__ row_of, int* __restrict__ labels,
                                                                  __nv_bfloat16* __restrict__ packed,
                                                                  const __nv_bfloat16* __restrict__ head, long long head_stride,
@@ -910,7 +911,7 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
   int rows = 0;
   for (int t = 0; t < PACK_TOKENS; ++t) rows += place[t] >= 0;
   rows += before;
-  if (threadIdx.x == 0) *count = rows;
+  if (threadIdx.x == 0) *count = rows, *done = 0;
   const long long end = min(tokens, static_cast<long long>((rows + BK - 1) / BK) * BK);
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (long long c = rows * static_cast<long long>(hidden) + threadIdx.x * 8; c < end * hidden; c += PACK_THREADS * 8)
@@ -921,19 +922,21 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
 constexpr int JOIN_SLICES = 32;
 
 // Maximum and sum of a packed row from its parts, 32 rows per block: every slice its share of the parts in their order,
-// then the slices in theirs.
+// then the slices in theirs. The block that finishes last adds up the losses, in an order of its own and in FP64, since a
+// thread's share may be long; `done`, which the packing pass has cleared, tells it.
 __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __restrict__ partial, long long pitch, int parts,
                                                                 const int* __restrict__ count,
                                                                 const int* __restrict__ labels,
                                                                 const int* __restrict__ row_of,
                                                                 const float* __restrict__ target_logit,
-                                                                float* __restrict__ lse, float* __restrict__ losses,
-                                                                float* __restrict__ token_loss) {
+                                                                float* __restrict__ lse, float* losses, int reduction,
+                                                                int* __restrict__ done, float* __restrict__ loss_out) {
   __shared__ float2 sums[JOIN_SLICES][33];
   chain_wait();
   chain_next();
   const int row = blockIdx.x * 32 + threadIdx.x;
-  const bool ok = row < *count;
+  const int rows = *count;
+  const bool ok = row < rows;
   float top = -INFINITY, sum = 0.0f;
   if (ok) {
     constexpr int AHEAD = 4;  // parts loaded together
@@ -954,39 +957,42 @@ __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __
   }
   sums[threadIdx.y][threadIdx.x] = make_float2(top, sum);
   __syncthreads();
-  if (threadIdx.y != 0 || !ok) return;
-  for (int s = 1; s < JOIN_SLICES; ++s) top = fmaxf(top, sums[s][threadIdx.x].x);
-  // the target's logit joins the others here: loss = log(1 + sum over the others exp(l_j - l_target))
-  const float own = target_logit[row], shift = fmaxf(top, own);
-  sum = 0.0f;
-  for (int s = 0; s < JOIN_SLICES; ++s) sum += sums[s][threadIdx.x].y * shifted_exp(sums[s][threadIdx.x].x, shift);
-  const float log_sum = own >= top ? log1pf(sum) : logf(sum + shifted_exp(own, shift));
-  float loss = log_sum + (shift - own);
-  // a target outside the vocabulary has no loss, and neither has a row whose largest logit is infinite: NaN, which no
-  // later sum hides
-  if (labels[row] < 0 || isinf(shift)) loss = __int_as_float(0x7fffffff);
-  lse[row] = shift + log_sum;
-  losses[row] = loss;
-  if (token_loss != nullptr) token_loss[row_of[row]] = loss;
-}
-
-// Sum (or mean) of the packed rows' losses by one block, in a fixed order; in FP64, since a thread's share may be long.
-__global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ losses, const int* __restrict__ count, int mean,
-                                                      float* __restrict__ loss) {
-  __shared__ double slots[32];
-  chain_wait();
-  const int rows = *count;
+  if (threadIdx.y == 0 && ok) {
+    for (int s = 1; s < JOIN_SLICES; ++s) top = fmaxf(top, sums[s][threadIdx.x].x);
+    // the target's logit joins the others here: loss = log(1 + sum over the others exp(l_j - l_target))
+    const float own = target_logit[row], shift = fmaxf(top, own);
+    sum = 0.0f;
+    for (int s = 0; s < JOIN_SLICES; ++s) sum += sums[s][threadIdx.x].y * shifted_exp(sums[s][threadIdx.x].x, shift);
+    const float log_sum = own >= top ? log1pf(sum) : logf(sum + shifted_exp(own, shift));
+    float loss = log_sum + (shift - own);
+    // a target outside the vocabulary has no loss, and neither has a row whose largest logit is infinite: NaN, which no
+    // later sum hides
+    if (labels[row] < 0 || isinf(shift)) loss = __int_as_float(0x7fffffff);
+    lse[row] = shift + log_sum;
+    losses[row] = loss;
+    if (reduction == HMC_REDUCE_NONE) loss_out[row_of[row]] = loss;
+  }
+  if (reduction == HMC_REDUCE_NONE) return;
+  __shared__ int last;
+  __shared__ double slots[JOIN_SLICES];
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0 && threadIdx.y == 0) last = atomicAdd(done, 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   double v = 0.0;
-  for (int i = threadIdx.x; i < rows; i += blockDim.x) v += static_cast<double>(losses[i]);
+  for (int i = threadIdx.y * 32 + threadIdx.x; i < rows; i += 32 * JOIN_SLICES) v += static_cast<double>(__ldcg(losses + i));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  if (threadIdx.x == 0) slots[threadIdx.y] = v;
   __syncthreads();
-  if (threadIdx.x >= 32) return;
+  if (threadIdx.y != 0) return;
   v = slots[threadIdx.x];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (threadIdx.x == 0) *loss = static_cast<float>(mean ? v / rows : v);  // no row: the mean is NaN
+  // no row: the mean is NaN
+  if (threadIdx.x == 0) *loss_out = static_cast<float>(reduction == HMC_REDUCE_MEAN ? v / rows : v);
 }
 
 // ------------------------------------------------------------------------------------------- gradient
@@ -1214,7 +1220,7 @@ long long up256(long long bytes) { return (bytes + 255) / 256 * 256; }
 
 // What a forward leaves for its gradient, in one buffer of the caller.
 struct State {
-  int *count, *position, *row_of, *labels;
+  int *count, *done, *position, *row_of, *labels;
   float *lse, *losses;
   __nv_bfloat16* packed;
   long long bytes;
@@ -1222,6 +1228,7 @@ struct State {
     char* p = static_cast<char*>(base);
     const long long words = up256(4 * tokens);
     count = reinterpret_cast<int*>(p);
+    done = count + 1;
     position = reinterpret_cast<int*>(p + 256);
     row_of = reinterpret_cast<int*>(p + 256 + words);
     labels = reinterpret_cast<int*>(p + 256 + 2 * words);
@@ -1342,7 +1349,8 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
   const Targets given{targets, targets_i64, ignore_index, vocab};
   const int vector = aligned16(x) && x_stride % 8 == 0;
   pack_rows_kernel<<<static_cast<unsigned>((tokens + PACK_TOKENS - 1) / PACK_TOKENS), PACK_THREADS, 0, s>>>(
-      static_cast<const __nv_bfloat16*>(x), x_stride, given, tokens, static_cast<int>(hidden), vector, st.count, st.position,
+      static_cast<const __nv_bfloat16*>(x), x_stride, given, tokens, static_cast<int>(hidden), vector, st.count, st.done,
+      st.position,
       st.row_of, st.labels, st.packed, static_cast<const __nv_bfloat16*>(weight), weight_stride, target_logit, token_loss);
   HMC_LAUNCH_OK();
 
@@ -1362,11 +1370,8 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
     if (int rc = launch_product<STATS>(a, b, a, p, tiles_of(tokens) * tiles_of(vocab), s)) return rc;
     parts = static_cast<int>(2 * tiles_of(vocab));
   }
-  if (int rc = launch_chained(join_kernel, dim3(static_cast<unsigned>((tokens + 31) / 32)), dim3(32, JOIN_SLICES), 0, s, partial, tokens,
-                              parts, st.count, st.labels, st.row_of, target_logit, st.lse, st.losses, token_loss))
-    return rc;
-  if (reduction == HMC_REDUCE_NONE) return 0;
-  return launch_chained(reduce_kernel, dim3(1), dim3(1024), 0, s, st.losses, st.count, reduction == HMC_REDUCE_MEAN, loss);
+  return launch_chained(join_kernel, dim3(static_cast<unsigned>((tokens + 31) / 32)), dim3(32, JOIN_SLICES), 0, s, partial, tokens, parts,
+                        st.count, st.labels, st.row_of, target_logit, st.lse, st.losses, reduction, st.done, loss);
 }
 
 extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_t weight_stride, int64_t tokens, int64_t hidden,
