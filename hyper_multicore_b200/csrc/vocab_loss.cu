@@ -1119,7 +1119,7 @@ __global__ void __launch_bounds__(WORD_THREADS) word_slices_kernel(int hidden, c
                                                                    const unsigned* __restrict__ slots,
                                                                    const int* __restrict__ members,
                                                                    float* __restrict__ word_sums) {
-  __shared__ int starts[WORD_THREADS];
+  __shared__ int starts[WORD_THREADS / WORD_SLICE + 1];
   chain_wait();
   chain_next();
   const int rows = *count;
@@ -1129,9 +1129,7 @@ __global__ void __launch_bounds__(WORD_THREADS) word_slices_kernel(int hidden, c
   if (label < 0 || slots[label] != static_cast<unsigned>(row)) return;
   const int all = members[label] + 1;
   if (all <= WORD_SLICE) return;
-  const int col = (blockIdx.y * WORD_THREADS + threadIdx.x) * 4;
-  float* mine = word_sums + static_cast<long long>(row) * hidden + col;
-  float4 sum = col < hidden ? *reinterpret_cast<const float4*>(mine) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float* mine = word_sums + static_cast<long long>(row) * hidden;
   int seen = 1;
   for (int base = row + 1; seen < all && base < rows; base += WORD_THREADS) {
     const int at = base + threadIdx.x;
@@ -1140,19 +1138,20 @@ __global__ void __launch_bounds__(WORD_THREADS) word_slices_kernel(int hidden, c
     const int found = matches(match, place);
     // slices start at every WORD_SLICE-th row of the word
     const int from = (seen + WORD_SLICE - 1) / WORD_SLICE, to = (seen + found + WORD_SLICE - 1) / WORD_SLICE;
-    if (match && (seen + place) % WORD_SLICE == 0) starts[(seen + place) / WORD_SLICE - from] = at;
+    seen += found;
+    if (from == to) continue;
+    if (match && (seen - found + place) % WORD_SLICE == 0) starts[(seen - found + place) / WORD_SLICE - from] = at;
     __syncthreads();
-    if (col < hidden) {
-#pragma unroll 4
+    for (int col = threadIdx.x * 4; col < hidden; col += WORD_THREADS * 4) {
+      float4 sum = *reinterpret_cast<const float4*>(mine + col);
       for (int i = 0; i < to - from; ++i) {
         const float4 q = *reinterpret_cast<const float4*>(word_sums + static_cast<long long>(starts[i]) * hidden + col);
         sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
       }
+      *reinterpret_cast<float4*>(mine + col) = sum;
     }
-    seen += found;
     __syncthreads();
   }
-  if (col < hidden) *reinterpret_cast<float4*>(mine) = sum;
 }
 
 // ------------------------------------------------------------------------------------------- host
@@ -1403,9 +1402,8 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
                               static_cast<__nv_bfloat16*>(grad_hidden)))
     return rc;
   if (grad_weight != nullptr && tokens > WORD_SLICE) {
-    const dim3 grid(static_cast<unsigned>(tokens), (width / 4 + WORD_THREADS - 1) / WORD_THREADS);
-    if (int rc = launch_chained(word_slices_kernel, grid, dim3(WORD_THREADS), 0, s, width, st.count, st.labels, w.slots, w.members,
-                                w.word_sums))
+    if (int rc = launch_chained(word_slices_kernel, dim3(static_cast<unsigned>(tokens)), dim3(WORD_THREADS), 0, s, width, st.count,
+                                st.labels, w.slots, w.members, w.word_sums))
       return rc;
   }
 
