@@ -61,77 +61,66 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* slots, int warps) 
 
 constexpr int MAX_WARPS = 32;
 
-// One row per blockDim.x threads, NV packs of VEC values per thread, the row in registers between its two passes: the
-// variance is that of the differences from the mean, so a common offset costs no digits. blockDim.y rows per block, one
-// per warp, where a row is short.
+// Short rows of any alignment, forward: a warp per row, NV packs of VEC values per lane in registers between the passes. The
+// variance is that of the differences from the mean, here as below, so that a common offset costs no digits. (16384 rows of
+// 300 BF16: 7.9 us.)
+constexpr int SHORT_ROWS = 4;  // per block
+
 template <typename T, typename W, int VEC, int NV, bool CENTER>
-__global__ void __launch_bounds__(1024) row_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, int hidden,
-                                                        const W* __restrict__ weight, const W* __restrict__ bias, float eps,
-                                                        T* __restrict__ y, float* __restrict__ mean_out,
-                                                        float* __restrict__ rstd_out) {
-  __shared__ float slots[2][MAX_WARPS];
-  const long long row = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (row >= rows) return;  // only where a row is one warp, which meets no barrier
-  const int warps = blockDim.x >> 5;
-  const int packs = hidden / VEC;
+__global__ void __launch_bounds__(32 * SHORT_ROWS)
+short_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, int hidden, const W* __restrict__ weight,
+                  const W* __restrict__ bias, float eps, T* __restrict__ y, float* __restrict__ mean_out,
+                  float* __restrict__ rstd_out) {
+  const int lane = threadIdx.x & 31, packs = hidden / VEC;
+  const long long row = static_cast<long long>(blockIdx.x) * SHORT_ROWS + (threadIdx.x >> 5);
+  if (row >= rows) return;
   const float scale = 1.0f / static_cast<float>(hidden);
   const T* src = x + row * x_stride;
-  Pack<T, VEC> in[NV];
-  float sum[1] = {0.0f};
+  float v[NV][VEC];
+  float mean = 0.0f, square = 0.0f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int at = j * blockDim.x + threadIdx.x;
-    if (at < packs) in[j] = load_pack<T, VEC>(src + static_cast<long long>(at) * VEC);
-  }
-  float mean = 0.0f;
-  if (CENTER) {
+    const int at = j * 32 + lane;
+    Pack<T, VEC> in;
+    if (at < packs) in = load_pack<T, VEC>(src + at * VEC);
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (j * blockDim.x + threadIdx.x < packs) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum[0] += widen(in[j].v[e]);
-      }
-    row_sum(sum, slots[0], warps);
-    mean = sum[0] * scale;
+    for (int e = 0; e < VEC; ++e) {
+      v[j][e] = at < packs ? widen(in.v[e]) : 0.0f;
+      mean += v[j][e];
+    }
   }
-  float square[1] = {0.0f};
+  mean = CENTER ? warp_sum(mean) * scale : 0.0f;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if (j * blockDim.x + threadIdx.x < packs) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d = widen(in[j].v[e]) - mean;
-        square[0] += d * d;
-      }
+    for (int e = 0; e < VEC; ++e) {
+      if (CENTER) v[j][e] = j * 32 + lane < packs ? v[j][e] - mean : 0.0f;
+      square += v[j][e] * v[j][e];
     }
-  row_sum(square, slots[1], warps);
-  const float rstd = rsqrtf(square[0] * scale + eps);
+  const float rstd = rsqrtf(warp_sum(square) * scale + eps);
   T* dst = y + row * hidden;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int at = j * blockDim.x + threadIdx.x;
-    if (at < packs) {
-      Pack<T, VEC> out;
-      Pack<W, VEC> w, b;
-      if (weight != nullptr) w = load_pack<W, VEC>(weight + static_cast<long long>(at) * VEC);
-      if (CENTER && bias != nullptr) b = load_pack<W, VEC>(bias + static_cast<long long>(at) * VEC);
+    const int at = j * 32 + lane;
+    if (at >= packs) continue;
+    Pack<T, VEC> out;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float v = (widen(in[j].v[e]) - mean) * rstd;
-        if (weight != nullptr) v *= widen(w.v[e]);
-        if (CENTER && bias != nullptr) v += widen(b.v[e]);
-        out.v[e] = narrow<T>(v);
-      }
-      store_pack<T, VEC>(dst + static_cast<long long>(at) * VEC, out);
+    for (int e = 0; e < VEC; ++e) {
+      float u = v[j][e] * rstd;
+      if (weight != nullptr) u *= widen(weight[at * VEC + e]);
+      if (CENTER && bias != nullptr) u += widen(bias[at * VEC + e]);
+      out.v[e] = narrow<T>(u);
     }
+    store_pack<T, VEC>(dst + at * VEC, out);
   }
-  if (threadIdx.x == 0 && rstd_out != nullptr) {
+  if (lane == 0 && rstd_out != nullptr) {
     if (CENTER) mean_out[row] = mean;
     rstd_out[row] = rstd;
   }
 }
 
-// Rows too long for the registers of a block: the same three passes, each reading the row again (from L2).
+// Rows too long for the registers of a block, or longer than SHORT rows in a tensor that starts on no 16-byte boundary: the same
+// three passes, each reading the row again (from L2).
 template <typename T, typename W, bool CENTER>
 __global__ void __launch_bounds__(1024) long_row_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows,
                                                              int hidden, const W* __restrict__ weight,
@@ -170,8 +159,8 @@ __global__ void __launch_bounds__(1024) long_row_norm_kernel(const T* __restrict
 
 // ------------------------------------------------------------------------------------------- many rows
 // 16 bytes of T as FP32 pairs: the arithmetic of the kernels below takes two values per instruction, because counted in
-// single ones it is longer than the memory's time (34 instructions per value in a first version, 123 us for 16384 rows of
-// 7168 against 72 us of traffic).
+// single ones it is longer than the memory's time (16384 rows of 7168 BF16, 72 us of traffic: 34 instructions per value and
+// 123 us in single values, 10 and 76 us now).
 template <typename T>
 struct Quad;
 template <>
@@ -275,7 +264,9 @@ __device__ __forceinline__ float2 block_sum(float2 v, float* slots) {
 
 // A block walks the rows blockIdx.x, + gridDim.x, ... and copies the next ones asynchronously while it works on one: a ring
 // of rows in shared memory in which a thread writes and reads its own packs only, so that the copies need no barrier.
-// What is left per row is the reduction's, at which the blocks of an SM take turns.
+// What is left per row is the reduction's, at which the blocks of an SM take turns: as many as their registers allow, with four
+// rows in each ring. Bound by memory: RMSNorm of 8192 x 4096 BF16 20.4 us (134 MB, the copy rate), layer norm of 16384 x 7168
+// 76 us (6.2 TB/s). One row alone takes 2.3 to 2.9 us; a block per row without a ring took 2.5 to 4.3.
 constexpr int FORWARD_STAGES = 4;
 constexpr int GRAD_STAGES = 3;
 
@@ -383,7 +374,8 @@ stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
 // The gradient over the same ring, x and dy per stage. Threads own columns: the parameters' gradients stay in registers over
 // all rows of a block, so that x and dy are read once. Behind the reduction a row is widened again from the ring: kept in
 // registers its g and u would leave room for 14 warps per SM instead of 28 (16384 rows, layer norm, BF16: 2048 wide 67 against
-// 45 us, 4096 100 against 83, 7168 203 against 144).
+// 46 us, 4096 100 against 87, 7168 203 against 140). Bound by instructions where the values are 16 bits (22 per value, issue
+// slots 54 % busy; 16384 x 7168 140 us for 108 us of traffic), by memory in FP32 (8192 x 7168 106 us, the copy rate).
 constexpr int WIDE_THREADS = 448;  // a row of 7168
 template <typename T, typename W, int NV, int PITCH, bool CENTER>
 __global__ void __launch_bounds__(PITCH, 2 * WIDE_THREADS / PITCH > 0 ? 2 * WIDE_THREADS / PITCH : 1)
@@ -526,8 +518,8 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
     }
 }
 
-// The gradient of the longest rows that stream, 32 values per thread and one block per SM: g and u stay in registers between the
-// reduction and dx.
+// The gradient of the longest rows that stream (above 8192), 32 values per thread and one block per SM, whose ring fills shared
+// memory: g and u stay in registers between the reduction and dx.
 template <typename T, typename W, int NV, int PITCH, bool CENTER>
 __global__ void __launch_bounds__(PITCH)
 stream_longest_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
@@ -649,8 +641,9 @@ stream_longest_grad_kernel(const T* __restrict__ x, long long x_stride, const T*
 // Rows that start on no 16-byte boundary, or are no multiple of 16 bytes, of a tensor that starts on one. A ring again, but of
 // windows: the 16-byte pieces that hold a row, copied by whichever thread, so that a barrier stands before their use. The
 // first piece may begin with the end of the row before (the first row of all begins on its boundary), the last one ends
-// with the row. VEC = 1 or 2 values per access behind that. (Straight from memory, two bytes at a time, too little was under
-// way: 237 us for 16384 rows of 5003 BF16 against 50 us of traffic.)
+// with the row. VEC = 1 or 2 values per access behind that, which bounds these kernels: 16384 rows of 5003 BF16 take 183 us
+// forward and 271 for the gradient (50 and 75 us of traffic), 4096 rows of 7161 FP32 55 and 90 us (36 and 54). Straight from
+// memory, with too little under way, the BF16 rows took 237 and 497 us.
 constexpr int WINDOW_WARPS = 16;
 constexpr int WINDOW_MOST = 8192;  // values of a row
 constexpr int WINDOW_STAGES = 6;
@@ -860,8 +853,9 @@ window_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
     }
 }
 
-// Short rows: a warp per row, no barrier per row, the next row's loads under way. The warps of a block join their sums over
-// rows one after the other in shared memory.
+// Short rows, gradient: a warp per row, no barrier per row, the next row's loads under way. The warps of a block join their sums
+// over rows one after the other in shared memory. Latency and the 32 accumulators per lane bound it: 16384 rows of 512 BF16
+// 19.5 us (7.7 us of traffic); at 1024 the block kernel above is faster (70 against 25 us).
 constexpr int SHORT_WARPS = 8;
 
 template <typename T, typename W, int VEC, int NV, bool CENTER>
@@ -955,7 +949,8 @@ short_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __r
   }
 }
 
-// Rows too long for a block's registers: dx by one block per row, the parameters' partial sums by columns.
+// Rows too long for a block's registers, or of a tensor that starts on no 16-byte boundary: dx by one block per row, the
+// parameters' partial sums by columns, everything read twice or three times (mostly from L2).
 template <typename T, typename W, bool CENTER>
 __global__ void __launch_bounds__(1024) long_row_norm_grad_kernel(const T* __restrict__ x, long long x_stride,
                                                                   const T* __restrict__ grad, long long grad_stride,
@@ -1002,7 +997,8 @@ __global__ void __launch_bounds__(256) column_grad_kernel(const T* __restrict__ 
   if (CENTER) partial_bias[static_cast<long long>(blockIdx.y) * hidden + c] = b;
 }
 
-// Parameters' gradients: the partial sums of a column in the order of the blocks that made them.
+// Parameters' gradients: the partial sums of a column in the order of the blocks that made them, 32 slices of them in
+// parallel (8 slices took 12 us for 296 sums of 7168 columns, 32 take 5 to 6).
 constexpr int FINISH_SLICES = 32;
 template <typename W>
 __global__ void __launch_bounds__(32 * FINISH_SLICES) param_grad_kernel(const float* __restrict__ partial_weight,
@@ -1057,12 +1053,9 @@ long long grad_parts(long long rows, long long hidden) {
 }
 
 template <typename T, typename W, int VEC, int NV, bool CENTER>
-int launch_forward(const NormCall& c) {
-  const int need = (c.hidden / VEC + NV - 1) / NV;
-  const int threads = round_up(need, 32);
-  const int rows_per_block = threads == 32 ? 4 : 1;
-  const long long blocks = (c.rows + rows_per_block - 1) / rows_per_block;
-  row_norm_kernel<T, W, VEC, NV, CENTER><<<static_cast<unsigned>(blocks), dim3(threads, rows_per_block), 0, c.stream>>>(
+int launch_short(const NormCall& c) {
+  const long long blocks = (c.rows + SHORT_ROWS - 1) / SHORT_ROWS;
+  short_norm_kernel<T, W, VEC, NV, CENTER><<<static_cast<unsigned>(blocks), 32 * SHORT_ROWS, 0, c.stream>>>(
       static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
       c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
   HMC_LAUNCH_OK();
@@ -1209,13 +1202,11 @@ int forward(const NormCall& c) {
   constexpr int VEC = 16 / sizeof(T);
   const bool wide = c.hidden % VEC == 0 && c.x_stride % VEC == 0 && aligned_to(c.x, 16) && aligned_to(c.y, 16) &&
                     aligned_to(c.weight, 16) && aligned_to(c.bias, 16);
-  if (wide && c.rows > 2ll * sm_count() && c.hidden > 32 * VEC * FORWARD_PACKS && c.hidden <= STREAM_THREADS * VEC * FORWARD_PACKS)
-    return stream<T, W, CENTER>(c);
-  if (wide && c.hidden <= 1024 * VEC * FORWARD_PACKS) return launch_forward<T, W, VEC, FORWARD_PACKS, CENTER>(c);
+  if (wide && c.hidden <= STREAM_THREADS * VEC * FORWARD_PACKS) return stream<T, W, CENTER>(c);
   const bool pairs = c.hidden % 2 == 0 && c.x_stride % 2 == 0 && aligned_to(c.x, 2 * sizeof(T)) && aligned_to(c.y, 2 * sizeof(T)) &&
                      aligned_to(c.weight, 2 * sizeof(W)) && aligned_to(c.bias, 2 * sizeof(W));
   if (c.hidden <= 32 * 16)
-    return pairs ? launch_forward<T, W, 2, 8, CENTER>(c) : launch_forward<T, W, 1, 16, CENTER>(c);
+    return pairs ? launch_short<T, W, 2, 8, CENTER>(c) : launch_short<T, W, 1, 16, CENTER>(c);
   if (aligned_to(c.x, 16) && c.hidden <= WINDOW_MOST) return pairs ? window<T, W, 2, CENTER>(c) : window<T, W, 1, CENTER>(c);
   long_row_norm_kernel<T, W, CENTER><<<static_cast<unsigned>(c.rows), 1024, 0, c.stream>>>(
       static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),

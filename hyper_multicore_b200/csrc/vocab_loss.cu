@@ -11,10 +11,14 @@
 // and two GEMMs take the piece to the two gradients. p without the target's entry only: that one is p - 1, which cancels for
 // a token the model is sure of and carries the largest weight for one it is not, so it stays in FP32 (expm1 of -loss) and
 // meets the products in FP32: for dx as the row w_t(i) in the epilogue, for dw as a sum over the tokens of a word made
-// beforehand. The rounding of the other entries to BF16 (2^-9 relative) averages over a sum of many.
+// beforehand. The rounding of the other entries to BF16 (2^-8 of the value at most) averages over a sum of many.
+// The logits are computed twice on purpose: kept as BF16 they would be the tensor of tokens x vocabulary that this operator
+// is there to avoid, and gradients taken in the forward pass would hold the weight's gradient in FP32 until the backward one.
 //
 // The GEMM: CTA pairs (tcgen05.mma.cta_group::2, M = N = 256), one TMA producer, one issuer, eight epilogue warps, two
-// accumulators; the layouts of the operands are those of the grouped GEMMs.
+// accumulators; the layouts of the operands are those of the grouped GEMMs. Bound by the tensor cores: 4096 x 32768 x 4096 takes
+// 750 us in each of the four forms (1466 TFLOP/s, 0.90 of cuBLAS in a burst, tensor pipe 80 to 88 % busy); over seconds the
+// power limit leaves 1250 to 1330 (cuBLAS: 1380). Short k (1024 and below) is bound by L2: 1 MB per 256 x 256 tile.
 #include <cuda.h>
 
 #include "common.cuh"
@@ -44,9 +48,12 @@ constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * STORE_STAGE_BYTES 
 constexpr int MAX_PARTS = 16;  // of a tile that is cut along k
 constexpr int MIN_PART = 8;    // k-blocks of a part, at the least
 // k-blocks that add up inside the tensor core before the sum goes to FP32 registers (STATS, few tokens). The loss of 8192 tokens
-// of 4096 over 131072 words: 8 7.63 ms, 16 7.30, 32 7.22, 64 (all of it) 6.85.
+// of 4096 over 131072 words: 8 7.63 ms, 16 7.30, 32 7.22, 64 (all of it) 6.85. With 32 the loss is off by 1.5e-7 to 3e-7
+// (FP32 throughout: 2.8e-7 to 9e-7).
 constexpr int PROMOTE = 32;
-constexpr int BAND = 16; // tile rows that are walked together, so that a band's rows stay in L2 while the weight passes by (8, 16, 32: 29987, 29527, 31442 us for a training step of 8192 x 4096 x 131072)
+// Tile rows that are walked together, so that a band's rows stay in L2 while the weight passes by once per band (8, 16, 32:
+// 29987, 29527, 31442 us for a training step of 8192 x 4096 x 131072).
+constexpr int BAND = 16;
 
 enum Product { STATS, PROBS, GRAD_HIDDEN, GRAD_WEIGHT };
 
@@ -81,8 +88,8 @@ struct Unit {
 
 // Tiles in bands of BAND tile rows, a band's columns one after the other. With `split`, the tiles that would leave pairs
 // idle in the last wave are cut along k: into as many parts as shorten that wave most, counted with a hundredth of a tile's
-// time per part for what they write, at most two parts per pair (4 tiles of 32 wide and k 32000 on 74 pairs: one part each in
-// 166 us, 9 in 29 us).
+// time per part for what they write, at most two parts per pair (512 x 1024 with k = 32000, 8 tiles for 74 pairs: 167 us whole, 35 +
+// 8 us for joining them in 9 parts; 3687 x 4096 with k = 65536, 240 tiles: 1621 us whole, 1395 + 13).
 struct Walker {
   int mt, nt, kiters, parts;
   long long whole, units;
@@ -566,8 +573,9 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
 
 // ------------------------------------------------------------------------------------------- few tokens
 // Up to 128 tokens: the weight's rows take the M side of the tile and the tokens N = 32, 64 or 128 columns, so that the tensor
-// cores do a fraction of a 256 x 256 tile's work beside the one pass over the weight, which is the bound (scoring of 16
-// tokens of 4096 over 131072 words: 1.07 GB). An accumulator row is a word: the sums over words run across the lanes of a warp.
+// cores do a fraction of a 256 x 256 tile's work beside the one pass over the weight, which is the bound: 16 tokens of 4096 over
+// 131072 words 171 us (1.07 GB, 6.3 TB/s; on 256 x 256 tiles 182 to 198). Whole calls of 128 tokens take 206 us this way, of 129 the
+// other way 236. An accumulator row is a word: the sums over words run across the lanes of a warp.
 template <int N>
 struct Few {
   static constexpr int B_BYTES = N / 2 * 128;                  // tokens' k-block that a CTA loads
@@ -845,8 +853,9 @@ __device__ __forceinline__ int block_count(int v) {  // sum over the block, in e
 }
 
 // The tokens that count, in their order, as rows without gaps, and the logit of each one's target by FP32 multiply-adds: it
-// enters the loss with its whole weight, where an error of the tensor core's sums would show. A block finds its place by counting the targets before
-// its own; the last one writes the number of rows and clears the rows up to the next k-block of a contraction over them.
+// enters the loss with its whole weight, where an error of the tensor core's sums would show. A block finds its place by
+// counting the targets before its own; the last one writes the number of rows and clears the rows up to the next k-block of
+// a contraction over them. Bound by latency (8192 x 4096: 50 us for 200 MB with the targets' rows; 5 us for 16 tokens).
 __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bfloat16* __restrict__ x, long long x_stride,
                                                                  Targets targets, long long tokens, int hidden, int vector,
                                                                  int* __restrict__ count, int* __restrict__ done,
@@ -1026,8 +1035,8 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
 }
 
 // The sum of coef_i x_i over the rows that have a word as target, in their order, in slices of WORD_SLICE rows of a word:
-// every row that is the first of a slice adds up its slice, into word_sums at its own row. (One block for all rows of a word
-// took 390 us for 8192 tokens drawn by a power law: the commonest word had 480 of them.)
+// every row that is the first of a slice adds up its slice, into word_sums at its own row. (8192 tokens of 4096 by a power law, the
+// commonest word with 480 of them: one block for all rows of a word 391 us, slices 74 us and their joining about 10.)
 constexpr int WORD_THREADS = 256;
 constexpr int WORD_SLICE = 32;
 
@@ -1258,7 +1267,8 @@ int launch_few(const CUtensorMap& words, const State& st, long long hidden, long
                         (p.k + BK - 1) / BK, p.count, p.labels, p.partial, p.pitch, p.status);
 }
 
-// A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size.
+// A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size. A training step of
+// 8192 x 4096 x 131072 with pieces of 256 MiB 29.0 ms, 512 28.6, 1 GiB 28.8, 2 GiB (one piece) 30.1.
 constexpr long long PIECE_BYTES = 512ll << 20;
 long long piece_words(long long tokens, long long vocab) {
   long long most = PIECE_BYTES / (2 * tokens) / TILE * TILE;

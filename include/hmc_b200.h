@@ -987,7 +987,7 @@ int hmc_row_norm(const void* x, int64_t x_stride, int64_t rows, int64_t hidden, 
                  const void* bias, int affine_dtype, int center, float eps, void* y, float* mean, float* rstd, void* stream);
 /* Gradients from grad = dy [rows, hidden] (rows grad_stride elements apart): grad_x [rows, hidden] of `dtype` without
  * gaps, grad_weight and grad_bias [hidden] of affine_dtype, summed over the rows in FP32 in an order that follows from
- * rows and hidden alone. Each of the three may be NULL. `workspace` (16-byte aligned, of ..._workspace_bytes, which do
+ * extents, types, strides and alignment alone. Each of the three may be NULL. `workspace` (16-byte aligned, of ..._workspace_bytes, which do
  * not fall as rows grow) is read for grad_weight and grad_bias only. */
 int64_t hmc_row_norm_grad_workspace_bytes(int64_t rows, int64_t hidden);
 int hmc_row_norm_grad(const void* x, int64_t x_stride, const void* grad, int64_t grad_stride, int64_t rows, int64_t hidden,
@@ -997,7 +997,8 @@ int hmc_row_norm_grad(const void* x, int64_t x_stride, const void* grad, int64_t
 /* Cross entropy of hidden states over a vocabulary: loss_i = log sum_j exp(x_i . w_j) - x_i . w_target(i), without ever
  * holding the logits. x [tokens, hidden] and weight [vocab, hidden] BF16 with rows x_stride and weight_stride elements
  * apart (weight rows on 16-byte boundaries, hidden a multiple of 8), targets INT32 or INT64. Tokens whose target is
- * ignore_index have no loss and are not read; a target outside [0, vocab) gives a loss of NaN. reduction: loss [tokens] (0 for
+ * ignore_index have no loss and are not read; a target outside [0, vocab), or a largest logit that is infinite, gives a
+ * loss of NaN. reduction: loss [tokens] (0 for
  * ignored tokens), or loss [1], the sum or the mean over the tokens that count (NaN where none does). `state` (16-byte
  * aligned, of ..._state_bytes) keeps what the gradient needs, the counted rows of x among it. Logits and sums in FP32. */
 #define HMC_REDUCE_NONE 0
