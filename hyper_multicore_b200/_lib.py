@@ -33,6 +33,7 @@ HMC_PROFILE_KINDS = ("grouped_gemm", "mx_gemm", "mx_quant", "ep", "route")
 HMC_DTYPE_BF16, HMC_DTYPE_F16, HMC_DTYPE_F32 = 0, 1, 2
 HMC_DTYPE = {torch.bfloat16: HMC_DTYPE_BF16, torch.float16: HMC_DTYPE_F16, torch.float32: HMC_DTYPE_F32}
 HMC_NORM_MAX_HIDDEN = 1048576
+HMC_NORM_MAX_ROWS = 2147418112
 HMC_REDUCE = {"none": 0, "mean": 1, "sum": 2}
 HMC_MOE_LAYOUT = {"EIO": 0, "EOI": 1}
 HMC_MOE_DISPATCH = {"push": 0, "pull": 1}

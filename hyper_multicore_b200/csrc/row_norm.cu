@@ -1312,9 +1312,10 @@ int run(NormCall& c, int dtype, int affine_dtype, bool center, bool backward) {
 }
 
 int check(const char* name, int64_t rows, int64_t hidden, int64_t stride, int dtype, int affine_dtype) {
-  HMC_REQUIRE(rows >= 0 && rows < (1ll << 31) && hidden > 0 && hidden <= HMC_NORM_MAX_HIDDEN, HMC_ERR_INVALID,
-              "%s: rows (%lld) must be in [0, 2^31) and hidden (%lld) in [1, %d]", name, (long long)rows, (long long)hidden,
-              HMC_NORM_MAX_HIDDEN);
+  // blocks step through the rows in 32 bits, by less than 2^16
+  HMC_REQUIRE(rows >= 0 && rows <= HMC_NORM_MAX_ROWS && hidden > 0 && hidden <= HMC_NORM_MAX_HIDDEN, HMC_ERR_INVALID,
+              "%s: rows (%lld) must be in [0, %d] and hidden (%lld) in [1, %d]", name, (long long)rows, HMC_NORM_MAX_ROWS,
+              (long long)hidden, HMC_NORM_MAX_HIDDEN);
   HMC_REQUIRE(stride >= 0, HMC_ERR_INVALID, "%s: row strides must not be negative", name);
   HMC_REQUIRE(dtype >= HMC_DTYPE_BF16 && dtype <= HMC_DTYPE_F32, HMC_ERR_INVALID, "%s: unknown dtype %d", name, dtype);
   HMC_REQUIRE(affine_dtype == dtype || affine_dtype == HMC_DTYPE_F32, HMC_ERR_INVALID,

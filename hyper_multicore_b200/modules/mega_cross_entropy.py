@@ -107,7 +107,8 @@ def mega_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torc
     tokens; the mean over none of them is NaN, as in torch. Ignored tokens are not read: whatever their hidden states hold,
     their gradient is zero and they add nothing to the weight's. A target outside [0, V) that is not ``ignore_index`` is not
     noticed on the host: its loss is NaN, and so are the gradients it enters. Differentiable once in ``hidden`` and ``weight``;
-    the gradients are BF16. The backward pass takes scratch of up to 512 MiB for probabilities and of up to 8 bytes per element of ``hidden``.
+    the gradients are BF16. The backward pass takes scratch of up to 512 MiB for probabilities (4096 words of them where that is
+    more), 8 bytes per element of ``hidden`` and 8 bytes per word.
     """
     _validate(hidden, weight, targets, ignore_index, reduction)
     rows = as_rows(hidden, weight.shape[1])

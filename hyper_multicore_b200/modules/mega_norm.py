@@ -20,7 +20,7 @@ def _fits(x, weight, bias, eps) -> bool:
     if type(x) is not torch.Tensor or not x.is_cuda or x.ndim == 0 or type(eps) is not float or not 0.0 <= eps < math.inf:
         return False
     dtype, hidden = x.dtype, x.shape[-1]
-    if not (1 <= hidden <= _lib.HMC_NORM_MAX_HIDDEN and x.numel() < hidden << 31 and dtype in _lib.HMC_DTYPE):
+    if not (1 <= hidden <= _lib.HMC_NORM_MAX_HIDDEN and x.numel() <= hidden * _lib.HMC_NORM_MAX_ROWS and dtype in _lib.HMC_DTYPE):
         return False
     if weight is not None and not (isinstance(weight, torch.Tensor) and weight.ndim == 1 and weight.shape[0] == hidden
                                    and weight.dtype in (dtype, torch.float32) and weight.device == x.device):
@@ -38,8 +38,8 @@ def _validate(x, weight, bias, eps) -> None:
         raise TypeError(f"x must be BF16, FP16 or FP32, got {x.dtype}.")
     if x.ndim < 1 or not 1 <= x.shape[-1] <= _lib.HMC_NORM_MAX_HIDDEN:
         raise ValueError(f"x must end in [hidden] with 1 <= hidden <= {_lib.HMC_NORM_MAX_HIDDEN}, got {tuple(x.shape)}.")
-    if x.numel() // x.shape[-1] >= 1 << 31:
-        raise ValueError("x must have fewer than 2^31 rows.")
+    if x.numel() // x.shape[-1] > _lib.HMC_NORM_MAX_ROWS:
+        raise ValueError(f"x must have at most {_lib.HMC_NORM_MAX_ROWS} rows.")
     first = None
     for name, parameter in (("weight", weight), ("bias", bias)):
         if parameter is None:

@@ -977,12 +977,14 @@ int hmc_mega_moe_mxfp8_abi_version(void);
 #define HMC_DTYPE_F16 1
 #define HMC_DTYPE_F32 2
 #define HMC_NORM_MAX_HIDDEN 1048576
+#define HMC_NORM_MAX_ROWS 2147418112 /* 2^31 - 2^16 */
 
 /* y[r] = (x[r] - mean) * rstd * weight + bias with mean and rstd = 1 / sqrt(mean((x - mean)^2) + eps) of the row's
  * `hidden` values; center == 0: mean = 0 and no bias (RMSNorm). x rows start x_stride elements apart (0: the same row
  * again), y is [rows, hidden] without gaps, both of `dtype`; weight and bias [hidden] of affine_dtype (dtype or FP32),
  * either may be NULL (1 and 0). mean and rstd, FP32 [rows], are what hmc_row_norm_grad reads: both or neither; without
- * centring there is no mean. Statistics in FP32, y rounded once. rows < 2^31, hidden <= HMC_NORM_MAX_HIDDEN. */
+ * centring there is no mean. Statistics in FP32, y rounded once. rows <= HMC_NORM_MAX_ROWS, hidden <=
+ * HMC_NORM_MAX_HIDDEN. */
 int hmc_row_norm(const void* x, int64_t x_stride, int64_t rows, int64_t hidden, int dtype, const void* weight,
                  const void* bias, int affine_dtype, int center, float eps, void* y, float* mean, float* rstd, void* stream);
 /* Gradients from grad = dy [rows, hidden] (rows grad_stride elements apart): grad_x [rows, hidden] of `dtype` without
@@ -1011,7 +1013,8 @@ int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weight, int64_t 
                    void* state, float* loss, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 /* Gradients from the state of a forward with the same sizes, weight and reduction, and grad_loss (FP32 [tokens] or [1]):
  * grad_hidden [tokens, hidden] (zeros for ignored tokens) and grad_weight [vocab, hidden], BF16 without gaps; either may be
- * NULL. The vocabulary is walked in pieces whose BF16 probabilities fit the workspace, the logits are computed again. Results do
+ * NULL. The vocabulary is walked in pieces whose BF16 probabilities take at most 512 MiB (or 4096 words, where those
+ * take more); the logits are computed again. Results do
  * not depend on timing. */
 int64_t hmc_vocab_loss_grad_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab);
 int hmc_vocab_loss_grad(const void* state, const void* weight, int64_t weight_stride, int64_t tokens, int64_t hidden,

@@ -17,6 +17,7 @@ BF16 = torch.bfloat16
     (TypeError, "BF16, FP16 or FP32", lambda: mega_rms_norm(torch.zeros(2, 8, dtype=torch.float64))),
     (ValueError, "must end in", lambda: mega_rms_norm(torch.zeros((), dtype=BF16))),
     (ValueError, "must end in", lambda: mega_rms_norm(torch.zeros(4, 0, dtype=BF16))),
+    (ValueError, "rows", lambda: mega_rms_norm(torch.zeros(1, 1).expand((1 << 31) - 1, 1))),
     (ValueError, "weight must have shape", lambda: mega_rms_norm(torch.zeros(2, 8), torch.ones(7))),
     (TypeError, "weight must have dtype", lambda: mega_rms_norm(torch.zeros(2, 8), torch.ones(8, dtype=BF16))),
     (TypeError, "one dtype", lambda: mega_layer_norm(torch.zeros(2, 8, dtype=BF16), torch.ones(8), torch.ones(8, dtype=BF16))),
@@ -73,6 +74,7 @@ def test_c_entries_refuse_without_touching_a_device():
         x=at, xs=8, rows=2, hidden=8, dtype=0, w=None, b=None, adt=0, center=1, eps=1e-6, y=at, mean=None, rstd=None,
         stream=None), **c}.values())
     refused(norm(rows=-1), b"rows")
+    refused(norm(rows=(1 << 31) - 1), b"rows")
     refused(norm(hidden=0), b"hidden")
     refused(norm(hidden=(1 << 20) + 1), b"hidden")
     refused(norm(dtype=3), b"dtype")

@@ -195,6 +195,9 @@ def test_strides_alignment_and_batches():
     loss, grad_x, grad_w = run(rows, weight, targets.view(3, 20), "none")
     assert loss.shape == (3, 20) and grad_x.shape == (3, 20, 128)
     check((loss.view(60), grad_x.view(60, 128), grad_w), rows.reshape(60, 128), weight, targets, "none")
+    one = run(x[7], weight, targets[7], "none")  # a token without a batch
+    assert one[0].shape == () and one[1].shape == (128,)
+    check((one[0].view(1), one[1].view(1, 128), one[2]), x[7:8], weight, targets[7:8], "none")
     strided = torch.full((60, 2), IGNORED, device="cuda")
     strided[:, 0] = targets
     check(run(x, weight, strided[:, 0]), x, weight, targets)

@@ -259,6 +259,16 @@ assert all(torch.equal(a, b) for a, b in zip(got, step()))
     subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
 
 
+def test_the_most_rows_there_may_be():
+    """Blocks step through rows in 32 bits: the last step must not run over."""
+    from hyper_multicore_b200 import _lib, mega_rms_norm
+
+    rows = _lib.HMC_NORM_MAX_ROWS
+    x = torch.ones(1, 8, device="cuda", dtype=torch.bfloat16).expand(rows, 8)
+    y = mega_rms_norm(x)
+    assert torch.equal(y[-5:], torch.ones(5, 8, device="cuda", dtype=torch.bfloat16)) and y.shape[0] == rows
+
+
 def test_other_streams_and_captured_graphs():
     x, weight, bias, grad = make(130, 1024, torch.bfloat16, torch.bfloat16, True, seed=17)
     want = run(x, weight, bias, grad, True)
