@@ -71,6 +71,8 @@ __global__ void __launch_bounds__(32 * SHORT_ROWS)
 short_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, int hidden, const W* __restrict__ weight,
                   const W* __restrict__ bias, float eps, T* __restrict__ y, float* __restrict__ mean_out,
                   float* __restrict__ rstd_out) {
+  chain_wait();
+  chain_next();
   const int lane = threadIdx.x & 31, packs = hidden / VEC;
   const long long row = static_cast<long long>(blockIdx.x) * SHORT_ROWS + (threadIdx.x >> 5);
   if (row >= rows) return;
@@ -126,6 +128,8 @@ __global__ void __launch_bounds__(1024) long_row_norm_kernel(const T* __restrict
                                                              int hidden, const W* __restrict__ weight,
                                                              const W* __restrict__ bias, float eps, T* __restrict__ y,
                                                              float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  chain_wait();
+  chain_next();
   __shared__ float slots[2][MAX_WARPS];
   const long long row = blockIdx.x;
   const int warps = blockDim.x >> 5;
@@ -275,6 +279,8 @@ __global__ void __launch_bounds__(STREAM_THREADS)
 stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, int hidden, const W* __restrict__ weight,
                    const W* __restrict__ bias, float eps, T* __restrict__ y, float* __restrict__ mean_out,
                    float* __restrict__ rstd_out) {
+  chain_wait();
+  chain_next();
   extern __shared__ uint4 ring_raw[];
   constexpr int stages = FORWARD_STAGES;
   __shared__ __align__(16) float slots[2][STREAM_WARPS];
@@ -383,6 +389,7 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
                         long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
                         const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
                         float* __restrict__ partial_bias) {
+  chain_wait();
   extern __shared__ uint4 ring_raw[];
   constexpr int stages = GRAD_STAGES, SUMS = CENTER ? 2 : 1;
   __shared__ __align__(16) float slots[2][SUMS * STREAM_WARPS];
@@ -526,6 +533,7 @@ stream_longest_grad_kernel(const T* __restrict__ x, long long x_stride, const T*
                         long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
                         const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
                         float* __restrict__ partial_bias) {
+  chain_wait();
   extern __shared__ uint4 ring_raw[];
   constexpr int stages = GRAD_STAGES, SUMS = CENTER ? 2 : 1;
   __shared__ __align__(16) float slots[2][SUMS * STREAM_WARPS];
@@ -676,6 +684,8 @@ __global__ void __launch_bounds__(32 * WINDOW_WARPS)
 window_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, int hidden, const W* __restrict__ weight,
                    const W* __restrict__ bias, float eps, T* __restrict__ y, float* __restrict__ mean_out,
                    float* __restrict__ rstd_out, int stages, int window) {
+  chain_wait();
+  chain_next();
   extern __shared__ uint4 ring_raw[];
   __shared__ float slots[2][WINDOW_WARPS];
   uint8_t* ring = reinterpret_cast<uint8_t*>(ring_raw);
@@ -763,6 +773,7 @@ window_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
                         long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
                         const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
                         float* __restrict__ partial_bias, int stages, int window) {
+  chain_wait();
   extern __shared__ uint4 ring_raw[];
   __shared__ __align__(16) float slots[2][2 * WINDOW_WARPS];
   uint8_t* ring = reinterpret_cast<uint8_t*>(ring_raw);  // [stage][x, dy]
@@ -864,6 +875,7 @@ short_norm_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __r
                        long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
                        const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
                        float* __restrict__ partial_bias) {
+  chain_wait();
   __shared__ float joined[2][32 * VEC * NV];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, packs = hidden / VEC;
   const float scale = 1.0f / static_cast<float>(hidden);
@@ -957,6 +969,8 @@ __global__ void __launch_bounds__(1024) long_row_norm_grad_kernel(const T* __res
                                                                   int hidden, const W* __restrict__ weight,
                                                                   const float* __restrict__ mean_in,
                                                                   const float* __restrict__ rstd_in, T* __restrict__ grad_x) {
+  chain_wait();
+  chain_next();
   __shared__ float slots[2 * MAX_WARPS];
   const long long row = blockIdx.x;
   const float scale = 1.0f / static_cast<float>(hidden);
@@ -985,6 +999,8 @@ __global__ void __launch_bounds__(256) column_grad_kernel(const T* __restrict__ 
                                                           const float* __restrict__ rstd_in,
                                                           float* __restrict__ partial_weight,
                                                           float* __restrict__ partial_bias) {
+  chain_wait();
+  chain_next();
   const int c = blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= hidden) return;
   float w = 0.0f, b = 0.0f;
@@ -1055,11 +1071,9 @@ long long grad_parts(long long rows, long long hidden) {
 template <typename T, typename W, int VEC, int NV, bool CENTER>
 int launch_short(const NormCall& c) {
   const long long blocks = (c.rows + SHORT_ROWS - 1) / SHORT_ROWS;
-  short_norm_kernel<T, W, VEC, NV, CENTER><<<static_cast<unsigned>(blocks), 32 * SHORT_ROWS, 0, c.stream>>>(
-      static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
-      c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(short_norm_kernel<T, W, VEC, NV, CENTER>, dim3(static_cast<unsigned>(blocks)), dim3(32 * SHORT_ROWS), 0,
+                        c.stream, static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight),
+                        static_cast<const W*>(c.bias), c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
 }
 
 constexpr int SM_SHARED = 227 * 1024;
@@ -1099,11 +1113,9 @@ int launch_stream(const NormCall& c) {
   int blocks = 0;
   if (int rc = resident_blocks(kernel, threads, bytes, known, &blocks)) return rc;
   const long long most = static_cast<long long>(blocks) * sm_count();
-  kernel<<<static_cast<unsigned>(c.rows < most ? c.rows : most), threads, bytes, c.stream>>>(
-      static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
-      c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(c.rows < most ? c.rows : most)), dim3(threads), bytes, c.stream,
+                        static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight),
+                        static_cast<const W*>(c.bias), c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
 }
 
 // Packs per thread, so that a row has about 256 threads and no more than STREAM_THREADS.
@@ -1123,11 +1135,10 @@ int launch_longest_grad(NormCall& c) {
   auto kernel = stream_longest_grad_kernel<T, W, NV, PITCH, CENTER>;
   if (int rc = allow_dynamic_smem(kernel, bytes, configured)) return rc;
   c.parts = static_cast<int>(c.rows < sm_count() ? c.rows : sm_count());
-  kernel<<<static_cast<unsigned>(c.parts), threads, bytes, c.stream>>>(
-      static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
-      static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(c.parts)), dim3(threads), bytes, c.stream,
+                        static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
+                        static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight,
+                        c.partial_bias);
 }
 
 template <typename T, typename W, int NV, int PITCH, bool CENTER>
@@ -1142,11 +1153,10 @@ int launch_wide_grad(NormCall& c) {
   if (blocks > grad_blocks(c.hidden)) blocks = grad_blocks(c.hidden);
   const long long most = static_cast<long long>(blocks) * sm_count();
   c.parts = static_cast<int>(c.rows < most ? c.rows : most);
-  kernel<<<static_cast<unsigned>(c.parts), threads, bytes, c.stream>>>(
-      static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
-      static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(c.parts)), dim3(threads), bytes, c.stream,
+                        static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
+                        static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight,
+                        c.partial_bias);
 }
 
 // Threads of the gradient of the longest rows that stream, 32 values each: three stages of x and dy fill shared memory.
@@ -1184,11 +1194,9 @@ int launch_window(const NormCall& c) {
   int blocks = 0;
   if (int rc = resident_blocks(kernel, threads, ring.bytes, known, &blocks)) return rc;
   const long long most = static_cast<long long>(blocks) * sm_count();
-  kernel<<<static_cast<unsigned>(c.rows < most ? c.rows : most), threads, ring.bytes, c.stream>>>(
-      static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
-      c.eps, static_cast<T*>(c.y), c.mean, c.rstd, ring.stages, ring.window);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(c.rows < most ? c.rows : most)), dim3(threads), ring.bytes, c.stream,
+                        static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight),
+                        static_cast<const W*>(c.bias), c.eps, static_cast<T*>(c.y), c.mean, c.rstd, ring.stages, ring.window);
 }
 
 template <typename T, typename W, int VEC, bool CENTER>
@@ -1208,11 +1216,9 @@ int forward(const NormCall& c) {
   if (c.hidden <= 32 * 16)
     return pairs ? launch_short<T, W, 2, 8, CENTER>(c) : launch_short<T, W, 1, 16, CENTER>(c);
   if (aligned_to(c.x, 16) && c.hidden <= WINDOW_MOST) return pairs ? window<T, W, 2, CENTER>(c) : window<T, W, 1, CENTER>(c);
-  long_row_norm_kernel<T, W, CENTER><<<static_cast<unsigned>(c.rows), 1024, 0, c.stream>>>(
-      static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
-      c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(long_row_norm_kernel<T, W, CENTER>, dim3(static_cast<unsigned>(c.rows)), dim3(1024), 0, c.stream,
+                        static_cast<const T*>(c.x), c.x_stride, c.rows, c.hidden, static_cast<const W*>(c.weight),
+                        static_cast<const W*>(c.bias), c.eps, static_cast<T*>(c.y), c.mean, c.rstd);
 }
 
 template <typename T, typename W, int VEC, int NV, bool CENTER>
@@ -1226,12 +1232,10 @@ int launch_window_grad(NormCall& c) {
   if (blocks > grad_blocks(c.hidden)) blocks = grad_blocks(c.hidden);
   const long long most = static_cast<long long>(blocks) * sm_count();
   c.parts = static_cast<int>(c.rows < most ? c.rows : most);
-  kernel<<<static_cast<unsigned>(c.parts), threads, ring.bytes, c.stream>>>(
-      static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
-      static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias, ring.stages,
-      ring.window);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(c.parts)), dim3(threads), ring.bytes, c.stream,
+                        static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
+                        static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight,
+                        c.partial_bias, ring.stages, ring.window);
 }
 
 template <typename T, typename W, int VEC, int NV, bool CENTER>
@@ -1243,11 +1247,10 @@ int launch_short_grad(NormCall& c) {
   const long long most = static_cast<long long>(blocks) * sm_count();
   const long long pieces = (c.rows + SHORT_WARPS - 1) / SHORT_WARPS;
   c.parts = static_cast<int>(pieces < most ? pieces : most);
-  short_norm_grad_kernel<T, W, VEC, NV, CENTER><<<static_cast<unsigned>(c.parts), 32 * SHORT_WARPS, 0, c.stream>>>(
-      static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
-      static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias);
-  HMC_LAUNCH_OK();
-  return 0;
+  return launch_chained(short_norm_grad_kernel<T, W, VEC, NV, CENTER>, dim3(static_cast<unsigned>(c.parts)),
+                        dim3(32 * SHORT_WARPS), 0, c.stream, static_cast<const T*>(c.x), c.x_stride,
+                        static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden, static_cast<const W*>(c.weight),
+                        c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight, c.partial_bias);
 }
 
 template <typename T, typename W, int VEC, bool CENTER>
@@ -1276,22 +1279,22 @@ int gradient(NormCall& c) {
     rc = pairs ? window_grad<T, W, 2, CENTER>(c) : window_grad<T, W, 1, CENTER>(c);
   } else {
     if (c.y != nullptr) {
-      long_row_norm_grad_kernel<T, W, CENTER><<<static_cast<unsigned>(c.rows), 1024, 0, c.stream>>>(
-          static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.hidden,
-          static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y));
-      HMC_LAUNCH_OK();
+      if (int rc = launch_chained(long_row_norm_grad_kernel<T, W, CENTER>, dim3(static_cast<unsigned>(c.rows)), dim3(1024), 0,
+                                  c.stream, static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad),
+                                  c.grad_stride, c.hidden, static_cast<const W*>(c.weight), c.mean_in, c.rstd_in,
+                                  static_cast<T*>(c.y))) return rc;
     }
     if (c.partial_weight != nullptr) {
       const dim3 grid((c.hidden + 255) / 256, c.parts);
-      column_grad_kernel<T, CENTER><<<grid, 256, 0, c.stream>>>(
-          static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden, c.mean_in,
-          c.rstd_in, c.partial_weight, c.partial_bias);
-      HMC_LAUNCH_OK();
+      if (int rc = launch_chained(column_grad_kernel<T, CENTER>, grid, dim3(256), 0, c.stream, static_cast<const T*>(c.x),
+                                  c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden, c.mean_in,
+                                  c.rstd_in, c.partial_weight, c.partial_bias)) return rc;
     }
   }
   if (rc != 0) return rc;
   if (c.partial_weight != nullptr) {
-    return launch_chained(param_grad_kernel<W>, dim3((c.hidden + 31) / 32), dim3(32, FINISH_SLICES), 0, c.stream, c.partial_weight,
+    return launch_chained(param_grad_kernel<W>, dim3((c.hidden + 31) / 32), dim3(32, FINISH_SLICES), 0, c.stream,
+                          c.partial_weight,
                           c.partial_bias, c.parts, c.hidden, static_cast<W*>(c.grad_weight), static_cast<W*>(c.grad_bias));
   }
   return 0;

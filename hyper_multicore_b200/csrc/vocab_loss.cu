@@ -656,7 +656,8 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
 
   if (warp == 0) {
     // ======================================================================== TMA producer (both CTAs)
-    // The weight does not come from this chain of launches: its first pieces are on their way before the tokens are packed.
+    // The weight was there before the packing pass began (which starts this launch early only once it has waited for what
+    // came before it): its first pieces are on their way before the tokens are packed.
     if (lane == 0) {
       const int first = pair * TILE + static_cast<int>(rank) * HALF, early = pair < tiles ? min(F::STAGES, kiters) : 0;
       for (int kb = 0; kb < early; ++kb) {
@@ -866,7 +867,8 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
                                                                  float* __restrict__ target_logit,
                                                                  float* __restrict__ token_loss) {
   __shared__ int place[PACK_TOKENS], known[PACK_TOKENS];  // packed row and target of a token, -1: none
-  chain_next();  // the first of its chain
+  chain_wait();
+  chain_next();
   const long long first = static_cast<long long>(blockIdx.x) * PACK_TOKENS;
   int before = 0;
   for (long long i = threadIdx.x; i < first; i += PACK_THREADS) before += targets.at(i) != targets.ignored;
@@ -1357,11 +1359,11 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
   float* token_loss = reduction == HMC_REDUCE_NONE ? loss : nullptr;
   const Targets given{targets, targets_i64, ignore_index, vocab};
   const int vector = aligned16(x) && x_stride % 8 == 0;
-  pack_rows_kernel<<<static_cast<unsigned>((tokens + PACK_TOKENS - 1) / PACK_TOKENS), PACK_THREADS, 0, s>>>(
-      static_cast<const __nv_bfloat16*>(x), x_stride, given, tokens, static_cast<int>(hidden), vector, st.count, st.done,
-      st.position,
-      st.row_of, st.labels, st.packed, static_cast<const __nv_bfloat16*>(weight), weight_stride, target_logit, token_loss);
-  HMC_LAUNCH_OK();
+  if (int rc = launch_chained(pack_rows_kernel, dim3(static_cast<unsigned>((tokens + PACK_TOKENS - 1) / PACK_TOKENS)), dim3(PACK_THREADS),
+                              0, s, static_cast<const __nv_bfloat16*>(x), x_stride, given, tokens, static_cast<int>(hidden), vector,
+                              st.count, st.done, st.position, st.row_of, st.labels, st.packed,
+                              static_cast<const __nv_bfloat16*>(weight), weight_stride, target_logit, token_loss))
+    return rc;
 
   Params p{};
   p.n = static_cast<int>(vocab), p.k = static_cast<int>(hidden);

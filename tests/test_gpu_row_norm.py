@@ -209,6 +209,43 @@ def test_rows_beyond_31_bits_of_elements():
         check(y[rows], [grads[0][rows], None, None], x[rows], None, None, x[rows], False, 1e-6)
 
 
+def test_early_started_launches_wait_for_what_they_read():
+    """Launches may be placed while the one before them runs: behind a slow copy in their own stream, and behind another stream's."""
+    from hyper_multicore_b200 import mega_cross_entropy
+
+    new, weight, bias, grad = make(600, 1024, torch.bfloat16, torch.bfloat16, True, seed=41)
+    head = (0.05 * torch.randn(3000, 1024, device="cuda")).bfloat16()
+    targets = torch.randint(0, 3000, (600,), device="cuda")
+    want = run(new, weight, bias, grad, True)
+    want_loss = mega_cross_entropy(new[:64], head, targets[:64], reduction="none")
+    x, w = torch.zeros_like(new), torch.zeros_like(head)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(20_000_000)
+    x.copy_(new)
+    w.copy_(head)
+    loss = mega_cross_entropy(x[:64], w, targets[:64], reduction="none")
+    got = run(x, weight, bias, grad, True)
+    torch.cuda.synchronize()
+    assert torch.equal(loss, want_loss)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
+    x.zero_()
+    w.zero_()
+    torch.cuda.synchronize()
+    maker, user = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(user):
+        call(new, weight, bias, True, 1e-6)  # a launch of ours is the last one in the stream
+    with torch.cuda.stream(maker):
+        torch.cuda._sleep(20_000_000)
+        x.copy_(new)
+        w.copy_(head)
+    user.wait_stream(maker)
+    with torch.cuda.stream(user):
+        y = call(x, weight, bias, True, 1e-6)
+        loss = mega_cross_entropy(x[:64], w, targets[:64], reduction="none")
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[0]) and torch.equal(loss, want_loss)
+
+
 @pytest.mark.parametrize("dtype,hidden", [(torch.bfloat16, 2560), (torch.bfloat16, 1001), (torch.bfloat16, 300), (torch.float32, 520)])
 def test_nothing_is_written_behind_the_rows(dtype, hidden):
     from hyper_multicore_b200 import _lib
