@@ -266,6 +266,33 @@ __device__ __forceinline__ float2 block_sum(float2 v, float* slots) {
   return make_float2(__shfl_sync(0xffffffffu, mine, 0), __shfl_sync(0xffffffffu, mine, 16));
 }
 
+// Of the pairs (or first values) of ROWS rows behind one barrier.
+template <int ROWS, bool BOTH>
+__device__ __forceinline__ void block_sums(float2 (&v)[ROWS], float* slots) {
+  const bool upper = (threadIdx.x & 16) != 0;
+  float mine[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (BOTH) {
+      mine[r] = over_16_lanes((upper ? v[r].y : v[r].x) + __shfl_xor_sync(0xffffffffu, upper ? v[r].x : v[r].y, 16));
+      if ((threadIdx.x & 15) == 0) slots[r * 2 * STREAM_WARPS + (threadIdx.x & 16) + (threadIdx.x >> 5)] = mine[r];
+    } else {
+      mine[r] = warp_sum(v[r].x);
+      if ((threadIdx.x & 31) == 0) slots[r * STREAM_WARPS + (threadIdx.x >> 5)] = mine[r];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (BOTH) {
+      mine[r] = over_16_lanes(slots[r * 2 * STREAM_WARPS + (threadIdx.x & 31)]);
+      v[r] = make_float2(__shfl_sync(0xffffffffu, mine[r], 0), __shfl_sync(0xffffffffu, mine[r], 16));
+    } else {
+      v[r].x = over_16_lanes(slots[r * STREAM_WARPS + (threadIdx.x & 15)]);
+    }
+  }
+}
+
 // A block walks the rows blockIdx.x, + gridDim.x, ... and copies the next ones asynchronously while it works on one: a ring
 // of rows in shared memory in which a thread writes and reads its own packs only, so that the copies need no barrier.
 // What is left per row is the reduction's, at which the blocks of an SM take turns: as many as their registers allow, with four
@@ -378,28 +405,29 @@ stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
 }
 
 // The gradient over the same ring, x and dy per stage. Threads own columns: the parameters' gradients stay in registers over
-// all rows of a block, so that x and dy are read once. Behind the reduction a row is widened again from the ring: kept in
-// registers its g and u would leave room for 14 warps per SM instead of 28 (16384 rows, layer norm, BF16: 2048 wide 67 against
-// 46 us, 4096 100 against 87, 7168 203 against 140). Bound by instructions where the values are 16 bits (22 per value, issue
-// slots 54 % busy; 16384 x 7168 140 us for 108 us of traffic), by memory in FP32 (8192 x 7168 106 us, the copy rate).
-constexpr int WIDE_THREADS = 448;  // a row of 7168
-template <typename T, typename W, int NV, int PITCH, bool CENTER>
-__global__ void __launch_bounds__(PITCH, 2 * WIDE_THREADS / PITCH > 0 ? 2 * WIDE_THREADS / PITCH : 1)
+// all rows of a block, so that x and dy are read once. Behind the reduction a row is widened again from the ring, since its g
+// and u kept in registers would leave room for half the warps. Two 16-bit rows go through a turn and share its barrier and its
+// loads of the weight (16384 rows, layer norm, BF16, against one row per turn: 1024 wide 20.6 us against 28, 2048 36 against
+// 46, 4096 66 against 87, 7168 126 against 140; the traffic alone takes 15.4, 31, 62 and 108). Three stages of two FP32 rows
+// do not fit, one row per turn is near the copy rate (8192 x 4096 67 us of 62, 8192 x 7168 116 of 108).
+constexpr int WIDE_THREADS = 448;  // rows of 4097 to 7168 values
+template <typename T, typename W, int NV, int ROWS, int PITCH, bool CENTER>
+__global__ void __launch_bounds__(PITCH, STREAM_THREADS / PITCH)
 stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
                         long long rows, int hidden, const W* __restrict__ weight, const float* __restrict__ mean_in,
                         const float* __restrict__ rstd_in, T* __restrict__ grad_x, float* __restrict__ partial_weight,
                         float* __restrict__ partial_bias) {
   chain_wait();
   extern __shared__ uint4 ring_raw[];
-  constexpr int stages = GRAD_STAGES, SUMS = CENTER ? 2 : 1;
-  __shared__ __align__(16) float slots[2][SUMS * STREAM_WARPS];
+  constexpr int stages = GRAD_STAGES, SUMS = (CENTER ? 2 : 1) * ROWS;
+  __shared__ float slots[2][SUMS * STREAM_WARPS];
   constexpr int PAIRS = Quad<T>::PAIRS, VEC = 2 * PAIRS;
   constexpr int WIDTH = NV * PITCH;  // known at compile time: offsets in the ring cost no arithmetic
   const int threads = blockDim.x;
   const int packs = hidden / VEC;
   const float scale = 1.0f / static_cast<float>(hidden);
-  uint4* ring = ring_raw + threadIdx.x;  // [stage][x, dy][NV][PITCH]; the weight in FP32 [NV][PAIRS / 2][PITCH]
-  float4* gain = reinterpret_cast<float4*>(ring_raw + 2 * stages * WIDTH) + threadIdx.x;
+  uint4* ring = ring_raw + threadIdx.x;  // [stage][row][x, dy][NV][PITCH]; the weight in FP32 [NV][PAIRS / 2][PITCH]
+  float4* gain = reinterpret_cast<float4*>(ring_raw + 2 * ROWS * stages * WIDTH) + threadIdx.x;
   for (int i = threadIdx.x; i < SUMS * STREAM_WARPS; i += threads) slots[0][i] = slots[1][i] = 0.0f;
   bool here[NV];
   float2 sum_weight[NV][PAIRS], sum_bias[CENTER ? NV : 1][PAIRS];
@@ -420,89 +448,112 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
     for (int i = 0; i < PAIRS; i += 2)
       gain[(j * PAIRS + i) / 2 * PITCH] = make_float4(w[i].x, w[i].y, w[i + 1].x, w[i + 1].y);
   }
-  const int step = gridDim.x, end = static_cast<int>(rows);
-  const T *src_x = x + blockIdx.x * x_stride + threadIdx.x * VEC, *src_grad = grad + blockIdx.x * grad_stride + threadIdx.x * VEC;
-  T* dst = grad_x + static_cast<long long>(blockIdx.x) * hidden + threadIdx.x * VEC;
+  const int first = ROWS * blockIdx.x, step = ROWS * gridDim.x, end = static_cast<int>(rows);
+  const T *src_x = x + first * x_stride + threadIdx.x * VEC, *src_grad = grad + first * grad_stride + threadIdx.x * VEC;
+  T* dst = grad_x + static_cast<long long>(first) * hidden + threadIdx.x * VEC;
   const long long x_step = step * x_stride, grad_step = step * grad_stride, dst_step = static_cast<long long>(step) * hidden;
-  int ahead = blockIdx.x;  // the next row to copy
+  int ahead = first;  // the next rows to copy
   auto fetch = [&](int stage) {
-    if (ahead < end) {
-      uint4* to = ring + stage * 2 * WIDTH;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (here[j]) {
-          copy_async_16(to + j * PITCH, src_x + j * threads * VEC);
-          copy_async_16(to + WIDTH + j * PITCH, src_grad + j * threads * VEC);
-        }
-      src_x += x_step, src_grad += grad_step;
-      ahead += step;
-    }
+    for (int r = 0; r < ROWS; ++r)
+      if (ahead + r < end) {
+        uint4* to = ring + (stage * ROWS + r) * 2 * WIDTH;
+        const T *a = src_x + r * x_stride, *d = src_grad + r * grad_stride;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (here[j]) {
+            copy_async_16(to + j * PITCH, a + j * threads * VEC);
+            copy_async_16(to + WIDTH + j * PITCH, d + j * threads * VEC);
+          }
+      }
+    src_x += x_step, src_grad += grad_step;
+    ahead = min(ahead + step, end);
     copy_async_commit();
   };
   for (int s = 0; s < stages - 1; ++s) fetch(s);
   __syncthreads();  // the slots are zero
   int stage = 0, last = stages - 1, turn = 0;
-  float next_mean = 0.0f, next_rstd = 0.0f;
-  auto stats = [&](int row) {
-    if (row < end) {
-      if (CENTER) next_mean = mean_in[row];
-      next_rstd = rstd_in[row];
+  float next_mean[ROWS], next_rstd[ROWS];
+  auto stats = [&](int row) {  // a row that does not exist has scale 0
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      next_mean[r] = CENTER && row + r < end ? mean_in[row + r] : 0.0f;
+      next_rstd[r] = row + r < end ? rstd_in[row + r] : 0.0f;
     }
   };
-  stats(blockIdx.x);
-  for (int row = blockIdx.x; row < end; row += step, turn ^= 1, dst += dst_step) {
-    const float mean = next_mean, rstd = next_rstd;
+  stats(first);
+  for (int row = first; row < end; row += step, turn ^= 1, dst += dst_step) {
+    float mean[ROWS], rstd[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) mean[r] = next_mean[r], rstd[r] = next_rstd[r];
     stats(row + step);
     fetch(last);
     copy_async_wait<stages - 1>();
-    const uint4* src = ring + stage * 2 * WIDTH;
-    float2 along = both(0.0f), total = both(0.0f);  // rstd times the sums of g (x - mean) and of g
-    auto widen = [&](int j, float2* c, float2* d, float2* w) {  // x - mean, dy, weight
-      Quad<T>::widen(src[j * PITCH], c);
-      Quad<T>::widen(src[WIDTH + j * PITCH], d);
+    const uint4* src = ring + stage * ROWS * 2 * WIDTH;
+    auto gains = [&](int j, float2* w) {
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) {
-        if (CENTER) c[i] = add2(c[i], both(-mean));
-        if ((i & 1) == 0) {
-          const float4 q = gain[(j * PAIRS + i) / 2 * PITCH];
-          w[i] = make_float2(q.x, q.y), w[i + 1] = make_float2(q.z, q.w);
-        }
+      for (int i = 0; i < PAIRS; i += 2) {
+        const float4 q = gain[(j * PAIRS + i) / 2 * PITCH];
+        w[i] = make_float2(q.x, q.y), w[i + 1] = make_float2(q.z, q.w);
       }
     };
+    auto widen = [&](int j, int r, float2* c, float2* d) {  // x - mean, dy
+      uint4 a = make_uint4(0, 0, 0, 0), b = a;
+      if (r == 0 || row + r < end) a = src[r * 2 * WIDTH + j * PITCH], b = src[(r * 2 + 1) * WIDTH + j * PITCH];
+      Quad<T>::widen(a, c);
+      Quad<T>::widen(b, d);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i)
+        if (CENTER) c[i] = add2(c[i], both(-mean[r]));
+    };
+    float2 along[ROWS], total[ROWS];  // rstd times the sums of g (x - mean) and of g
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) along[r] = total[r] = both(0.0f);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (here[j]) {
-        float2 c[PAIRS], d[PAIRS], w[PAIRS];
-        widen(j, c, d, w);
+        float2 w[PAIRS];
+        gains(j, w);
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-          if (CENTER) sum_bias[j][i] = add2(sum_bias[j][i], d[i]);
-          d[i] = times2(d[i], both(rstd));
-          sum_weight[j][i] = madd2(d[i], c[i], sum_weight[j][i]);
-          d[i] = times2(d[i], w[i]);
-          along = madd2(d[i], c[i], along);
-          if (CENTER) total = add2(total, d[i]);
-        }
-      }
-    float2 sums = make_float2(along.x + along.y, total.x + total.y);
-    if (CENTER) sums = block_sum(sums, slots[turn]);
-    else sums.x = block_sum(sums.x, slots[turn]);
-    if (grad_x != nullptr) {
-      // dx = rstd g - (x - mean) rstd^2 mean(g u) - rstd mean(g), u = (x - mean) rstd
-      const float2 back = both(-sums.x * scale * rstd * rstd), offset = both(CENTER ? -sums.y * scale : 0.0f);
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (here[j]) {
-          float2 c[PAIRS], d[PAIRS], w[PAIRS];
-          widen(j, c, d, w);
+        for (int r = 0; r < ROWS; ++r) {
+          float2 c[PAIRS], d[PAIRS];
+          widen(j, r, c, d);
 #pragma unroll
           for (int i = 0; i < PAIRS; ++i) {
-            d[i] = times2(d[i], both(rstd));
-            d[i] = CENTER ? madd2(d[i], w[i], offset) : times2(d[i], w[i]);
-            d[i] = madd2(c[i], back, d[i]);
+            if (CENTER) sum_bias[j][i] = add2(sum_bias[j][i], d[i]);
+            d[i] = times2(d[i], both(rstd[r]));
+            sum_weight[j][i] = madd2(d[i], c[i], sum_weight[j][i]);
+            d[i] = times2(d[i], w[i]);
+            along[r] = madd2(d[i], c[i], along[r]);
+            if (CENTER) total[r] = add2(total[r], d[i]);
           }
-          st_16(dst + j * threads * VEC, Quad<T>::narrow(d));
         }
+      }
+    float2 sums[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) sums[r] = make_float2(along[r].x + along[r].y, total[r].x + total[r].y);
+    block_sums<ROWS, CENTER>(sums, slots[turn]);
+    if (grad_x != nullptr) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (r > 0 && row + r >= end) break;
+        // dx = rstd g - (x - mean) rstd^2 mean(g u) - rstd mean(g), u = (x - mean) rstd
+        const float2 back = both(-sums[r].x * scale * rstd[r] * rstd[r]), offset = both(CENTER ? -sums[r].y * scale : 0.0f);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (here[j]) {
+            float2 c[PAIRS], d[PAIRS], w[PAIRS];
+            gains(j, w);
+            widen(j, r, c, d);
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+              d[i] = times2(d[i], both(rstd[r]));
+              d[i] = CENTER ? madd2(d[i], w[i], offset) : times2(d[i], w[i]);
+              d[i] = madd2(c[i], back, d[i]);
+            }
+            st_16(dst + r * hidden + j * threads * VEC, Quad<T>::narrow(d));
+          }
+      }
     }
     last = stage;
     if (++stage == stages) stage = 0;
@@ -1141,18 +1192,18 @@ int launch_longest_grad(NormCall& c) {
                         c.partial_bias);
 }
 
-template <typename T, typename W, int NV, int PITCH, bool CENTER>
+template <typename T, typename W, int NV, int ROWS, int PITCH, bool CENTER>
 int launch_wide_grad(NormCall& c) {
   constexpr int VEC = 16 / sizeof(T);
   const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
-  const int bytes = NV * PITCH * (GRAD_STAGES * 2 * 16 + VEC * 4);
+  const int bytes = NV * PITCH * (GRAD_STAGES * ROWS * 2 * 16 + VEC * 4);
   static Residency known{};
-  auto kernel = stream_wide_grad_kernel<T, W, NV, PITCH, CENTER>;
+  auto kernel = stream_wide_grad_kernel<T, W, NV, ROWS, PITCH, CENTER>;
   int blocks = 0;
   if (int rc = resident_blocks(kernel, threads, bytes, known, &blocks)) return rc;
   if (blocks > grad_blocks(c.hidden)) blocks = grad_blocks(c.hidden);
-  const long long most = static_cast<long long>(blocks) * sm_count();
-  c.parts = static_cast<int>(c.rows < most ? c.rows : most);
+  const long long most = static_cast<long long>(blocks) * sm_count(), pieces = (c.rows + ROWS - 1) / ROWS;
+  c.parts = static_cast<int>(pieces < most ? pieces : most);
   return launch_chained(kernel, dim3(static_cast<unsigned>(c.parts)), dim3(threads), bytes, c.stream,
                         static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.grad), c.grad_stride, c.rows, c.hidden,
                         static_cast<const W*>(c.weight), c.mean_in, c.rstd_in, static_cast<T*>(c.y), c.partial_weight,
@@ -1165,12 +1216,13 @@ constexpr int LONGEST = sizeof(T) == 4 ? 288 : STREAM_THREADS;
 
 template <typename T, typename W, bool CENTER>
 int stream_grad(NormCall& c) {
-  constexpr int NV = sizeof(T) == 4 ? 4 : 2;  // 16 values per thread
-  if (c.hidden <= 16 * 64) return launch_wide_grad<T, W, NV, 64, CENTER>(c);
-  if (c.hidden <= 16 * 128) return launch_wide_grad<T, W, NV, 128, CENTER>(c);
-  if (c.hidden <= 16 * 256) return launch_wide_grad<T, W, NV, 256, CENTER>(c);
-  if (c.hidden <= 16 * WIDE_THREADS) return launch_wide_grad<T, W, NV, WIDE_THREADS, CENTER>(c);
-  if (c.hidden <= 16 * STREAM_THREADS) return launch_wide_grad<T, W, NV, STREAM_THREADS, CENTER>(c);
+  constexpr int NV = sizeof(T) == 4 ? 4 : 2;    // 16 values per thread
+  constexpr int ROWS = sizeof(T) == 4 ? 1 : 2;  // three stages of two FP32 rows do not fit shared memory
+  if (c.hidden <= 16 * 64) return launch_wide_grad<T, W, NV, ROWS, 64, CENTER>(c);
+  if (c.hidden <= 16 * 128) return launch_wide_grad<T, W, NV, ROWS, 128, CENTER>(c);
+  if (c.hidden <= 16 * 256) return launch_wide_grad<T, W, NV, ROWS, 256, CENTER>(c);
+  if (c.hidden <= 16 * WIDE_THREADS) return launch_wide_grad<T, W, NV, ROWS, WIDE_THREADS, CENTER>(c);
+  if (c.hidden <= 16 * STREAM_THREADS) return launch_wide_grad<T, W, NV, ROWS, STREAM_THREADS, CENTER>(c);
   return launch_longest_grad<T, W, 2 * NV, LONGEST<T>, CENTER>(c);
 }
 
