@@ -416,11 +416,11 @@ SIGNATURES: dict[str, tuple] = {
     "hmc_mega_moe_mxfp8": (_I, [ctypes.POINTER(MegaMoeMxfp8Args), _P]),
     "hmc_mega_moe_mxfp8_grad": (_I, [ctypes.POINTER(MegaMoeMxfp8GradArgs), _P]),
     "hmc_mega_moe_mxfp8_abi_version": (_I, []),
-    "hmc_vocab_loss_state_bytes": (_L, [_L, _L]),
+    "hmc_vocab_loss_state_bytes": (_L, [_L, _L, _L, _I]),
     "hmc_vocab_loss_workspace_bytes": (_L, [_L, _L]),
-    "hmc_vocab_loss": (_I, [_P, _L, _P, _L, _P, _I, _L, _L, _L, _L, _I, _P, _P, _P, _L, _P, _P]),
+    "hmc_vocab_loss": (_I, [_P, _L, _P, _L, _P, _I, _L, _L, _L, _L, _I, _I, _P, _P, _P, _L, _P, _P]),
     "hmc_vocab_loss_grad_workspace_bytes": (_L, [_L, _L, _L]),
-    "hmc_vocab_loss_grad": (_I, [_P, _P, _L, _L, _L, _L, _I, _P, _P, _P, _P, _L, _P, _P]),
+    "hmc_vocab_loss_grad": (_I, [_P, _P, _L, _L, _L, _L, _I, _I, _P, _P, _P, _P, _L, _P, _P]),
     "hmc_row_norm": (_I, [_P, _L, _L, _L, _I, _P, _P, _I, _I, _F, _P, _P, _P, _P]),
     "hmc_row_norm_grad_workspace_bytes": (_L, [_L, _L]),
     "hmc_row_norm_grad": (_I, [_P, _L, _P, _L, _L, _L, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P, _L, _P]),

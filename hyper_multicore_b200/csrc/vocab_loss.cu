@@ -1,4 +1,4 @@
-// Cross entropy of hidden states over a vocabulary, without keeping the logits:
+// Cross entropy of hidden states over a vocabulary, without logits in full:
 //   l_ij = x_i . w_j,  lse_i = log sum_j exp(l_ij),  loss_i = lse_i - l_i,t(i)
 //   p_ij = exp(l_ij - lse_i)
 //   dx_i = g_i (sum_{j != t(i)} p_ij w_j + (p_i,t(i) - 1) w_t(i))
@@ -7,13 +7,15 @@
 // rows that count are packed, and every kernel takes their number from the device.
 //
 // Forward: one GEMM over 256 x 256 tiles whose epilogue keeps a row's maximum and sum of exponentials per 128 columns, and
-// a kernel that joins those. Gradient: the same GEMM again, its epilogue writes p in BF16 for a piece of the vocabulary,
-// and two GEMMs take the piece to the two gradients. p without the target's entry only: that one is p - 1, which cancels for
-// a token the model is sure of and carries the largest weight for one it is not, so it stays in FP32 (expm1 of -loss) and
-// meets the products in FP32: for dx as the row w_t(i) in the epilogue, for dw as a sum over the tokens of a word made
-// beforehand. The rounding of the other entries to BF16 (2^-8 of the value at most) averages over a sum of many.
-// The logits are computed twice on purpose: kept as BF16 they would be the tensor of tokens x vocabulary that this operator
-// is there to avoid, and gradients taken in the forward pass would hold the weight's gradient in FP32 until the backward one.
+// a kernel that joins those. Gradient: p in BF16 for a piece of the vocabulary, from what the forward kept of the logits or
+// from the same GEMM again, and two GEMMs that take the piece to the two gradients. p without the target's entry only: that
+// one is p - 1, which cancels for a token the model is sure of and carries the largest weight for one it is not, so it stays
+// in FP32 (expm1 of -loss) and meets the products in FP32: for dx as the row w_t(i) in the epilogue, for dw as a sum over the
+// tokens of a word made beforehand. The rounding of the other entries to BF16 (2^-8 of the value at most) averages over a sum
+// of many.
+// A training step of 8192 x 4096 x 131072 takes 23.2 ms with all its logits kept (2 GiB of 16-bit codes) and 28.4 ms with none,
+// 512 x 1024 x 32000 168 against 194 us. Gradients taken in the forward pass would hold the weight's gradient in FP32 until the
+// backward one and only fit a loss that is reduced.
 //
 // The GEMM: CTA pairs (tcgen05.mma.cta_group::2, M = N = 256), one TMA producer, one issuer, eight epilogue warps, two
 // accumulators; the layouts of the operands are those of the grouped GEMMs. Bound by the tensor cores: 4096 x 32768 x 4096 takes
@@ -67,6 +69,8 @@ struct Params {
   const float* coef;   // [rows] weight * (p_target - 1)
   float2* partial;     // STATS: [2 * n_tiles][pitch] maximum and sum
   long long pitch;
+  int kept;            // STATS: the words whose codes are stored, in whole tiles
+  float* tops;         // STATS: [kept / HALF][pitch] what the codes count from
   int first_word;       // PROBS, GRAD_*: first word of the piece
   const int* row_of;    // GRAD_HIDDEN: token of a packed row
   float* sums;          // GRAD_HIDDEN: [rows, n] FP32 sums over pieces, or NULL
@@ -134,9 +138,55 @@ struct Walker {
 
 __device__ __forceinline__ float shifted_exp(float v, float top) { return __expf(v - top); }
 
-// Maximum and sum of exponentials of one row's 128 columns, without the target's.
-__device__ __forceinline__ void epilogue_stats(const Params& p, float (&v)[HALF], int row, int col, int half_tile) {
-  const int label = p.labels[row] - col;
+// A kept logit: how far it is below the largest of its row's 128 columns, in steps of 2^-10 of a power of two. Rounding to
+// a step is off by 2^-11 of one, 3.4e-4 of the probability, a twelfth of what BF16 adds afterwards. Codes end at 64 powers of two:
+// what is further below, 5e-20 of the largest, is zero, as are the target's entry and the columns behind the vocabulary.
+constexpr float CODE_STEPS = 1024.0f;
+constexpr float LOG2_E = 1.44269504f;
+constexpr float ROUND = 8388608.0f;  // 2^23: a sum with it is a whole number, in the low bits of the word
+constexpr unsigned CODE_ZERO = 0xffff;
+
+__device__ __forceinline__ uint32_t codes_of(float below0, float below1) {
+  const float last = ROUND + static_cast<float>(CODE_ZERO);  // NaN too: its row's sum is NaN, which is enough
+  const float a = fminf(__fmaf_rn(below0, -CODE_STEPS * LOG2_E, ROUND), last);
+  const float b = fminf(__fmaf_rn(below1, -CODE_STEPS * LOG2_E, ROUND), last);
+  return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410);
+}
+
+// 32 x 32 values of 16 bits leave as one box through shared memory; two boxes per warp in flight. A lane's row of values.
+__device__ __forceinline__ void store_box(const CUtensorMap* tm, uint8_t* stage, unsigned& issued, const uint4 (&q)[4], int col,
+                                          int row, int lane) {
+  uint8_t* box = stage + (issued & 1) * (STORE_STAGE_BYTES / 2);
+  if (issued > 1) {
+    if (lane == 0) bulk_wait_read_but_one();
+    __syncwarp();
+  }
+  uint8_t* base = box + lane * 64;  // 64-byte rows under the 64-byte swizzle
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(base + ((i ^ ((lane >> 1) & 3)) << 4)) = q[i];
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(tm, box, col, row);
+    bulk_commit_group();
+  }
+  ++issued;
+}
+__device__ __forceinline__ void store_box(const CUtensorMap* tm, uint8_t* stage, unsigned& issued, const float* v, int col,
+                                          int row, int lane) {
+  uint4 q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    q[i] = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                      pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
+  store_box(tm, stage, issued, q, col, row, lane);
+}
+
+// Maximum and sum of exponentials of one row's 128 columns, without the target's; codes of the words that are kept.
+__device__ __forceinline__ void epilogue_stats(const Params& p, const CUtensorMap* tm, uint8_t* stage, unsigned& issued,
+                                               float (&v)[HALF], int first_row, int row, bool row_ok, int col, int half_tile,
+                                               int lane) {
+  const int label = row_ok ? p.labels[row] - col : -1;
   if (col + HALF > p.n) {
 #pragma unroll
     for (int j = 0; j < HALF; ++j)
@@ -155,30 +205,21 @@ __device__ __forceinline__ void epilogue_stats(const Params& p, float (&v)[HALF]
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < HALF; ++j) sum[j & 3] += shifted_exp(v[j], shift);
-  p.partial[half_tile * p.pitch + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-}
-
-// 32 x 32 values leave as one BF16 box through shared memory; two boxes per warp in flight.
-__device__ __forceinline__ void store_box(const CUtensorMap* tm, uint8_t* stage, unsigned& issued, const float* v, int col,
-                                          int row, int lane) {
-  uint8_t* box = stage + (issued & 1) * (STORE_STAGE_BYTES / 2);
-  if (issued > 1) {
-    if (lane == 0) bulk_wait_read_but_one();
-    __syncwarp();
-  }
-  uint8_t* base = box + lane * 64;  // 64-byte rows under the 64-byte swizzle
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    *reinterpret_cast<uint4*>(base + ((q ^ ((lane >> 1) & 3)) << 4)) =
-        make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                   pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
-  fence_proxy_async_smem();
+  if (row_ok) p.partial[half_tile * p.pitch + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (col >= p.kept) return;
+  if (row_ok) p.tops[half_tile * p.pitch + row] = top;
   __syncwarp();
-  if (lane == 0) {
-    tma_store_2d(tm, box, col, row);
-    bulk_commit_group();
+#pragma unroll
+  for (int c = 0; c < HALF; c += 32) {
+    uint4 q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* b = v + c + 8 * i;
+      q[i] = make_uint4(codes_of(b[0] - shift, b[1] - shift), codes_of(b[2] - shift, b[3] - shift),
+                        codes_of(b[4] - shift, b[5] - shift), codes_of(b[6] - shift, b[7] - shift));
+    }
+    store_box(tm, stage, issued, q, col + c, first_row, lane);
   }
-  ++issued;
 }
 
 // 64 columns of the accumulator row of each lane: two loads under way at a time.
@@ -543,7 +584,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           }
           release();
         }
-        if (ok && row_ok) epilogue_stats(p, v, row, col, 2 * u.ni + half);
+        if (ok) epilogue_stats(p, &tm_c, my_stage, issued, v, first_row, row, row_ok, col, 2 * u.ni + half, lane);
         __syncwarp();
         continue;
       }
@@ -1036,6 +1077,51 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
   }
 }
 
+// p of a piece of the vocabulary out of its codes, times the row's gradient: what PROBS computes from the logits. A warp per row
+// and 1024 words, eight rows per block; rows behind the last one that the products read with it are zero. Bound by memory:
+// 3687 x 65536 178 us (0.97 GB, 5.4 TB/s) where the product takes 1400.
+constexpr int SPREAD_WORDS = 1024;
+__global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict__ codes, long long codes_pitch,
+                                                     const float* __restrict__ tops, long long tops_pitch, int first_word, int width,
+                                                     const int* __restrict__ count, const float* __restrict__ lse,
+                                                     const float* __restrict__ weights, long long tokens,
+                                                     __nv_bfloat16* __restrict__ probs, long long probs_pitch) {
+  chain_wait();
+  chain_next();
+  const int rows = *count;
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= (rows + TILE - 1) / TILE * TILE || row >= tokens) return;
+  const int col = blockIdx.y * SPREAD_WORDS + (threadIdx.x & 31) * 8;
+  const bool row_ok = row < rows;
+  const float norm = row_ok ? lse[row] : 0.0f, weight = row_ok ? weights[row] : 0.0f;
+  const uint16_t* src = codes + row * codes_pitch + first_word + col;
+  __nv_bfloat16* dst = probs + row * probs_pitch + col;
+  uint4 q[SPREAD_WORDS / 256];
+  float from[SPREAD_WORDS / 256];
+#pragma unroll
+  for (int i = 0; i < SPREAD_WORDS / 256; ++i) {
+    if (!row_ok || col + 256 * i >= width) continue;
+    q[i] = ld_16(src + 256 * i);
+    from[i] = tops[(first_word + col + 256 * i) / HALF * tops_pitch + row];
+  }
+#pragma unroll
+  for (int i = 0; i < SPREAD_WORDS / 256; ++i) {
+    if (col + 256 * i >= width) break;
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (row_ok) {
+      const float above = (from[i] - norm) * LOG2_E;
+      auto two = [&](uint32_t pair) {
+        const unsigned lo = pair & 0xffffu, hi = pair >> 16;
+        const float a = lo == CODE_ZERO ? -INFINITY : static_cast<float>(lo) * (-1.0f / CODE_STEPS);
+        const float b = hi == CODE_ZERO ? -INFINITY : static_cast<float>(hi) * (-1.0f / CODE_STEPS);
+        return pack_bf16x2(exp2f(above + a) * weight, exp2f(above + b) * weight);
+      };
+      out = make_uint4(two(q[i].x), two(q[i].y), two(q[i].z), two(q[i].w));
+    }
+    st_16(dst + 256 * i, out);
+  }
+}
+
 // The sum of coef_i x_i over the rows that have a word as target, in their order, in slices of WORD_SLICE rows of a word:
 // every row that is the first of a slice adds up its slice, into word_sums at its own row. (8192 tokens of 4096 by a power law, the
 // commonest word with 480 of them: one block for all rows of a word 391 us, slices 74 us and their joining about 10.)
@@ -1228,13 +1314,39 @@ int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
 
 long long up256(long long bytes) { return (bytes + 255) / 256 * 256; }
 
+constexpr long long FEW_TOKENS = 128;
+
+// A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size. A training step of
+// 8192 x 4096 x 131072 without kept logits, with pieces of 256 MiB 29.0 ms, 512 28.6, 1 GiB 28.8, 2 GiB (one piece) 30.1.
+constexpr long long PIECE_BYTES = 512ll << 20;
+long long piece_words(long long tokens, long long vocab) {
+  long long most = PIECE_BYTES / (2 * tokens) / TILE * TILE;
+  if (most < 4096) most = 4096;
+  const long long pieces = (vocab + most - 1) / most;
+  return tiles_of((vocab + pieces - 1) / pieces) * TILE;
+}
+
+// The words whose codes a forward leaves: as many pieces as KEEP_BYTES hold (a fortieth of the GPU's memory), in whole tiles.
+// Kept against computed again: 4096 x 1024 x 32000 743 and 878 us, 16384 x 2048 x 131072 (all of it) 24.0 and 28.7 ms, twice the
+// tokens (half of it) 53.9 and 61.8, 131072 x 512 x 65536 (a quarter of it) 44.9 and 45.9. The
+// few-token kernel keeps none: with so few rows the logits cost one pass over the weight.
+constexpr long long KEEP_BYTES = 4ll << 30;
+long long kept_words(long long tokens, long long vocab) {
+  if (tokens <= FEW_TOKENS) return 0;
+  const long long piece = piece_words(tokens, vocab), most = KEEP_BYTES / (2 * tokens * piece) * piece, all = tiles_of(vocab) * TILE;
+  return most < all ? most : all;
+}
+
 // What a forward leaves for its gradient, in one buffer of the caller.
 struct State {
   int *count, *done, *position, *row_of, *labels;
   float *lse, *losses;
   __nv_bfloat16* packed;
-  long long bytes;
-  State(void* base, long long tokens, long long hidden) {
+  uint16_t* codes;  // [tokens][kept]
+  float* tops;      // [kept / HALF][tokens]
+  long long kept, bytes;
+  State(void* base, long long tokens, long long hidden, long long vocab, bool keep) {
+    kept = keep ? kept_words(tokens, vocab) : 0;
     char* p = static_cast<char*>(base);
     const long long words = up256(4 * tokens);
     count = reinterpret_cast<int*>(p);
@@ -1245,11 +1357,12 @@ struct State {
     lse = reinterpret_cast<float*>(p + 256 + 3 * words);
     losses = reinterpret_cast<float*>(p + 256 + 4 * words);
     packed = reinterpret_cast<__nv_bfloat16*>(p + 256 + 5 * words);
-    bytes = 256 + 5 * words + 2 * tokens * hidden;
+    const long long at = 256 + 5 * words + up256(2 * tokens * hidden);
+    codes = reinterpret_cast<uint16_t*>(p + at);
+    tops = reinterpret_cast<float*>(p + at + 2 * tokens * kept);
+    bytes = at + 2 * tokens * kept + 4 * tokens * (kept / HALF);
   }
 };
-
-constexpr long long FEW_TOKENS = 128;
 
 // Parts that a launch over `vocab` words leaves per token: one per epilogue warp and column, or two per tile.
 long long few_parts(long long vocab) {
@@ -1267,16 +1380,6 @@ int launch_few(const CUtensorMap& words, const State& st, long long hidden, long
   *parts = static_cast<int>(few_parts(p.n));
   return launch_chained(few_tokens_kernel<N>, dim3(*parts / 4), dim3(Few<N>::THREADS), Few<N>::SMEM, stream, words, rows, p.n,
                         (p.k + BK - 1) / BK, p.count, p.labels, p.partial, p.pitch, p.status);
-}
-
-// A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size. A training step of
-// 8192 x 4096 x 131072 with pieces of 256 MiB 29.0 ms, 512 28.6, 1 GiB 28.8, 2 GiB (one piece) 30.1.
-constexpr long long PIECE_BYTES = 512ll << 20;
-long long piece_words(long long tokens, long long vocab) {
-  long long most = PIECE_BYTES / (2 * tokens) / TILE * TILE;
-  if (most < 4096) most = 4096;
-  const long long pieces = (vocab + most - 1) / most;
-  return tiles_of((vocab + pieces - 1) / pieces) * TILE;
 }
 
 struct GradSpace {
@@ -1325,8 +1428,8 @@ int check_sizes(const char* name, int64_t tokens, int64_t hidden, int64_t vocab,
 }  // namespace
 }  // namespace hmc
 
-extern "C" int64_t hmc_vocab_loss_state_bytes(int64_t tokens, int64_t hidden) {
-  return tokens > 0 && hidden > 0 ? hmc::State(nullptr, tokens, hidden).bytes : 0;
+extern "C" int64_t hmc_vocab_loss_state_bytes(int64_t tokens, int64_t hidden, int64_t vocab, int keep) {
+  return tokens > 0 && hidden > 0 && vocab > 0 ? hmc::State(nullptr, tokens, hidden, vocab, keep != 0).bytes : 0;
 }
 
 extern "C" int64_t hmc_vocab_loss_workspace_bytes(int64_t tokens, int64_t vocab) {
@@ -1343,7 +1446,7 @@ extern "C" int64_t hmc_vocab_loss_grad_workspace_bytes(int64_t tokens, int64_t h
 
 extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* targets,
                               int targets_i64, int64_t tokens, int64_t hidden, int64_t vocab, int64_t ignore_index, int reduction,
-                              void* state, float* loss, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+                              int keep, void* state, float* loss, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
   using namespace hmc;
   if (int rc = check_sizes("hmc_vocab_loss", tokens, hidden, vocab, weight_stride, weight, reduction)) return rc;
   HMC_REQUIRE(x != nullptr && targets != nullptr && state != nullptr && loss != nullptr && x_stride >= 0, HMC_ERR_INVALID,
@@ -1353,7 +1456,7 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
               HMC_ERR_INVALID, "hmc_vocab_loss: the workspace must hold %lld bytes, it and the state on 16-byte boundaries",
               (long long)hmc_vocab_loss_workspace_bytes(tokens, vocab));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const State st(state, tokens, hidden);
+  const State st(state, tokens, hidden, vocab, keep != 0);
   float* target_logit = static_cast<float*>(workspace);
   float2* partial = reinterpret_cast<float2*>(static_cast<char*>(workspace) + up256(4 * tokens));
   float* token_loss = reduction == HMC_REDUCE_NONE ? loss : nullptr;
@@ -1378,7 +1481,12 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
     if (rc != 0) return rc;
   } else {
     if (int rc = map_k_major(&a, st.packed, hidden, tokens, hidden)) return rc;
-    if (int rc = launch_product<STATS>(a, b, a, p, tiles_of(tokens) * tiles_of(vocab), s)) return rc;
+    CUtensorMap codes = a;
+    if (st.kept > 0) {
+      if (int rc = map_store(&codes, st.codes, st.kept, tokens, st.kept)) return rc;
+      p.kept = static_cast<int>(st.kept), p.tops = st.tops;
+    }
+    if (int rc = launch_product<STATS>(a, b, codes, p, tiles_of(tokens) * tiles_of(vocab), s)) return rc;
     parts = static_cast<int>(2 * tiles_of(vocab));
   }
   return launch_chained(join_kernel, dim3(static_cast<unsigned>((tokens + 31) / 32)), dim3(32, JOIN_SLICES), 0, s, partial, tokens, parts,
@@ -1386,7 +1494,7 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
 }
 
 extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_t weight_stride, int64_t tokens, int64_t hidden,
-                                   int64_t vocab, int reduction, const float* grad_loss, void* grad_hidden, void* grad_weight,
+                                   int64_t vocab, int reduction, int keep, const float* grad_loss, void* grad_hidden, void* grad_weight,
                                    void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
   using namespace hmc;
   if (int rc = check_sizes("hmc_vocab_loss_grad", tokens, hidden, vocab, weight_stride, weight, reduction)) return rc;
@@ -1400,7 +1508,7 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
               HMC_ERR_INVALID, "hmc_vocab_loss_grad: the workspace must hold %lld bytes on a 16-byte boundary",
               (long long)hmc_vocab_loss_grad_workspace_bytes(tokens, hidden, vocab));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const State st(const_cast<void*>(state), tokens, hidden);
+  const State st(const_cast<void*>(state), tokens, hidden, vocab, keep != 0);
   const GradSpace w(workspace, tokens, hidden, vocab);
   const int width = static_cast<int>(hidden);
   if (grad_weight != nullptr) HMC_CUDA_OK(cudaMemsetAsync(w.slots, 0xff, w.slot_bytes, s));  // no first row, -1 members
@@ -1429,12 +1537,21 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
     const long long words = vocab - first < w.piece ? vocab - first : w.piece;
     const __nv_bfloat16* head = static_cast<const __nv_bfloat16*>(weight) + first * weight_stride;
     CUtensorMap head_k, head_mn, probs_store, probs_k, probs_mn;
-    if (int rc = map_k_major(&head_k, head, hidden, words, weight_stride)) return rc;
-    if (int rc = map_store(&probs_store, w.probs, words, tokens, w.piece)) return rc;
     Params p = base;
     p.first_word = static_cast<int>(first);
     p.n = static_cast<int>(words), p.k = width;
-    if (int rc = launch_product<PROBS>(rows_k, head_k, probs_store, p, tiles_of(tokens) * tiles_of(words), s)) return rc;
+    if (first < st.kept) {
+      const int whole = static_cast<int>(tiles_of(words) * TILE);
+      if (int rc = launch_chained(spread_kernel,
+                                  dim3(static_cast<unsigned>((tokens + 7) / 8), (whole + SPREAD_WORDS - 1) / SPREAD_WORDS), dim3(256), 0,
+                                  s, st.codes, st.kept, st.tops, tokens, p.first_word, whole, st.count, st.lse, w.weights, tokens,
+                                  w.probs, w.piece))
+        return rc;
+    } else {
+      if (int rc = map_k_major(&head_k, head, hidden, words, weight_stride)) return rc;
+      if (int rc = map_store(&probs_store, w.probs, words, tokens, w.piece)) return rc;
+      if (int rc = launch_product<PROBS>(rows_k, head_k, probs_store, p, tiles_of(tokens) * tiles_of(words), s)) return rc;
+    }
     if (grad_hidden != nullptr) {
       if (int rc = map_k_major(&probs_k, w.probs, words, tokens, w.piece)) return rc;
       if (int rc = map_mn_major(&head_mn, head, hidden, words, weight_stride)) return rc;

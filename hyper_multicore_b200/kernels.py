@@ -820,22 +820,26 @@ def row_norm_grad(grad, x, weight, stats, center: bool, affine_dtype, need_x: bo
     return grad_x, grad_weight, grad_bias
 
 
-def vocab_loss(x, weight, targets, *, ignore_index: int, reduction: str, status=None):
-    """Cross entropy of ``x`` [T, H] against ``weight`` [V, H] and ``targets`` [T]: (loss [T] or [], state for the gradient)."""
+def vocab_loss(x, weight, targets, *, ignore_index: int, reduction: str, keep: bool = False, status=None):
+    """Cross entropy of ``x`` [T, H] against ``weight`` [V, H] and ``targets`` [T]: (loss [T] or [], state for the gradient).
+
+    With ``keep`` the state holds the logits of as many words as 4 GiB do, in 16 bits each.
+    """
     device = _require_cuda(x, weight, targets)
     (tokens, hidden), vocab = x.shape, weight.shape[0]
     loss = torch.empty((tokens,) if reduction == "none" else (), dtype=torch.float32, device=device)
-    state = torch.empty(_size("hmc_vocab_loss_state_bytes", tokens, hidden), dtype=torch.uint8, device=device)
+    state = torch.empty(_size("hmc_vocab_loss_state_bytes", tokens, hidden, vocab, keep), dtype=torch.uint8, device=device)
     need = _size("hmc_vocab_loss_workspace_bytes", tokens, vocab)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _call("hmc_vocab_loss", device, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), targets.data_ptr(),
-          targets.dtype == torch.int64, tokens, hidden, vocab, ignore_index, _lib.HMC_REDUCE[reduction], state.data_ptr(),
-          loss.data_ptr(), workspace.data_ptr(), need, _lib.ptr(status))
+          targets.dtype == torch.int64, tokens, hidden, vocab, ignore_index, _lib.HMC_REDUCE[reduction], keep,
+          state.data_ptr(), loss.data_ptr(), workspace.data_ptr(), need, _lib.ptr(status))
     return loss, state
 
 
-def vocab_loss_grad(grad_loss, state, weight, tokens: int, *, reduction: str, need_hidden: bool, need_weight: bool, status=None):
-    """Gradients of ``vocab_loss`` from its state: (grad_hidden [T, H], grad_weight [V, H]), None where not needed."""
+def vocab_loss_grad(grad_loss, state, weight, tokens: int, *, reduction: str, need_hidden: bool, need_weight: bool,
+                    keep: bool = False, status=None):
+    """Gradients of ``vocab_loss`` from its state (``keep`` as there): (grad_hidden [T, H], grad_weight [V, H]), None where not needed."""
     device = _require_cuda(grad_loss, state, weight)
     vocab, hidden = weight.shape
     grad_hidden = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=device) if need_hidden else None
@@ -843,6 +847,6 @@ def vocab_loss_grad(grad_loss, state, weight, tokens: int, *, reduction: str, ne
     need = _size("hmc_vocab_loss_grad_workspace_bytes", tokens, hidden, vocab)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _call("hmc_vocab_loss_grad", device, state.data_ptr(), weight.data_ptr(), weight.stride(0), tokens, hidden, vocab,
-          _lib.HMC_REDUCE[reduction], grad_loss.data_ptr(), _lib.ptr(grad_hidden), _lib.ptr(grad_weight), workspace.data_ptr(),
-          need, _lib.ptr(status))
+          _lib.HMC_REDUCE[reduction], keep, grad_loss.data_ptr(), _lib.ptr(grad_hidden), _lib.ptr(grad_weight),
+          workspace.data_ptr(), need, _lib.ptr(status))
     return grad_hidden, grad_weight

@@ -1,4 +1,4 @@
-"""MegaCrossEntropy: the head of a model and its loss over the vocabulary in one, without the logits.
+"""MegaCrossEntropy: the head of a model and its loss over the vocabulary in one, without logits in full.
 
 The reference ends before the head; this is the operator that follows the last norm in training and in scoring.
 """
@@ -65,24 +65,24 @@ def _weight_rows(weight: torch.Tensor) -> torch.Tensor:
     return weight.clone(memory_format=torch.contiguous_format)
 
 
-def _forward(rows, weight, targets, ignore_index, reduction):
+def _forward(rows, weight, targets, ignore_index, reduction, keep=False):
     """(loss, state); without a token the empty tensor, sum or mean."""
     if targets.numel() == 0:
         f32 = dict(dtype=torch.float32, device=rows.device)
         loss = torch.empty(0, **f32) if reduction == "none" else torch.full((), math.nan if reduction == "mean" else 0.0, **f32)
         return loss, None
-    return kernels.vocab_loss(rows, weight, targets, ignore_index=ignore_index, reduction=reduction)
+    return kernels.vocab_loss(rows, weight, targets, ignore_index=ignore_index, reduction=reduction, keep=keep)
 
 
 class _CrossEntropyFunction(torch.autograd.Function):
     """Loss of packed rows with its matching backward; first order."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, reduction):  # pylint: disable=arguments-differ
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction, keep):  # pylint: disable=arguments-differ
         rows_of_weight = _weight_rows(weight)
-        loss, state = _forward(hidden, rows_of_weight, targets, ignore_index, reduction)
+        loss, state = _forward(hidden, rows_of_weight, targets, ignore_index, reduction, keep)
         ctx.save_for_backward(state, rows_of_weight)
-        ctx.tokens, ctx.reduction = hidden.shape[0], reduction
+        ctx.tokens, ctx.reduction, ctx.keep = hidden.shape[0], reduction, keep
         return loss
 
     @staticmethod
@@ -91,30 +91,34 @@ class _CrossEntropyFunction(torch.autograd.Function):
         state, weight = ctx.saved_tensors
         if ctx.tokens == 0:
             return (torch.empty((0, weight.shape[1]), dtype=torch.bfloat16, device=weight.device),
-                    torch.zeros(weight.shape, dtype=torch.bfloat16, device=weight.device), None, None, None)
+                    torch.zeros(weight.shape, dtype=torch.bfloat16, device=weight.device), None, None, None, None)
         grad = plain_grad(grad_loss, "MegaCrossEntropy's backward").resolve_neg().contiguous()
-        grad_hidden, grad_weight = kernels.vocab_loss_grad(grad, state, weight, ctx.tokens, reduction=ctx.reduction,
+        grad_hidden, grad_weight = kernels.vocab_loss_grad(grad, state, weight, ctx.tokens, reduction=ctx.reduction, keep=ctx.keep,
                                                            need_hidden=ctx.needs_input_grad[0], need_weight=ctx.needs_input_grad[1])
-        return grad_hidden, grad_weight, None, None, None
+        return grad_hidden, grad_weight, None, None, None, None
 
 
 def mega_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
-                       reduction: str = "mean") -> torch.Tensor:
-    """Cross entropy of ``hidden @ weight.T`` against ``targets``, FP32, without holding the logits.
+                       reduction: str = "mean", recompute: bool = False) -> torch.Tensor:
+    """Cross entropy of ``hidden @ weight.T`` against ``targets``, FP32, without logits in full.
 
     ``hidden`` BF16 [..., H] with any strides, ``weight`` BF16 [V, H] with H a multiple of 8, ``targets`` INT32 or INT64 [...].
     ``reduction`` "none" gives a loss per token (0 where the target is ``ignore_index``), "sum" and "mean" run over the other
     tokens; the mean over none of them is NaN, as in torch. Ignored tokens are not read: whatever their hidden states hold,
     their gradient is zero and they add nothing to the weight's. A target outside [0, V) that is not ``ignore_index`` is not
     noticed on the host: its loss is NaN, and so are the gradients it enters. Differentiable once in ``hidden`` and ``weight``;
-    the gradients are BF16. The backward pass takes scratch of up to 512 MiB for probabilities (4096 words of them where that is
+    the gradients are BF16. For the backward pass the forward keeps logits as 16-bit distances from their row's largest, of as many
+    words as fit 4 GiB (none up to 128 tokens), and the others are computed again; with ``recompute`` all of them are and nothing of
+    tokens x vocab is held. The backward pass takes scratch of up to 512 MiB for probabilities (4096 words of them where that is
     more), 8 bytes per element of ``hidden`` and 8 bytes per word.
     """
     _validate(hidden, weight, targets, ignore_index, reduction)
+    if type(recompute) is not bool:
+        raise TypeError(f"recompute must be a bool, got {recompute!r}.")
     rows = as_rows(hidden, weight.shape[1])
     flat = targets if targets.ndim == 1 and targets.is_contiguous() else targets.reshape(-1).contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        loss = _CrossEntropyFunction.apply(rows, weight, flat, ignore_index, reduction)
+        loss = _CrossEntropyFunction.apply(rows, weight, flat, ignore_index, reduction, not recompute)
     else:
         loss = _forward(rows, _weight_rows(weight), flat, ignore_index, reduction)[0]
     return loss.view(targets.shape) if reduction == "none" and targets.ndim != 1 else loss
@@ -124,7 +128,7 @@ class MegaCrossEntropy(torch.nn.Module):
     """Own the head's weight [vocab, hidden] and give the loss of hidden states against targets."""
 
     def __init__(self, hidden_size: int, vocab_size: int, *, ignore_index: int = -100, reduction: str = "mean",
-                 initializer_range: float = 0.02, device: Any | None = None) -> None:
+                 recompute: bool = False, initializer_range: float = 0.02, device: Any | None = None) -> None:
         super().__init__()
         for name, value in (("hidden_size", hidden_size), ("vocab_size", vocab_size)):
             if not isinstance(value, int) or isinstance(value, bool) or value <= 0:
@@ -133,10 +137,12 @@ class MegaCrossEntropy(torch.nn.Module):
             raise ValueError(f"hidden_size must be a multiple of 8, got {hidden_size}.")
         if reduction not in _lib.HMC_REDUCE:
             raise ValueError(f"reduction must be one of {tuple(_lib.HMC_REDUCE)}, got {reduction!r}.")
+        if not isinstance(recompute, bool):
+            raise ValueError(f"recompute must be a bool, got {recompute!r}.")
         if not math.isfinite(initializer_range) or initializer_range < 0.0:
             raise ValueError("initializer_range must be finite and nonnegative")
         self.hidden_size, self.vocab_size = hidden_size, vocab_size
-        self.ignore_index, self.reduction = ignore_index, reduction
+        self.ignore_index, self.reduction, self.recompute = ignore_index, reduction, recompute
         self.weight = torch.nn.Parameter(torch.empty(vocab_size, hidden_size, device=device, dtype=torch.bfloat16))
         torch.nn.init.normal_(self.weight, mean=0.0, std=initializer_range)
 
@@ -153,4 +159,5 @@ class MegaCrossEntropy(torch.nn.Module):
         return result
 
     def forward(self, hidden: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-        return mega_cross_entropy(hidden, self.weight, targets, ignore_index=self.ignore_index, reduction=self.reduction)
+        return mega_cross_entropy(hidden, self.weight, targets, ignore_index=self.ignore_index, reduction=self.reduction,
+                                  recompute=self.recompute)

@@ -996,30 +996,31 @@ int hmc_row_norm_grad(const void* x, int64_t x_stride, const void* grad, int64_t
                       int dtype, const void* weight, int affine_dtype, int center, const float* mean, const float* rstd,
                       void* grad_x, void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Cross entropy of hidden states over a vocabulary: loss_i = log sum_j exp(x_i . w_j) - x_i . w_target(i), without ever
- * holding the logits. x [tokens, hidden] and weight [vocab, hidden] BF16 with rows x_stride and weight_stride elements
+/* Cross entropy of hidden states over a vocabulary: loss_i = log sum_j exp(x_i . w_j) - x_i . w_target(i), without
+ * logits in full. x [tokens, hidden] and weight [vocab, hidden] BF16 with rows x_stride and weight_stride elements
  * apart (weight rows on 16-byte boundaries, hidden a multiple of 8), targets INT32 or INT64. Tokens whose target is
  * ignore_index have no loss and are not read; a target outside [0, vocab), or a largest logit that is infinite, gives a
  * loss of NaN. reduction: loss [tokens] (0 for
  * ignored tokens), or loss [1], the sum or the mean over the tokens that count (NaN where none does). `state` (16-byte
- * aligned, of ..._state_bytes) keeps what the gradient needs, the counted rows of x among it. Logits and sums in FP32. */
+ * aligned, of ..._state_bytes) keeps what the gradient needs, the counted rows of x among it, and with
+ * `keep` the logits of the words that fit 4 GiB as 16-bit distances from the largest of 128 (none for up to 128 tokens).
+ * Logits and sums in FP32. */
 #define HMC_REDUCE_NONE 0
 #define HMC_REDUCE_MEAN 1
 #define HMC_REDUCE_SUM 2
-int64_t hmc_vocab_loss_state_bytes(int64_t tokens, int64_t hidden);
+int64_t hmc_vocab_loss_state_bytes(int64_t tokens, int64_t hidden, int64_t vocab, int keep);
 int64_t hmc_vocab_loss_workspace_bytes(int64_t tokens, int64_t vocab);
 int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* targets,
                    int targets_i64, int64_t tokens, int64_t hidden, int64_t vocab, int64_t ignore_index, int reduction,
-                   void* state, float* loss, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
-/* Gradients from the state of a forward with the same sizes, weight and reduction, and grad_loss (FP32 [tokens] or [1]):
+                   int keep, void* state, float* loss, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+/* Gradients from the state of a forward with the same sizes, weight, reduction and keep, and grad_loss (FP32 [tokens] or [1]):
  * grad_hidden [tokens, hidden] (zeros for ignored tokens) and grad_weight [vocab, hidden], BF16 without gaps; either may be
  * NULL. The vocabulary is walked in pieces whose BF16 probabilities take at most 512 MiB (or 4096 words, where those
- * take more); the logits are computed again. Results do
- * not depend on timing. */
+ * take more); logits that were not kept are computed again. Results do not depend on timing. */
 int64_t hmc_vocab_loss_grad_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab);
 int hmc_vocab_loss_grad(const void* state, const void* weight, int64_t weight_stride, int64_t tokens, int64_t hidden,
-                        int64_t vocab, int reduction, const float* grad_loss, void* grad_hidden, void* grad_weight,
-                        void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+                        int64_t vocab, int reduction, int keep, const float* grad_loss, void* grad_hidden,
+                        void* grad_weight, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

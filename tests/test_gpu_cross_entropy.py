@@ -3,8 +3,10 @@
 Tolerances. A logit is a sum of H exact products, added 16 at a time: H / 16 additions in FP32, each off by at most two
 steps (2^-22) of the sum of magnitudes S_ij = sum_k |x_ik w_jk|, so E_i = H / 16 * 2^-22 max_j S_ij. A loss is the difference of
 two such values and of FP32 logarithms: 2 E_i + 2^-20 (1 + |lse|). A probability carries exp's relative error, 2 E_i + 2^-20,
-and one rounding to BF16, 2^-8; the target's entry p - 1 stays in FP32. So grad_hidden is off by 2^-8 of itself (its own
-rounding) and g (sum_j p_j |w_j| (2^-8 + 2 E + 2^-19) + |w_target| (2 E + 2^-19)); grad_weight likewise over the tokens."""
+where its logit was kept half a step of 2^-10 of a power of two (log 2 * 2^-11; nothing is kept up to 128 tokens or with
+recompute), and one rounding to BF16, 2^-8; the target's entry p - 1 stays in FP32. So grad_hidden is off by 2^-8 of itself (its own
+rounding) and g (sum_j p_j |w_j| (2^-8 + kept + 2 E + 2^-19) + |w_target| (2 E + 2^-19)); grad_weight likewise over the tokens.
+A kept logit more than 64 powers of two below the largest of its row's 128 columns counts as none: off by 2^-64 of that p."""
 
 import math
 
@@ -14,6 +16,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 HALF = 2.0 ** -8  # half a step of BF16
+KEPT = math.log(2) * 2.0 ** -11  # half a step of a kept logit
 IGNORED = -100
 
 
@@ -27,16 +30,16 @@ def make(tokens, hidden, vocab, *, ignored=0.0, seed=0, scale=1.0):
     return x.cuda(), weight.cuda(), targets.cuda()
 
 
-def run(x, weight, targets, reduction="mean", grad=None, ignore_index=IGNORED):
+def run(x, weight, targets, reduction="mean", grad=None, ignore_index=IGNORED, **options):
     from hyper_multicore_b200 import mega_cross_entropy
 
     x, weight = x.detach().requires_grad_(True), weight.detach().requires_grad_(True)
-    loss = mega_cross_entropy(x, weight, targets, ignore_index=ignore_index, reduction=reduction)
+    loss = mega_cross_entropy(x, weight, targets, ignore_index=ignore_index, reduction=reduction, **options)
     grad = torch.ones_like(loss) if grad is None else grad
     return (loss.detach(), *torch.autograd.grad(loss, (x, weight), grad))
 
 
-def check(got, x, weight, targets, reduction="mean", grad=None, ignore_index=IGNORED):
+def check(got, x, weight, targets, reduction="mean", grad=None, ignore_index=IGNORED, recompute=False):
     loss, grad_x, grad_w = got
     x64, w64 = x.double(), weight.double()
     counted = targets != ignore_index
@@ -57,9 +60,10 @@ def check(got, x, weight, targets, reduction="mean", grad=None, ignore_index=IGN
     per_token = per_token * (1.0 if grad is None else grad.double()) * counted
     p = torch.exp(logits - lse.unsqueeze(1))
     rel = (2 * error + 2.0 ** -19).unsqueeze(1)
+    kept = 0.0 if recompute or x.shape[0] <= 128 else KEPT
     onehot = torch.zeros_like(p).scatter_(1, index, 1.0)
     d = (p - onehot) * per_token.unsqueeze(1)
-    slack = (p * (1 - onehot) * (HALF + rel) + onehot * rel) * per_token.abs().unsqueeze(1)
+    slack = (p * (1 - onehot) * (HALF + kept + rel) + onehot * rel + 2.0 ** -64 * (kept > 0)) * per_token.abs().unsqueeze(1)
     for name, out, exact, off in (("grad_hidden", grad_x, d @ w64, slack @ w64.abs()),
                                   ("grad_weight", grad_w, d.t() @ x64, slack.t() @ x64.abs())):
         assert out.dtype == torch.bfloat16
@@ -78,17 +82,58 @@ SIZES = [(1, 8, 1), (1, 64, 2), (2, 8, 255), (3, 1000, 256), (5, 72, 257), (33, 
 def test_loss_and_gradients_match_the_definition(tokens, hidden, vocab, reduction):
     x, weight, targets = make(tokens, hidden, vocab, ignored=0.2 if tokens > 4 else 0.0, seed=tokens + vocab)
     grad = torch.rand(tokens if reduction == "none" else (), device="cuda") + 0.5
-    check(run(x, weight, targets, reduction, grad), x, weight, targets, reduction, grad)
+    for recompute in (False, True):
+        check(run(x, weight, targets, reduction, grad, recompute=recompute), x, weight, targets, reduction, grad, recompute=recompute)
 
 
+@pytest.mark.parametrize("recompute", [False, True])
 @pytest.mark.parametrize("tokens,hidden,vocab", [(4096, 64, 70001), (40, 4096, 20000), (2500, 256, 3000)])
-def test_large_sizes_and_pieces_of_the_vocabulary(tokens, hidden, vocab):
+def test_large_sizes_and_pieces_of_the_vocabulary(tokens, hidden, vocab, recompute):
     """The first one's probabilities take two pieces; its weight's gradient has words of both."""
     x, weight, targets = make(tokens, hidden, vocab, ignored=0.1, seed=vocab)
-    got = run(x, weight, targets)
-    check(got, x, weight, targets)
-    again = run(x, weight, targets)
+    got = run(x, weight, targets, recompute=recompute)
+    check(got, x, weight, targets, recompute=recompute)
+    again = run(x, weight, targets, recompute=recompute)
     assert all(torch.equal(a, b) for a, b in zip(got, again)), "the same call twice gives other bits"
+
+
+def test_words_beyond_what_is_kept_are_computed_again():
+    """20000 x 120001 words take more than 4 GiB: the loss is the same, a gradient differs by two roundings of p at most."""
+    from hyper_multicore_b200 import kernels as K
+
+    x, weight, targets = make(20_000, 64, 120_001, ignored=0.1, seed=23)
+    held = K._size("hmc_vocab_loss_state_bytes", 20_000, 64, 120_001, True) - K._size("hmc_vocab_loss_state_bytes", 20_000, 64, 120_001, False)
+    assert 0 < held < 2 * 20_000 * 120_001
+    loss, grad_x, grad_w = run(x, weight, targets)
+    other, want_x, want_w = run(x, weight, targets, recompute=True)
+    assert torch.equal(loss, other)
+    # one rounding of each result, and p's of both: at most 2 (2 * 2^-8 + KEPT) of sums of magnitudes, on the whole of their norms
+    for got, want in ((grad_x, want_x), (grad_w, want_w)):
+        assert not torch.equal(got, want)
+        assert (got.double() - want.double()).norm() <= 2 * (2 * HALF + KEPT) * want.double().norm()
+    check_rows = slice(19_900, 20_000)
+    counted = targets[check_rows] != IGNORED
+    p = torch.softmax(x[check_rows].double() @ weight.double().t(), 1)
+    p.scatter_add_(1, torch.where(counted, targets[check_rows], 0).unsqueeze(1), torch.full((100, 1), -1.0, dtype=torch.float64, device="cuda"))
+    exact = p * counted.unsqueeze(1) / (targets != IGNORED).sum() @ weight.double()
+    assert (grad_x[check_rows].double() - exact).norm() <= HALF * exact.norm()
+
+
+def test_kept_logits_far_below_the_largest():
+    """Weights that put most words 100 powers of two below the rest of their 128, among them minus infinity."""
+    x, weight, targets = make(300, 64, 1000, seed=24)
+    x[:, 0] = 1.0
+    weight[::3, 0] = -70.0
+    weight[7] = 0.0
+    weight[7, 0] = -float("inf")
+    targets[targets % 3 == 0] += 1
+    targets[targets == 7] = 8
+    loss, grad_x, grad_w = run(x, weight, targets, "none")
+    other, want_x, want_w = run(x, weight, targets, "none", recompute=True)
+    assert torch.equal(loss, other) and loss.isfinite().all()
+    assert torch.equal(grad_x.isnan(), want_x.isnan()) and torch.equal(grad_w.isnan(), want_w.isnan())
+    kept = grad_w[1::3]
+    assert (kept.double() - want_w[1::3].double()).norm() <= 2 * (2 * HALF + KEPT) * kept.double().norm()
 
 
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
@@ -272,7 +317,7 @@ def test_rows_of_the_output_are_written_and_nothing_else():
     gx, gw = (torch.full((n + 64, 72), 3.0, dtype=torch.bfloat16, device="cuda") for n in (70, 300))
     grad = torch.ones((), device="cuda")
     status = _lib.new_status(x.device)
-    _lib.launch("hmc_vocab_loss_grad", x.device, state.data_ptr(), weight.data_ptr(), 72, 70, 72, 300, 1, grad.data_ptr(),
+    _lib.launch("hmc_vocab_loss_grad", x.device, state.data_ptr(), weight.data_ptr(), 72, 70, 72, 300, 1, 0, grad.data_ptr(),
                 gx.data_ptr(), gw.data_ptr(), space.data_ptr(), need, status.data_ptr())
     _lib.raise_on_status(status, "gradient")
     _, want_x, want_w = run(x, weight, targets)
