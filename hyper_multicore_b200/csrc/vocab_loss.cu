@@ -1328,8 +1328,8 @@ long long piece_words(long long tokens, long long vocab) {
 
 // The words whose codes a forward leaves: as many pieces as KEEP_BYTES hold (a fortieth of the GPU's memory), in whole tiles.
 // Kept against computed again: 4096 x 1024 x 32000 743 and 878 us, 16384 x 2048 x 131072 (all of it) 24.0 and 28.7 ms, twice the
-// tokens (half of it) 53.9 and 61.8, 131072 x 512 x 65536 (a quarter of it) 44.9 and 45.9. The
-// few-token kernel keeps none: with so few rows the logits cost one pass over the weight.
+// tokens (half of it) 53.9 and 61.8, 131072 x 512 x 65536 (a quarter of it) 44.9 and 45.9. The few-token kernel
+// keeps none: with so few rows the logits cost one pass over the weight.
 constexpr long long KEEP_BYTES = 4ll << 30;
 long long kept_words(long long tokens, long long vocab) {
   if (tokens <= FEW_TOKENS) return 0;

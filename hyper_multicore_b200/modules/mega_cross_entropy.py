@@ -112,9 +112,9 @@ def mega_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torc
     tokens x vocab is held. The backward pass takes scratch of up to 512 MiB for probabilities (4096 words of them where that is
     more), 8 bytes per element of ``hidden`` and 8 bytes per word.
     """
+    if recompute is not False and recompute is not True:
+        raise ValueError(f"recompute must be a bool, got {recompute!r}.")
     _validate(hidden, weight, targets, ignore_index, reduction)
-    if type(recompute) is not bool:
-        raise TypeError(f"recompute must be a bool, got {recompute!r}.")
     rows = as_rows(hidden, weight.shape[1])
     flat = targets if targets.ndim == 1 and targets.is_contiguous() else targets.reshape(-1).contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):

@@ -39,6 +39,8 @@ def _loss(x=(4, 16), w=(10, 16), t=(4,), x_dtype=BF16, w_dtype=BF16, t_dtype=tor
 @pytest.mark.parametrize("error,match,call", [
     (TypeError, "targets must be a Tensor", lambda: mega_cross_entropy(torch.zeros(1, 8), torch.zeros(2, 8), 1)),
     (ValueError, "reduction", lambda: _loss(reduction="average")),
+    (ValueError, "recompute", lambda: _loss(recompute=1)),
+    (ValueError, "recompute", lambda: MegaCrossEntropy(16, 10, recompute=None)),
     (ValueError, "ignore_index", lambda: _loss(ignore_index=1.5)),
     (ValueError, "ignore_index", lambda: _loss(ignore_index=1 << 63)),
     (ValueError, "multiple of 8", lambda: _loss(x=(4, 12), w=(10, 12))),
@@ -92,7 +94,7 @@ def test_c_entries_refuse_without_touching_a_device():
     refused(grad(mean=None), b"null")
     refused(grad(center=0, gb=at), b"no bias")
     loss = lambda **c: lib.hmc_vocab_loss(*{**dict(  # noqa: E731
-        x=at, xs=16, w=at, ws=16, t=at, wide=1, tokens=4, hidden=16, vocab=10, ignored=-100, red=1, state=at, loss=at, space=at,
+        x=at, xs=16, w=at, ws=16, t=at, wide=1, tokens=4, hidden=16, vocab=10, ignored=-100, red=1, keep=1, state=at, loss=at, space=at,
         sb=1 << 40, status=None, stream=None), **c}.values())
     refused(loss(tokens=0), b"tokens")
     refused(loss(vocab=0), b"vocab")
@@ -105,7 +107,7 @@ def test_c_entries_refuse_without_touching_a_device():
     refused(loss(sb=8), b"workspace")
     refused(loss(state=at + 8), b"boundaries")
     back = lambda **c: lib.hmc_vocab_loss_grad(*{**dict(  # noqa: E731
-        state=at, w=at, ws=16, tokens=4, hidden=16, vocab=10, red=1, g=at, gh=at, gw=at, space=at, sb=1 << 40, status=None,
+        state=at, w=at, ws=16, tokens=4, hidden=16, vocab=10, red=1, keep=1, g=at, gh=at, gw=at, space=at, sb=1 << 40, status=None,
         stream=None), **c}.values())
     refused(back(g=None), b"null")
     refused(back(gh=at + 2), b"aligned")
@@ -119,9 +121,14 @@ def test_workspaces_hold_every_smaller_call():
         sizes = [lib.hmc_row_norm_grad_workspace_bytes(rows, hidden) for rows in [*range(1, 700), 4096, 16384]]
         assert sizes == sorted(sizes)
     for vocab in (1, 50257, 131072):
-        for size in (lambda t, v=vocab: lib.hmc_vocab_loss_workspace_bytes(t, v), lambda t: lib.hmc_vocab_loss_state_bytes(t, 64)):
+        for size in (lambda t, v=vocab: lib.hmc_vocab_loss_workspace_bytes(t, v), lambda t, v=vocab: lib.hmc_vocab_loss_state_bytes(t, 64, v, 0)):
             sizes = [size(t) for t in (1, 2, 255, 256, 257, 4096, 8192, 65536)]
             assert sizes == sorted(sizes)
+        # kept logits: none up to 128 tokens, 4 GiB and a 64th of it at the most
+        for tokens in (1, 128, 129, 4096, 20_000, 65536, 1 << 20):
+            held = lib.hmc_vocab_loss_state_bytes(tokens, 64, vocab, 1) - lib.hmc_vocab_loss_state_bytes(tokens, 64, vocab, 0)
+            assert (held == 0) if tokens <= 128 else (0 <= held <= (4 << 30) * 65 // 64 + 256)
+            assert tokens > 4096 or tokens <= 128 or held > 2 * tokens * vocab
     # probabilities of a piece: half a GiB, and no fewer than 4096 words
     assert lib.hmc_vocab_loss_grad_workspace_bytes(8192, 8, 1 << 20) < 600 << 20
 
