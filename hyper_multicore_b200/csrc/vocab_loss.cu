@@ -1092,7 +1092,7 @@ __device__ __forceinline__ float power_of(uint32_t pair, uint32_t half, float ab
 
 // p of a piece of the vocabulary out of its codes, times the row's gradient: what PROBS computes from the logits. A warp per row
 // and 1024 words, eight rows per block; rows behind the last one that the products read with it are zero. Bound by memory:
-// 3687 x 65536 165 us (0.97 GB, 5.9 TB/s) where the product takes 1400; with a conversion and exp2f per code 178.
+// 3687 x 65536 175 us (0.97 GB, 5.5 TB/s) where the product takes 1400; 2101 x 50257 77 us, 80 with a conversion and exp2f per code.
 constexpr int SPREAD_WORDS = 1024;
 __global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict__ codes, long long codes_pitch,
                                                      const float* __restrict__ tops, long long tops_pitch, int first_word, int width,

@@ -441,6 +441,19 @@ def test_end_of_a_training_step():
     assert math.isfinite(loss.item()) and grad_leaf.abs().max() > 0
 
 
+def test_module_computes_logits_again_where_asked_to():
+    from hyper_multicore_b200 import MegaCrossEntropy
+
+    x, weight, targets = make(300, 64, 500, seed=25)
+    head = MegaCrossEntropy(64, 500, recompute=True, device="cuda")
+    head.weight.data.copy_(weight)
+    hidden = x.detach().requires_grad_(True)
+    head(hidden, targets).backward()
+    _, want_x, want_w = run(x, weight, targets, recompute=True)
+    _, kept_x, _ = run(x, weight, targets)
+    assert torch.equal(hidden.grad, want_x) and torch.equal(head.weight.grad, want_w) and not torch.equal(want_x, kept_x)
+
+
 def test_module_shares_the_weight_of_an_existing_head():
     from hyper_multicore_b200 import MegaCrossEntropy
 
