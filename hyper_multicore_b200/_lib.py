@@ -473,8 +473,9 @@ def launch(name: str, device: torch.device, *args) -> None:
     function = _FUNCTIONS.get(name)
     if function is None:
         function = _FUNCTIONS[name] = getattr(load(), name)
-    if device.index is None or device.index == torch._C._cuda_getDevice():  # pylint: disable=protected-access
-        code = function(*args, stream_ptr(device))
+    index, current = device.index, torch._C._cuda_getDevice()  # pylint: disable=protected-access
+    if index is None or index == current:
+        code = function(*args, torch._C._cuda_getCurrentRawStream(current))  # pylint: disable=protected-access
     else:
         with torch.cuda.device(device):
             code = function(*args, stream_ptr(device))

@@ -19,16 +19,18 @@ def _fits(x, weight, bias, eps) -> bool:
     """All of ``_validate`` in one expression, which builds no message; that one then says what is wrong."""
     if type(x) is not torch.Tensor or not x.is_cuda or x.ndim == 0 or type(eps) is not float or not 0.0 <= eps < math.inf:
         return False
-    dtype, hidden = x.dtype, x.shape[-1]
-    if not (1 <= hidden <= _lib.HMC_NORM_MAX_HIDDEN and x.numel() <= hidden * _lib.HMC_NORM_MAX_ROWS and dtype in _lib.HMC_DTYPE):
+    dtype, index = x.dtype, x.get_device()
+    shape = x.shape[-1:]
+    if not (1 <= shape[0] <= _lib.HMC_NORM_MAX_HIDDEN and x.numel() <= shape[0] * _lib.HMC_NORM_MAX_ROWS and dtype in _lib.HMC_DTYPE):
         return False
-    if weight is not None and not (isinstance(weight, torch.Tensor) and weight.ndim == 1 and weight.shape[0] == hidden
-                                   and weight.dtype in (dtype, torch.float32) and weight.device == x.device):
-        return False
-    if bias is None:
-        return True
-    return (isinstance(bias, torch.Tensor) and bias.ndim == 1 and bias.shape[0] == hidden and bias.device == x.device
-            and bias.dtype in ((dtype, torch.float32) if weight is None else (weight.dtype,)))
+    affine = (dtype, torch.float32)
+    if weight is not None:
+        if not (isinstance(weight, torch.Tensor) and weight.shape == shape and weight.is_cuda and weight.get_device() == index
+                and weight.dtype in affine):
+            return False
+        affine = (weight.dtype,)
+    return bias is None or (isinstance(bias, torch.Tensor) and bias.shape == shape and bias.is_cuda and bias.get_device() == index
+                            and bias.dtype in affine)
 
 
 def _validate(x, weight, bias, eps) -> None:
@@ -68,20 +70,20 @@ class _RowNormFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, center, eps):  # pylint: disable=arguments-differ
         y, rows, weight, bias, stats = _forward(x, weight, bias, center, eps, True)
         ctx.save_for_backward(rows, weight, stats)
-        ctx.center, ctx.shape = center, x.shape
-        ctx.affine_dtype = x.dtype if weight is None and bias is None else bias.dtype if weight is None else weight.dtype
+        ctx.of = center, x.shape, None if weight is not None else x.dtype if bias is None else bias.dtype
         return y
 
     @staticmethod
     @first_order
     def backward(ctx, grad):  # pylint: disable=arguments-differ
         rows, weight, stats = ctx.saved_tensors
-        need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
-        grad = as_rows(plain_grad(grad, "a row norm's backward"), rows.shape[1])
-        grad_x, grad_weight, grad_bias = kernels.row_norm_grad(grad, rows, weight, stats, ctx.center, ctx.affine_dtype, need_x,
-                                                               need_weight, need_bias)
-        if need_x and len(ctx.shape) != 2:
-            grad_x = grad_x.view(ctx.shape)
+        center, shape, affine_dtype = ctx.of
+        need_x, need_weight, need_bias, _, _ = ctx.needs_input_grad
+        grad = as_rows(plain_grad(grad, "a row norm's backward"), shape[-1])
+        grad_x, grad_weight, grad_bias = kernels.row_norm_grad(grad, rows, weight, stats, center, affine_dtype, need_x, need_weight,
+                                                               need_bias, rows.device)
+        if need_x and len(shape) != 2:
+            grad_x = grad_x.view(shape)
         return grad_x, grad_weight, grad_bias, None, None
 
 
