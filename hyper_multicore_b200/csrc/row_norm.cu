@@ -677,7 +677,7 @@ stream_longest_grad_kernel(const T* __restrict__ x, long long x_stride, const T*
 // windows: the 16-byte pieces that hold a row, copied by whichever thread, so that a barrier stands before their use. The
 // first piece may begin with the end of the row before (the first row of all begins on its boundary), the last one ends
 // with the row. VEC = 1 or 2 values per access behind that, which bounds these kernels: 16384 rows of 5003 BF16 take 183 us
-// forward and 271 for the gradient (50 and 75 us of traffic), 4096 rows of 7161 FP32 55 and 90 us (36 and 54). Straight from
+// forward and 271 for the gradient (50 and 75 us of traffic), 4096 rows of 7161 FP32 57 and 95 us (36 and 54). Straight from
 // memory, with too little under way, the BF16 rows took 237 and 497 us.
 constexpr int WINDOW_WARPS = 16;
 constexpr int WINDOW_MOST = 8192;  // values of a row
@@ -1202,7 +1202,8 @@ int stream_grad(NormCall& c) {
   return launch_longest_grad<T, W, 2 * NV, LONGEST<T>, CENTER>(c);
 }
 
-// Windows of a row in a ring of `each` of them per stage.
+// Windows of a row in a ring of `each` of them per stage, of the longest row that the block's threads hold: the shared memory and
+// with it the blocks per SM, from which the gradient's order of summation follows, depend on the block size alone.
 struct WindowRing {
   int window, stages, bytes;
   WindowRing(long long row_bytes, int each) {
@@ -1216,7 +1217,7 @@ struct WindowRing {
 template <typename T, typename W, int VEC, int NV, bool CENTER>
 int launch_window(const NormCall& c) {
   const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
-  const WindowRing ring(c.hidden * sizeof(T), 1);
+  const WindowRing ring(threads * NV * VEC * sizeof(T), 1);
   static Residency known{};
   auto kernel = window_norm_kernel<T, W, VEC, NV, CENTER>;
   int blocks = 0;
@@ -1252,7 +1253,7 @@ int forward(const NormCall& c) {
 template <typename T, typename W, int VEC, int NV, bool CENTER>
 int launch_window_grad(NormCall& c) {
   const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
-  const WindowRing ring(c.hidden * sizeof(T), 2);
+  const WindowRing ring(threads * NV * VEC * sizeof(T), 2);
   static Residency known{};
   auto kernel = window_norm_grad_kernel<T, W, VEC, NV, CENTER>;
   int blocks = 0;

@@ -296,6 +296,32 @@ assert all(torch.equal(a, b) for a, b in zip(got, step()))
     subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
 
 
+def test_order_of_sums_does_not_depend_on_earlier_calls():
+    """Two row lengths that share a block size: the second one's bits are those it has in a process of its own."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import sys, hashlib
+import torch
+from hyper_multicore_b200 import mega_layer_norm
+for hidden in map(int, sys.argv[1:]):
+    g = torch.Generator().manual_seed(hidden)
+    x, dy = (torch.randn(2000, hidden, generator=g).cuda() for _ in range(2))
+    weight, bias = (torch.randn(hidden, generator=g).cuda().requires_grad_(True) for _ in range(2))
+    grads = torch.autograd.grad(mega_layer_norm(x, weight, bias), (weight, bias), dy)
+print(hashlib.sha256(b"".join(q.cpu().numpy().tobytes() for q in grads)).hexdigest())
+"""
+    root = Path(__file__).resolve().parents[1]
+
+    def digest(*sizes):
+        return subprocess.run([sys.executable, "-c", code, *map(str, sizes)], check=True, cwd=root, timeout=300,
+                              capture_output=True, text=True).stdout
+
+    assert digest(1537, 1791) == digest(1791)
+
+
 def test_the_most_rows_there_may_be():
     """Blocks step through rows in 32 bits: the last step must not run over."""
     from hyper_multicore_b200 import _lib, mega_rms_norm
