@@ -382,11 +382,13 @@ stream_norm_kernel(const T* __restrict__ x, long long x_stride, long long rows, 
 
 // The gradient over the same ring, x and dy per stage. Threads own columns: the parameters' gradients stay in registers over
 // all rows of a block, so that x and dy are read once. Behind the reduction a row is widened again from the ring, since its g
-// and u kept in registers would leave room for half the warps. Two 16-bit rows go through a turn and share its barrier and its
-// loads of the weight (16384 rows, layer norm, BF16, against one row per turn: 1024 wide 20.6 us against 28, 2048 36 against
-// 46, 4096 66 against 87, 7168 126 against 140; the traffic alone takes 15.4, 31, 62 and 108). Three stages of two FP32 rows
-// do not fit, one row per turn is near the copy rate (8192 x 4096 67 us of 62, 8192 x 7168 116 of 108).
+// and u kept in registers would leave room for half the warps. Three 16-bit rows go through a turn and share its barrier and its
+// loads of the weight, two turns fit the ring (16384 rows, layer norm, BF16, against two rows in three stages and one row in
+// three: 1024 wide 19.7, 20.6 and 28 us, 2048 34, 36 and 46, 4096 66, 66 and 87, 7168 120, 127 and 140; the traffic alone takes
+// 15.4, 31, 62 and 108). Two turns of two FP32 rows do not fit; one row per turn is near the copy rate (8192 x 4096 67 us of 62,
+// 8192 x 7168 116 of 108).
 constexpr int WIDE_THREADS = 448;  // rows of 4097 to 7168 values
+__host__ __device__ constexpr int wide_stages(int rows) { return rows > 1 ? 2 : GRAD_STAGES; }
 template <typename T, typename W, int NV, int ROWS, int PITCH, bool CENTER>
 __global__ void __launch_bounds__(PITCH, STREAM_THREADS / PITCH)
 stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ grad, long long grad_stride,
@@ -395,7 +397,7 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
                         float* __restrict__ partial_bias) {
   chain_wait();
   extern __shared__ uint4 ring_raw[];
-  constexpr int stages = GRAD_STAGES, SUMS = (CENTER ? 2 : 1) * ROWS;
+  constexpr int stages = wide_stages(ROWS), SUMS = (CENTER ? 2 : 1) * ROWS;
   __shared__ float slots[2][SUMS * STREAM_WARPS];
   constexpr int PAIRS = Quad<T>::PAIRS, VEC = 2 * PAIRS;
   constexpr int WIDTH = NV * PITCH;  // known at compile time: offsets in the ring cost no arithmetic
@@ -1172,7 +1174,7 @@ template <typename T, typename W, int NV, int ROWS, int PITCH, bool CENTER>
 int launch_wide_grad(NormCall& c) {
   constexpr int VEC = 16 / sizeof(T);
   const int threads = round_up((c.hidden / VEC + NV - 1) / NV, 32);
-  const int bytes = NV * PITCH * (GRAD_STAGES * ROWS * 2 * 16 + VEC * 4);
+  const int bytes = NV * PITCH * (wide_stages(ROWS) * ROWS * 2 * 16 + VEC * 4);
   static Residency known{};
   auto kernel = stream_wide_grad_kernel<T, W, NV, ROWS, PITCH, CENTER>;
   int blocks = 0;
@@ -1193,7 +1195,7 @@ constexpr int LONGEST = sizeof(T) == 4 ? 288 : STREAM_THREADS;
 template <typename T, typename W, bool CENTER>
 int stream_grad(NormCall& c) {
   constexpr int NV = sizeof(T) == 4 ? 4 : 2;    // 16 values per thread
-  constexpr int ROWS = sizeof(T) == 4 ? 1 : 2;  // three stages of two FP32 rows do not fit shared memory
+  constexpr int ROWS = sizeof(T) == 4 ? 1 : 3;  // of a turn
   if (c.hidden <= 16 * 64) return launch_wide_grad<T, W, NV, ROWS, 64, CENTER>(c);
   if (c.hidden <= 16 * 128) return launch_wide_grad<T, W, NV, ROWS, 128, CENTER>(c);
   if (c.hidden <= 16 * 256) return launch_wide_grad<T, W, NV, ROWS, 256, CENTER>(c);
