@@ -11,8 +11,14 @@
 // from the same GEMM again, and two GEMMs that take the piece to the two gradients. p without the target's entry only: that
 // one is p - 1, which cancels for a token the model is sure of and carries the largest weight for one it is not, so it stays
 // in FP32 (expm1 of -loss) and meets the products in FP32: for dx as the row w_t(i) in the epilogue, for dw as a sum over the
-// tokens of a word made beforehand. The rounding of the other entries to BF16 (2^-8 of the value at most) averages over a sum
-// of many.
+// tokens of a word made beforehand. The other entries are off by 2^-8 of their value at most (BF16) and, where their logits
+// were kept, by 3.4e-4 before that. A row of dx is made of differences, p_ij (w_j - w_t(i)): what the words' rows have in common
+// cancels only if the coefficients of a row add up to nothing. So the rounded entries of a row are added up in FP32, the
+// target's row enters with minus that sum, and the whole is scaled by what the sum should be (1 - p_t(i)) over what it is. An error
+// that all entries share, or that of one word which holds nearly all of the rest, then cancels too; left is
+// 2 * 2^-8 sum_j p_ij |w_j - w_c| at most, c the likeliest wrong word. (Rows of 256 over 1000 words with a common component of ten times
+// their own size: up to 1.8 % of a row's norm without this, its own rounding of 0.2 % with it.) A row of dw has no such sum: it is off by 2^-8 sum_i g_i p_ij |x_i| at
+// most, all of it where one token holds nearly all of a word.
 // A training step of 8192 x 4096 x 131072 takes 23.2 ms with all its logits kept (2 GiB of 16-bit codes) and 28.4 ms with none,
 // 512 x 1024 x 32000 168 against 194 us. Gradients taken in the forward pass would hold the weight's gradient in FP32 until the
 // backward one and only fit a loss that is reduced.
@@ -72,6 +78,8 @@ struct Params {
   int kept;            // STATS: the words whose codes are stored, in whole tiles
   float* tops;         // STATS: [kept / HALF][pitch] what the codes count from
   int first_word;       // PROBS, GRAD_*: first word of the piece
+  float* row_sums;      // PROBS: [2 * n_tiles][pitch] sums of what is stored
+  const float* others;  // GRAD_HIDDEN: [rows] sum of a packed row's stored entries over all pieces
   const int* row_of;    // GRAD_HIDDEN: token of a packed row
   float* sums;          // GRAD_HIDDEN: [rows, n] FP32 sums over pieces, or NULL
   int add, last;        // GRAD_HIDDEN: sums holds earlier pieces; this piece is the last
@@ -237,9 +245,18 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, float (&v)[64]) {
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(lo[j]), v[32 + j] = __uint_as_float(hi[j]);
 }
 
-// p of one row's 128 columns times the row's gradient, the target's entry left out.
+// Eight values as BF16; their sum as rounded.
+__device__ __forceinline__ uint4 pack_8(const float* v, float2& sum) {
+  const uint4 q = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  sum = add2(sum, add2(add2(unpack_bf16x2(q.x), unpack_bf16x2(q.y)), add2(unpack_bf16x2(q.z), unpack_bf16x2(q.w))));
+  return q;
+}
+
+// p of one row's 128 columns times the row's gradient, the target's entry left out, and the sum of what is stored.
 __device__ __forceinline__ void epilogue_probs(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
-                                               unsigned& issued, int first_row, int row, bool row_ok, int col, int lane) {
+                                               unsigned& issued, int first_row, int row, bool row_ok, int col, int half_tile,
+                                               int lane) {
+  float2 sum = both(0.0f);
   const float lse = row_ok ? p.lse[row] : 0.0f;
   const float weight = row_ok ? p.weights[row] : 0.0f;
   const int label = row_ok ? p.labels[row] - p.first_word - col : -1;
@@ -256,16 +273,34 @@ __device__ __forceinline__ void epilogue_probs(const Params& p, const CUtensorMa
       for (int j = 0; j < 64; ++j)
         if (j == own) v[j] = 0.0f;
     }
+    if (col + c + 64 > p.n) {  // columns behind the piece are neither stored nor summed
+#pragma unroll
+      for (int j = 0; j < 64; ++j)
+        if (col + c + j >= p.n) v[j] = 0.0f;
+    }
     __syncwarp();
 #pragma unroll
-    for (int h = 0; h < 64; h += 32)
-      if (col + c + h < p.n) store_box(tm, stage, issued, v + h, col + c + h, first_row, lane);
+    for (int h = 0; h < 64; h += 32) {
+      if (col + c + h >= p.n) break;
+      uint4 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = pack_8(v + h + 8 * i, sum);
+      store_box(tm, stage, issued, q, col + c + h, first_row, lane);
+    }
   }
+  if (row_ok) p.row_sums[half_tile * p.pitch + row] = sum.x + sum.y;
+}
+
+// With the last piece: what a row of dx takes the target's row times, and what the whole is scaled by.
+__device__ __forceinline__ float2 row_coefficients(const Params& p, int row) {
+  const float coef = p.coef[row], others = p.others[row], scale = *p.scale;
+  // nothing stored (a gradient of zero, no other word, a certain token): the true coefficient, which is as small
+  return others != 0.0f ? make_float2(-others, scale * (-coef / others)) : make_float2(coef, scale);
 }
 
 // Eight columns of a row of dx from this piece's sums: added to those of earlier pieces, and with the last piece the target's
 // row on top, scaled, rounded and stored at the token's place.
-__device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int col, float* v, float scale) {
+__device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int col, float* v, float2 by) {
   float* sums = p.sums + static_cast<long long>(row) * p.n + col;
   if (p.add) {
     const float4 a = *reinterpret_cast<const float4*>(sums), b = *reinterpret_cast<const float4*>(sums + 4);
@@ -278,23 +313,23 @@ __device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int
   }
   const int label = p.labels[row];
   if (label >= 0) {
-    const float coef = p.coef[row];
     const uint4 w = ld_16(p.head + label * p.head_stride + col);
     const uint32_t parts[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 f = unpack_bf16x2(parts[e]);
-      v[2 * e] += coef * f.x;
-      v[2 * e + 1] += coef * f.y;
+      v[2 * e] += by.x * f.x;
+      v[2 * e + 1] += by.x * f.y;
     }
   }
+  const float scale = by.y;
   st_16(p.out + static_cast<long long>(p.row_of[row]) * p.n + col,
         make_uint4(pack_bf16x2(v[0] * scale, v[1] * scale), pack_bf16x2(v[2] * scale, v[3] * scale),
                    pack_bf16x2(v[4] * scale, v[5] * scale), pack_bf16x2(v[6] * scale, v[7] * scale)));
 }
 
 __device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t taddr, int row, bool row_ok, int col) {
-  const float scale = *p.scale;
+  const float2 by = row_ok && p.last ? row_coefficients(p, row) : both(0.0f);
 #pragma unroll 1
   for (int c = 0; c < HALF; c += 64) {
     if (col + c >= p.n) break;
@@ -303,7 +338,7 @@ __device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t t
     if (row_ok) {
 #pragma unroll
       for (int j = 0; j < 64; j += 8)
-        if (col + c + j < p.n) finish_grad_hidden(p, row, col + c + j, v + j, scale);
+        if (col + c + j < p.n) finish_grad_hidden(p, row, col + c + j, v + j, by);
     }
   }
 }
@@ -343,7 +378,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(Params p, int pairs) {
     v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
     src += TILE * TILE;
   }
-  finish_grad_hidden(p, row, col, v, *p.scale);
+  finish_grad_hidden(p, row, col, v, p.last ? row_coefficients(p, row) : both(0.0f));
 }
 
 __device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
@@ -594,7 +629,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       }
       if (!filled()) break;
       const uint32_t taddr = lane_base + static_cast<uint32_t>(acc * TILE);
-      if (KIND == PROBS) epilogue_probs(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane);
+      if (KIND == PROBS) epilogue_probs(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, 2 * u.ni + half, lane);
       if (KIND == GRAD_HIDDEN) {
         if (u.part >= 0) epilogue_part(p, taddr, u.part, in_tile + lane, row_ok, half);
         else epilogue_grad_hidden(p, taddr, row, row_ok, col);
@@ -1091,14 +1126,16 @@ __device__ __forceinline__ float power_of(uint32_t pair, uint32_t half, float ab
 }
 
 // p of a piece of the vocabulary out of its codes, times the row's gradient: what PROBS computes from the logits. A warp per row
-// and 1024 words, eight rows per block; rows behind the last one that the products read with it are zero. Bound by memory:
+// and 1024 words, eight rows per block, and the sum of what it stores; rows behind the last one that the products read with it are
+// zero. Bound by memory:
 // 3687 x 65536 175 us (0.97 GB, 5.5 TB/s) where the product takes 1400; 2101 x 50257 77 us, 80 with a conversion and exp2f per code.
 constexpr int SPREAD_WORDS = 1024;
 __global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict__ codes, long long codes_pitch,
                                                      const float* __restrict__ tops, long long tops_pitch, int first_word, int width,
                                                      const int* __restrict__ count, const float* __restrict__ lse,
                                                      const float* __restrict__ weights, long long tokens,
-                                                     __nv_bfloat16* __restrict__ probs, long long probs_pitch) {
+                                                     __nv_bfloat16* __restrict__ probs, long long probs_pitch,
+                                                     float* __restrict__ row_sums) {
   chain_wait();
   chain_next();
   const int rows = *count;
@@ -1117,6 +1154,7 @@ __global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict_
     q[i] = ld_16(src + 256 * i);
     from[i] = tops[(first_word + col + 256 * i) / HALF * tops_pitch + row];
   }
+  float2 sum = both(0.0f);
 #pragma unroll
   for (int i = 0; i < SPREAD_WORDS / 256; ++i) {
     if (col + 256 * i >= width) break;
@@ -1124,12 +1162,40 @@ __global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict_
     if (row_ok) {
       const float above = (from[i] - norm) * LOG2_E;
       auto two = [&](uint32_t pair) {
-        return pack_bf16x2(power_of(pair, 0x7610, above) * weight, power_of(pair, 0x7632, above) * weight);
+        const uint32_t word = pack_bf16x2(power_of(pair, 0x7610, above) * weight, power_of(pair, 0x7632, above) * weight);
+        sum = add2(sum, unpack_bf16x2(word));
+        return word;
       };
       out = make_uint4(two(q[i].x), two(q[i].y), two(q[i].z), two(q[i].w));
     }
     st_16(dst + 256 * i, out);
   }
+  const float all = warp_sum(sum.x + sum.y);
+  if (row_ok && (threadIdx.x & 31) == 0) row_sums[blockIdx.y * tops_pitch + row] = all;
+}
+
+// Sums of a packed row's stored entries: this piece's parts in their order, 32 slices of them in parallel, on top of those of
+// earlier pieces. Bound by latency.
+__global__ void __launch_bounds__(32 * JOIN_SLICES) row_sums_kernel(const float* __restrict__ row_sums, long long pitch, int parts,
+                                                                    const int* __restrict__ count, int add,
+                                                                    float* __restrict__ others) {
+  __shared__ float sums[JOIN_SLICES][33];
+  chain_wait();
+  chain_next();
+  const int row = blockIdx.x * 32 + threadIdx.x;
+  const bool ok = row < *count;
+  float sum = 0.0f;
+  if (ok) {
+#pragma unroll 8
+    for (int i = threadIdx.y; i < parts; i += JOIN_SLICES) sum += row_sums[i * pitch + row];
+  }
+  sums[threadIdx.y][threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.y != 0 || !ok) return;
+  sum = add ? others[row] : 0.0f;
+#pragma unroll 8
+  for (int s = 0; s < JOIN_SLICES; ++s) sum += sums[s][threadIdx.x];
+  others[row] = sum;
 }
 
 // The sum of coef_i x_i over the rows that have a word as target, in their order, in slices of WORD_SLICE rows of a word:
@@ -1393,7 +1459,7 @@ int launch_few(const CUtensorMap& words, const State& st, long long hidden, long
 }
 
 struct GradSpace {
-  float *scale, *weights, *coef, *word_sums, *sums, *part_sums;
+  float *scale, *weights, *coef, *word_sums, *sums, *part_sums, *row_sums, *others;
   unsigned* slots;
   int* members;
   __nv_bfloat16* probs;
@@ -1415,6 +1481,8 @@ struct GradSpace {
     word_sums = reinterpret_cast<float*>(take(4 * tokens * hidden));
     sums = piece < vocab ? reinterpret_cast<float*>(take(4 * tokens * hidden)) : nullptr;
     part_sums = reinterpret_cast<float*>(take(2ll * (sm_count() / 2) * TILE * TILE * 4));
+    row_sums = reinterpret_cast<float*>(take(4 * tokens * (piece / HALF)));
+    others = reinterpret_cast<float*>(take(4 * tokens));
     probs = reinterpret_cast<__nv_bfloat16*>(take(2 * tokens * piece));
     bytes = at;
   }
@@ -1550,26 +1618,32 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
     Params p = base;
     p.first_word = static_cast<int>(first);
     p.n = static_cast<int>(words), p.k = width;
+    p.row_sums = w.row_sums, p.pitch = tokens;
+    int parts;  // sums that the probabilities of a row leave
     if (first < st.kept) {
       const int whole = static_cast<int>(tiles_of(words) * TILE);
-      if (int rc = launch_chained(spread_kernel,
-                                  dim3(static_cast<unsigned>((tokens + 7) / 8), (whole + SPREAD_WORDS - 1) / SPREAD_WORDS), dim3(256), 0,
-                                  s, st.codes, st.kept, st.tops, tokens, p.first_word, whole, st.count, st.lse, w.weights, tokens,
-                                  w.probs, w.piece))
+      parts = (whole + SPREAD_WORDS - 1) / SPREAD_WORDS;
+      if (int rc = launch_chained(spread_kernel, dim3(static_cast<unsigned>((tokens + 7) / 8), parts), dim3(256), 0, s, st.codes,
+                                  st.kept, st.tops, tokens, p.first_word, whole, st.count, st.lse, w.weights, tokens, w.probs, w.piece,
+                                  w.row_sums))
         return rc;
     } else {
+      parts = static_cast<int>(2 * tiles_of(words));
       if (int rc = map_k_major(&head_k, head, hidden, words, weight_stride)) return rc;
       if (int rc = map_store(&probs_store, w.probs, words, tokens, w.piece)) return rc;
       if (int rc = launch_product<PROBS>(rows_k, head_k, probs_store, p, tiles_of(tokens) * tiles_of(words), s)) return rc;
     }
     if (grad_hidden != nullptr) {
+      if (int rc = launch_chained(row_sums_kernel, dim3(static_cast<unsigned>((tokens + 31) / 32)), dim3(32, JOIN_SLICES), 0, s, w.row_sums,
+                                  tokens, parts, st.count, first > 0, w.others))
+        return rc;
       if (int rc = map_k_major(&probs_k, w.probs, words, tokens, w.piece)) return rc;
       if (int rc = map_mn_major(&head_mn, head, hidden, words, weight_stride)) return rc;
       p.n = width, p.k = static_cast<int>(words);
       p.sums = w.sums, p.add = first > 0, p.last = first + words == vocab;
       p.head = static_cast<const __nv_bfloat16*>(weight), p.head_stride = weight_stride;
       p.out = static_cast<__nv_bfloat16*>(grad_hidden);
-      p.part_sums = w.part_sums;
+      p.part_sums = w.part_sums, p.others = w.others;
       const long long tiles = tiles_of(tokens) * tiles_of(width);
       if (int rc = launch_product<GRAD_HIDDEN>(probs_k, head_mn, probs_k, p, tiles, s)) return rc;
       if (int rc = launch_chained(join_parts_kernel, dim3(TILE / 8, static_cast<unsigned>(cut_tiles(tiles))), dim3(256), 0, s, p,
