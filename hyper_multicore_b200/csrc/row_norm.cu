@@ -517,8 +517,8 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         if (r > 0 && row + r >= end) break;
-        // dx = rstd g - (x - mean) rstd^2 mean(g u) - rstd mean(g), u = (x - mean) rstd
-        const float2 back = both(-sums[r].x * scale * rstd[r] * rstd[r]), offset = both(CENTER ? -sums[r].y * scale : 0.0f);
+        // dx = rstd (g - (x - mean) rstd mean(g u)) - rstd mean(g), u = (x - mean) rstd: rstd^2 alone may be out of range
+        const float2 back = both(-sums[r].x * scale * rstd[r]), offset = both(CENTER ? -sums[r].y * scale : 0.0f);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
           if (here[j]) {
@@ -527,9 +527,8 @@ stream_wide_grad_kernel(const T* __restrict__ x, long long x_stride, const T* __
             widen(j, r, c, d);
 #pragma unroll
             for (int i = 0; i < PAIRS; ++i) {
-              d[i] = times2(d[i], both(rstd[r]));
-              d[i] = CENTER ? madd2(d[i], w[i], offset) : times2(d[i], w[i]);
-              d[i] = madd2(c[i], back, d[i]);
+              d[i] = madd2(c[i], back, times2(d[i], w[i]));
+              d[i] = CENTER ? madd2(d[i], both(rstd[r]), offset) : times2(d[i], both(rstd[r]));
             }
             st_16(dst + r * hidden + j * threads * VEC, Quad<T>::narrow(d));
           }
