@@ -19,6 +19,13 @@ def as_rows(tensor: torch.Tensor, width: int) -> torch.Tensor:
     return rows if width == 1 or rows.stride(1) == 1 else rows.contiguous()
 
 
+def as_vector(tensor: torch.Tensor) -> torch.Tensor:
+    """``tensor`` [width] as adjacent values; a lazily negated view is one of other values, contiguous or not."""
+    if tensor.is_neg():
+        tensor = tensor.resolve_neg()
+    return tensor if tensor.is_contiguous() else tensor.contiguous()
+
+
 def plain_grad(grad: torch.Tensor, what: str) -> torch.Tensor:
     """``grad``; one that is batched by vmap (``is_grads_batched``) and so no memory of its own is refused."""
     if _functorch.is_legacy_batchedtensor(grad) or _functorch.is_functorch_wrapped_tensor(grad):

@@ -12,7 +12,7 @@ from typing import Any
 import torch
 
 from .. import _lib, kernels
-from ._rows import as_rows, first_order, plain_grad
+from ._rows import as_rows, as_vector, first_order, plain_grad
 
 
 def _fits(x, weight, bias, eps) -> bool:
@@ -90,10 +90,10 @@ class _RowNormFunction(torch.autograd.Function):
 def _forward(x, weight, bias, center, eps, keep):
     """(y, x as rows, parameters as the kernel reads them, statistics)"""
     rows = as_rows(x, x.shape[-1])
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
+    if weight is not None:
+        weight = as_vector(weight)
+    if bias is not None:
+        bias = as_vector(bias)
     y, stats = kernels.row_norm(rows, weight, bias, center, eps, keep, x.device)
     return y if x.ndim == 2 else y.view(x.shape), rows, weight, bias, stats
 

@@ -23,3 +23,14 @@ def test_tiny_rows_without_eps(center, hidden, dtype, exponent):
     y, grads = run(x, weight, bias, grad, center, eps=0.0)
     assert all(t.isfinite().all() for t in (y, *(g for g in grads if g is not None)))
     check(y, grads, x, weight, bias, grad, center, 0.0)
+
+
+@pytest.mark.parametrize("hidden", [1, 64, 1000])
+def test_lazily_negated_tensors(hidden):
+    """A conjugate's imaginary part is a view that is negated when it is read."""
+    x, weight, bias, grad = make(6, hidden, torch.float32, torch.float32, True, seed=2)
+    negated = [torch._neg_view(-t) for t in (x, weight, bias, grad)]
+    assert all(n.is_neg() and torch.equal(n, t) for n, t in zip(negated, (x, weight, bias, grad)))
+    want, want_grads = run(x, weight, bias, grad, True)
+    y, grads = run(*negated, True)
+    assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(grads, want_grads))
