@@ -5,6 +5,7 @@ from __future__ import annotations
 from collections.abc import Callable
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 _functorch = torch._C._functorch  # pylint: disable=protected-access
@@ -31,6 +32,15 @@ def plain_grad(grad: torch.Tensor, what: str) -> torch.Tensor:
     if _functorch.is_legacy_batchedtensor(grad) or _functorch.is_functorch_wrapped_tensor(grad):
         raise RuntimeError(f"{what} does not take gradients batched by vmap (is_grads_batched); call its backward once each")
     return grad
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """An error where forward mode would differentiate ``what``: a dual tensor requires no gradient, so nothing else stops it from
+    being read as its value alone, a derivative of zero."""
+    if forward_ad._current_level < 0:  # pylint: disable=protected-access
+        return
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative; differentiate it in reverse")
 
 
 def first_order(backward: Callable) -> Callable:

@@ -11,7 +11,7 @@ from typing import Any
 import torch
 
 from .. import _lib, kernels
-from ._rows import as_rows, first_order, plain_grad
+from ._rows import as_rows, first_order, plain_grad, refuse_tangents
 
 
 def _fits(hidden, weight, targets, ignore_index, reduction) -> bool:
@@ -114,6 +114,7 @@ def mega_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torc
     """
     if recompute is not False and recompute is not True:
         raise ValueError(f"recompute must be a bool, got {recompute!r}.")
+    refuse_tangents("MegaCrossEntropy", hidden, weight)
     _validate(hidden, weight, targets, ignore_index, reduction)
     rows = as_rows(hidden, weight.shape[1])
     flat = targets if targets.ndim == 1 and targets.is_contiguous() else targets.reshape(-1).contiguous()

@@ -12,7 +12,7 @@ from typing import Any
 import torch
 
 from .. import _lib, kernels
-from ._rows import as_rows, as_vector, first_order, plain_grad
+from ._rows import as_rows, as_vector, first_order, plain_grad, refuse_tangents
 
 
 def _fits(x, weight, bias, eps) -> bool:
@@ -99,6 +99,7 @@ def _forward(x, weight, bias, center, eps, keep):
 
 
 def _norm(x, weight, bias, center, eps):
+    refuse_tangents("a row norm", x, weight, bias)
     if not _fits(x, weight, bias, eps):
         _validate(x, weight, bias, eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
