@@ -758,9 +758,18 @@ def mx_pack_weight_scale(scale: torch.Tensor, axis: int, experts: int, m: int, n
 
 # ------------------------------------------------------------------------------- norms and the vocabulary
 @functools.lru_cache(maxsize=256)
-def _size(name: str, *extents: int) -> int:
-    """What a ``..._bytes`` entry point says; it depends on the extents alone."""
-    return getattr(_lib.load(), name)(*extents)
+def _size_on(index: int, name: str, *extents: int) -> int:
+    if index == torch.cuda.current_device():
+        return getattr(_lib.load(), name)(*extents)
+    with torch.cuda.device(index):
+        return getattr(_lib.load(), name)(*extents)
+
+
+def _size(name: str, *extents: int, device: torch.device | None = None) -> int:
+    """What a ``..._bytes`` entry point says on ``device`` (the current one if None): it depends on the extents and on the
+    device's number of SMs."""
+    index = None if device is None else device.index
+    return _size_on(torch.cuda.current_device() if index is None else index, name, *extents)
 
 
 def _rows_like(x: torch.Tensor) -> torch.Tensor:
@@ -820,7 +829,7 @@ def row_norm_grad(grad, x, weight, stats, center: bool, affine_dtype, need_x: bo
         grad_bias = torch.empty(hidden, dtype=affine_dtype, device=device) if weight is None else torch.empty_like(weight)
         db = grad_bias.data_ptr()
     if need_weight or need_bias:
-        need = _size("hmc_row_norm_grad_workspace_bytes", rows, hidden)
+        need = _size("hmc_row_norm_grad_workspace_bytes", rows, hidden, device=device)
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
         space = workspace.data_ptr()
     rstd = stats.data_ptr()
@@ -840,8 +849,8 @@ def vocab_loss(x, weight, targets, *, ignore_index: int, reduction: str, keep: b
     device = _require_cuda(x, weight, targets)
     (tokens, hidden), vocab = x.shape, weight.shape[0]
     loss = torch.empty((tokens,) if reduction == "none" else (), dtype=torch.float32, device=device)
-    state = torch.empty(_size("hmc_vocab_loss_state_bytes", tokens, hidden, vocab, keep), dtype=torch.uint8, device=device)
-    need = _size("hmc_vocab_loss_workspace_bytes", tokens, vocab)
+    state = torch.empty(_size("hmc_vocab_loss_state_bytes", tokens, hidden, vocab, keep, device=device), dtype=torch.uint8, device=device)
+    need = _size("hmc_vocab_loss_workspace_bytes", tokens, vocab, device=device)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _call("hmc_vocab_loss", device, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), targets.data_ptr(),
           targets.dtype == torch.int64, tokens, hidden, vocab, ignore_index, _lib.HMC_REDUCE[reduction], keep,
@@ -856,7 +865,7 @@ def vocab_loss_grad(grad_loss, state, weight, tokens: int, *, reduction: str, ne
     vocab, hidden = weight.shape
     grad_hidden = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=device) if need_hidden else None
     grad_weight = torch.empty((vocab, hidden), dtype=torch.bfloat16, device=device) if need_weight else None
-    need = _size("hmc_vocab_loss_grad_workspace_bytes", tokens, hidden, vocab)
+    need = _size("hmc_vocab_loss_grad_workspace_bytes", tokens, hidden, vocab, device=device)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _call("hmc_vocab_loss_grad", device, state.data_ptr(), weight.data_ptr(), weight.stride(0), tokens, hidden, vocab,
           _lib.HMC_REDUCE[reduction], keep, grad_loss.data_ptr(), _lib.ptr(grad_hidden), _lib.ptr(grad_weight),
