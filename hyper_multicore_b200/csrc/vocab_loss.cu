@@ -89,8 +89,30 @@ struct Params {
   const int* slots;           // GRAD_WEIGHT: [vocab] row of word_sums, or -1
   const float* word_sums;     // GRAD_WEIGHT: [rows, n]
   float* part_sums;           // GRAD_HIDDEN: [parts][TILE][TILE] of the tiles that are cut
-  int* status;
+  int* failed;  // status words of this chain of launches
+  int* status;  // the caller's, or NULL
 };
+
+// A wait that gave up is told to the chain, whose later launches answer with NaN, and to the caller.
+__device__ __forceinline__ void give_up(int* failed, int* status, int role, int stage, int kb) {
+  report_status(failed, HMC_STATUS_TIMEOUT_PIPELINE, role, stage, kb);
+  report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, role, stage, kb);
+}
+__device__ __forceinline__ bool has_failed(const int* failed, const int* status) {
+  return __ldcg(failed) != 0 || (status != nullptr && __ldcg(status) != 0);
+}
+__device__ __forceinline__ float not_a_number() { return __int_as_float(0x7fffffff); }
+
+// After a wait that gave up: the copies that are still on their way into shared memory, from this stage on. The leader's
+// barriers count both CTAs' bytes, and the partner cannot leave before the leader. A stage that was never filled costs a tenth of a second.
+__device__ __forceinline__ void await_copies(uint64_t* full_bar, int stages, int stage, uint32_t phase) {
+  volatile int unused = 0;
+  for (int s = 0; s < stages; ++s) {
+    mbar_wait(&full_bar[stage], phase, &unused, 100ull * 1000 * 1000);
+    unused = 0;
+    if (++stage == stages) stage = 0, phase ^= 1u;
+  }
+}
 
 // A unit of work: a tile and its range of k-blocks. Part -1 is the whole of it.
 struct Unit {
@@ -293,7 +315,7 @@ __device__ __forceinline__ void epilogue_probs(const Params& p, const CUtensorMa
 
 // With the last piece: what a row of dx takes the target's row times, and what the whole is scaled by.
 __device__ __forceinline__ float2 row_coefficients(const Params& p, int row) {
-  const float coef = p.coef[row], others = p.others[row], scale = *p.scale;
+  const float coef = p.coef[row], others = p.others[row], scale = has_failed(p.failed, p.status) ? not_a_number() : *p.scale;
   // nothing stored (a gradient of zero, no other word, a certain token): the true coefficient, which is as small
   return others != 0.0f ? make_float2(-others, scale * (-coef / others)) : make_float2(coef, scale);
 }
@@ -328,13 +350,19 @@ __device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int
                    pack_bf16x2(v[4] * scale, v[5] * scale), pack_bf16x2(v[6] * scale, v[7] * scale)));
 }
 
-__device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t taddr, int row, bool row_ok, int col) {
+// lost: nothing is in the accumulator.
+__device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t taddr, int row, bool row_ok, int col, bool lost) {
   const float2 by = row_ok && p.last ? row_coefficients(p, row) : both(0.0f);
 #pragma unroll 1
   for (int c = 0; c < HALF; c += 64) {
     if (col + c >= p.n) break;
     float v[64];
-    load_columns(taddr + c, v);
+    if (lost) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) v[j] = not_a_number();
+    } else {
+      load_columns(taddr + c, v);
+    }
     if (row_ok) {
 #pragma unroll
       for (int j = 0; j < 64; j += 8)
@@ -383,8 +411,8 @@ __global__ void __launch_bounds__(256) join_parts_kernel(Params p, int pairs) {
 
 __device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
                                                      unsigned& issued, int first_row, int row, bool row_ok, int col, int lane,
-                                                     bool empty) {
-  const float scale = *p.scale;
+                                                     bool empty, float filler) {
+  const float scale = has_failed(p.failed, p.status) ? not_a_number() : *p.scale;
   const int slot = row_ok ? p.slots[p.first_word + row] : -1;
   const float* more = p.word_sums + static_cast<long long>(slot >= 0 ? slot : 0) * p.n + col;
 #pragma unroll 1
@@ -393,7 +421,7 @@ __device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUte
     float v[64];
     if (empty) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j) v[j] = 0.0f;
+      for (int j = 0; j < 64; ++j) v[j] = filler;
     } else {
       load_columns(taddr + c, v);
       if (slot >= 0) {
@@ -482,7 +510,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         const int n0 = u.ni * TILE + static_cast<int>(rank) * HALF;
         for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
-            report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 0, stage, kb);
+            give_up(p.failed, p.status, 0, stage, kb);
             ok = false;
             break;
           }
@@ -527,7 +555,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         for (int first = u.kb0; ok && first < u.kb1; first += KIND == STATS ? CHAIN : u.kb1 - u.kb0) {
           const int end = KIND == STATS ? min(u.kb1, first + CHAIN) : u.kb1;
           if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
-            if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 1, acc, 0);
+            if (lane == 0) give_up(p.failed, p.status, 1, acc, 0);
             ok = false;
             break;
           }
@@ -535,7 +563,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * TILE);
           for (int kb = first; kb < end; ++kb) {
             if (!mbar_wait(&full_bar[stage], phase, abort_word, PIPE_BUDGET_NS)) {
-              if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 2, stage, kb);
+              if (lane == 0) give_up(p.failed, p.status, 2, stage, kb);
               ok = false;
               break;
             }
@@ -565,6 +593,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           }
         }
       }
+      if (!ok) await_copies(full_bar, STAGES, stage, phase);
     }
   } else {
     // ======================================================================== epilogue (both CTAs)
@@ -579,7 +608,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * HALF);
     auto filled = [&]() {  // the next accumulator, once its MMAs are done
       if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_word, PIPE_BUDGET_NS)) {
-        if (lane == 0) report_status(p.status, HMC_STATUS_TIMEOUT_PIPELINE, 3, acc, 0);
+        if (lane == 0) give_up(p.failed, p.status, 3, acc, 0);
         ok = false;
       }
       tc_fence_after_sync();
@@ -594,14 +623,15 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         acc_phase ^= 1u;
       }
     };
-    for (long long idx = pair; ok && walker.get(idx, u); idx += pairs) {
+    // a gradient's tiles that are lost to a wait that gave up are filled with NaN
+    for (long long idx = pair; (ok || KIND == GRAD_HIDDEN || KIND == GRAD_WEIGHT) && walker.get(idx, u); idx += pairs) {
       const int in_tile = static_cast<int>(rank) * HALF + quarter * 32;
       const int first_row = u.mi * TILE + in_tile;
       const int row = first_row + lane;
       const bool row_ok = row < p.m;
       const int col = u.ni * TILE + half * HALF;
       if (kiters == 0) {  // no token counts: the weight's gradient is zero
-        if (KIND == GRAD_WEIGHT) epilogue_grad_weight(p, &tm_c, 0, my_stage, issued, first_row, row, row_ok, col, lane, true);
+        if (KIND == GRAD_WEIGHT) epilogue_grad_weight(p, &tm_c, 0, my_stage, issued, first_row, row, row_ok, col, lane, true, 0.0f);
         continue;
       }
       if (KIND == STATS) {
@@ -627,15 +657,21 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         __syncwarp();
         continue;
       }
-      if (!filled()) break;
+      if (!ok || !filled()) {
+        // of a tile that is cut, the launch that joins its parts writes NaN
+        if (KIND == GRAD_HIDDEN && u.part < 0) epilogue_grad_hidden(p, 0, row, row_ok, col, true);
+        if (KIND == GRAD_WEIGHT)
+          epilogue_grad_weight(p, &tm_c, 0, my_stage, issued, first_row, row, row_ok, col, lane, true, not_a_number());
+        continue;
+      }
       const uint32_t taddr = lane_base + static_cast<uint32_t>(acc * TILE);
       if (KIND == PROBS) epilogue_probs(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, 2 * u.ni + half, lane);
       if (KIND == GRAD_HIDDEN) {
         if (u.part >= 0) epilogue_part(p, taddr, u.part, in_tile + lane, row_ok, half);
-        else epilogue_grad_hidden(p, taddr, row, row_ok, col);
+        else epilogue_grad_hidden(p, taddr, row, row_ok, col, false);
       }
       if (KIND == GRAD_WEIGHT)
-        epilogue_grad_weight(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane, false);
+        epilogue_grad_weight(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane, false, 0.0f);
       release();
     }
     if (issued > 0 && lane == 0) bulk_wait_all();  // this thread's stores are in global memory
@@ -693,7 +729,7 @@ template <int N>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Few<N>::THREADS, 1)
 few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_constant__ CUtensorMap tm_tokens, int vocab, int kiters,
                   const int* __restrict__ count, const int* __restrict__ labels, float2* __restrict__ partial, long long pitch,
-                  int* status) {
+                  int* failed, int* status) {
   using F = Few<N>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -754,7 +790,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
         const int word = t * TILE + static_cast<int>(rank) * HALF;
         for (int kb = t == pair ? early : 0; kb < kiters; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
-            report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 0, stage, kb);
+            give_up(failed, status, 0, stage, kb);
             ok = false;
             break;
           }
@@ -783,14 +819,14 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
         for (int first = 0; ok && first < kiters; first += PROMOTE) {
           const int end = min(kiters, first + PROMOTE);
           if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
-            if (lane == 0) report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 1, acc, 0);
+            if (lane == 0) give_up(failed, status, 1, acc, 0);
             ok = false;
             break;
           }
           tc_fence_after_sync();
           for (int kb = first; kb < end; ++kb) {
             if (!mbar_wait(&full_bar[stage], phase, abort_word, PIPE_BUDGET_NS)) {
-              if (lane == 0) report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 2, stage, kb);
+              if (lane == 0) give_up(failed, status, 2, stage, kb);
               ok = false;
               break;
             }
@@ -820,6 +856,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
           }
         }
       }
+      if (!ok) await_copies(full_bar, F::STAGES, stage, phase);
     }
   } else {
     // ======================================================================== epilogue (both CTAs)
@@ -846,7 +883,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tm_words, const __grid_con
       for (int j = 0; j < C; ++j) v[j] = 0.0f;
       for (int first = 0; first < kiters; first += PROMOTE) {
         if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_word, PIPE_BUDGET_NS)) {
-          if (lane == 0) report_status(status, HMC_STATUS_TIMEOUT_PIPELINE, 3, acc, 0);
+          if (lane == 0) give_up(failed, status, 3, acc, 0);
           ok = false;
           break;
         }
@@ -939,7 +976,7 @@ __device__ __forceinline__ int block_count(int v) {  // sum over the block, in e
 // a contraction over them. Bound by latency (8192 x 4096: 50 us for 200 MB with the targets' rows; 5 us for 16 tokens).
 __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bfloat16* __restrict__ x, long long x_stride,
                                                                  Targets targets, long long tokens, int hidden, int vector,
-                                                                 int* __restrict__ count, int* __restrict__ done,
+                                                                 int* __restrict__ count, int* __restrict__ done, int* __restrict__ failed,
                                                                  int* __restrict__ position,
                                                                  int* __restrict__ row_of, int* __restrict__ labels,
                                                                  __nv_bfloat16* __restrict__ packed,
@@ -1003,6 +1040,7 @@ __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const __nv_bflo
   for (int t = 0; t < PACK_TOKENS; ++t) rows += place[t] >= 0;
   rows += before;
   if (threadIdx.x == 0) *count = rows, *done = 0;
+  if (threadIdx.x < HMC_STATUS_WORDS) failed[threadIdx.x] = 0;
   const long long end = min(tokens, static_cast<long long>((rows + BK - 1) / BK) * BK);
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (long long c = rows * static_cast<long long>(hidden) + threadIdx.x * 8; c < end * hidden; c += PACK_THREADS * 8)
@@ -1021,10 +1059,13 @@ __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __
                                                                 const int* __restrict__ row_of,
                                                                 const float* __restrict__ target_logit,
                                                                 float* __restrict__ lse, float* losses, int reduction,
-                                                                int* __restrict__ done, float* __restrict__ loss_out) {
+                                                                int* __restrict__ done, int* failed, const int* status,
+                                                                float* __restrict__ loss_out) {
   __shared__ float2 sums[JOIN_SLICES][33];
   chain_wait();
   chain_next();
+  const bool lost = has_failed(failed, status);
+  if (lost && blockIdx.x == 0 && threadIdx.x == 0 && threadIdx.y == 0) *failed = HMC_STATUS_TIMEOUT_PIPELINE;  // for the gradient
   const int row = blockIdx.x * 32 + threadIdx.x;
   const int rows = *count;
   const bool ok = row < rows;
@@ -1056,9 +1097,9 @@ __global__ void __launch_bounds__(32 * JOIN_SLICES) join_kernel(const float2* __
     for (int s = 0; s < JOIN_SLICES; ++s) sum += sums[s][threadIdx.x].y * shifted_exp(sums[s][threadIdx.x].x, shift);
     const float log_sum = own >= top ? log1pf(sum) : logf(sum + shifted_exp(own, shift));
     float loss = log_sum + (shift - own);
-    // a target outside the vocabulary has no loss, and neither has a row whose largest logit is infinite: NaN, which no
-    // later sum hides
-    if (labels[row] < 0 || isinf(shift)) loss = __int_as_float(0x7fffffff);
+    // a target outside the vocabulary has no loss, and neither has a row whose largest logit is infinite, or one whose sums were
+    // not finished: NaN, which no later sum hides
+    if (labels[row] < 0 || isinf(shift) || lost) loss = not_a_number();
     lse[row] = shift + log_sum;
     losses[row] = loss;
     if (reduction == HMC_REDUCE_NONE) loss_out[row_of[row]] = loss;
@@ -1094,7 +1135,8 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
                                                         const int* __restrict__ row_of, const float* __restrict__ losses,
                                                         float* __restrict__ weights, float* __restrict__ coef,
                                                         float* __restrict__ scale, unsigned* __restrict__ slots,
-                                                        int* __restrict__ members) {
+                                                        int* __restrict__ members, const int* __restrict__ forward_failed,
+                                                        const int* __restrict__ status, int* __restrict__ failed) {
   chain_next();  // the first of its chain
   const int rows = *count;
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
@@ -1104,10 +1146,12 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
     if (reduction == HMC_REDUCE_MEAN) s = rows > 0 ? grad[0] / static_cast<float>(rows) : 0.0f;
     *scale = s;
   }
+  const bool lost = has_failed(forward_failed, status);
+  if (i < HMC_STATUS_WORDS) failed[i] = 0;
   if (i >= rows) return;
   const int label = labels[i];
   float w = reduction == HMC_REDUCE_NONE ? grad[row_of[i]] : 1.0f;
-  if (label < 0) w = __int_as_float(0x7fffffff);
+  if (label < 0 || lost) w = not_a_number();
   weights[i] = w;
   coef[i] = label >= 0 ? w * expm1f(-losses[i]) : 0.0f;  // w (p_target - 1)
   if (slots != nullptr && label >= 0) {
@@ -1415,7 +1459,7 @@ long long kept_words(long long tokens, long long vocab) {
 
 // What a forward leaves for its gradient, in one buffer of the caller.
 struct State {
-  int *count, *done, *position, *row_of, *labels;
+  int *count, *done, *failed, *position, *row_of, *labels;
   float *lse, *losses;
   __nv_bfloat16* packed;
   uint16_t* codes;  // [tokens][kept]
@@ -1427,6 +1471,7 @@ struct State {
     const long long words = up256(4 * tokens);
     count = reinterpret_cast<int*>(p);
     done = count + 1;
+    failed = count + 4;  // status words
     position = reinterpret_cast<int*>(p + 256);
     row_of = reinterpret_cast<int*>(p + 256 + words);
     labels = reinterpret_cast<int*>(p + 256 + 2 * words);
@@ -1455,13 +1500,13 @@ int launch_few(const CUtensorMap& words, const State& st, long long hidden, long
   if (int rc = allow_dynamic_smem(few_tokens_kernel<N>, Few<N>::SMEM, configured)) return rc;
   *parts = static_cast<int>(few_parts(p.n));
   return launch_chained(few_tokens_kernel<N>, dim3(*parts / 4), dim3(Few<N>::THREADS), Few<N>::SMEM, stream, words, rows, p.n,
-                        (p.k + BK - 1) / BK, p.count, p.labels, p.partial, p.pitch, p.status);
+                        (p.k + BK - 1) / BK, p.count, p.labels, p.partial, p.pitch, p.failed, p.status);
 }
 
 struct GradSpace {
   float *scale, *weights, *coef, *word_sums, *sums, *part_sums, *row_sums, *others;
   unsigned* slots;
-  int* members;
+  int *members, *failed;
   __nv_bfloat16* probs;
   long long slot_bytes, bytes, piece;
   GradSpace(void* base, long long tokens, long long hidden, long long vocab) {
@@ -1473,6 +1518,7 @@ struct GradSpace {
       return p;
     };
     scale = reinterpret_cast<float*>(take(4));
+    failed = reinterpret_cast<int*>(take(4 * HMC_STATUS_WORDS));
     weights = reinterpret_cast<float*>(take(4 * tokens));
     coef = reinterpret_cast<float*>(take(4 * tokens));
     slots = reinterpret_cast<unsigned*>(take(4 * vocab));
@@ -1542,13 +1588,13 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
   const int vector = aligned16(x) && x_stride % 8 == 0;
   if (int rc = launch_chained(pack_rows_kernel, dim3(static_cast<unsigned>((tokens + PACK_TOKENS - 1) / PACK_TOKENS)), dim3(PACK_THREADS),
                               0, s, static_cast<const __nv_bfloat16*>(x), x_stride, given, tokens, static_cast<int>(hidden), vector,
-                              st.count, st.done, st.position, st.row_of, st.labels, st.packed,
+                              st.count, st.done, st.failed, st.position, st.row_of, st.labels, st.packed,
                               static_cast<const __nv_bfloat16*>(weight), weight_stride, target_logit, token_loss))
     return rc;
 
   Params p{};
   p.n = static_cast<int>(vocab), p.k = static_cast<int>(hidden);
-  p.count = st.count, p.labels = st.labels, p.partial = partial, p.pitch = tokens, p.status = status;
+  p.count = st.count, p.labels = st.labels, p.partial = partial, p.pitch = tokens, p.failed = st.failed, p.status = status;
   CUtensorMap a, b;
   if (int rc = map_k_major(&b, weight, hidden, vocab, weight_stride)) return rc;
   int parts = 0;
@@ -1568,7 +1614,7 @@ extern "C" int hmc_vocab_loss(const void* x, int64_t x_stride, const void* weigh
     parts = static_cast<int>(2 * tiles_of(vocab));
   }
   return launch_chained(join_kernel, dim3(static_cast<unsigned>((tokens + 31) / 32)), dim3(32, JOIN_SLICES), 0, s, partial, tokens, parts,
-                        st.count, st.labels, st.row_of, target_logit, st.lse, st.losses, reduction, st.done, loss);
+                        st.count, st.labels, st.row_of, target_logit, st.lse, st.losses, reduction, st.done, st.failed, status, loss);
 }
 
 extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_t weight_stride, int64_t tokens, int64_t hidden,
@@ -1592,7 +1638,7 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
   if (grad_weight != nullptr) HMC_CUDA_OK(cudaMemsetAsync(w.slots, 0xff, w.slot_bytes, s));  // no first row, -1 members
   grad_rows_kernel<<<static_cast<unsigned>((tokens + 255) / 256), 256, 0, s>>>(
       grad_loss, reduction, st.count, st.labels, st.row_of, st.losses, w.weights, w.coef, w.scale,
-      grad_weight != nullptr ? w.slots : nullptr, w.members);
+      grad_weight != nullptr ? w.slots : nullptr, w.members, st.failed, status, w.failed);
   HMC_LAUNCH_OK();
   float* word_sums = grad_weight != nullptr ? w.word_sums : nullptr;
   if (int rc = launch_chained(token_rows_kernel, dim3(static_cast<unsigned>(tokens)), dim3(WORD_THREADS), 0, s, st.packed, width, st.count,
@@ -1607,7 +1653,7 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
 
   Params base{};
   base.count = st.count, base.labels = st.labels, base.lse = st.lse, base.weights = w.weights, base.scale = w.scale;
-  base.coef = w.coef, base.row_of = st.row_of, base.status = status;
+  base.coef = w.coef, base.row_of = st.row_of, base.failed = w.failed, base.status = status;
   CUtensorMap rows_k, rows_mn;
   if (int rc = map_k_major(&rows_k, st.packed, hidden, tokens, hidden)) return rc;
   if (int rc = map_mn_major(&rows_mn, st.packed, hidden, tokens, hidden)) return rc;

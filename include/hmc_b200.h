@@ -1004,7 +1004,9 @@ int hmc_row_norm_grad(const void* x, int64_t x_stride, const void* grad, int64_t
  * ignored tokens), or loss [1], the sum or the mean over the tokens that count (NaN where none does). `state` (16-byte
  * aligned, of ..._state_bytes) keeps what the gradient needs, the counted rows of x among it, and with
  * `keep` the logits of the words that fit 4 GiB as 16-bit distances from the largest of 128 (none for up to 128 tokens).
- * Logits and sums in FP32. */
+ * Logits and sums in FP32. A wait inside a kernel that gives up is told in `status` (int32[HMC_STATUS_WORDS] or NULL) and in the
+ * state: every loss that counts is NaN then, and so is every gradient from that state; the same holds while `status` carries an
+ * error from before. A gradient that gives up by itself leaves NaN in what it could not finish. */
 #define HMC_REDUCE_NONE 0
 #define HMC_REDUCE_MEAN 1
 #define HMC_REDUCE_SUM 2
