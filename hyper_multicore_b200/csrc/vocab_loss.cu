@@ -61,6 +61,10 @@ constexpr int MIN_PART = 8;    // k-blocks of a part, at the least
 // of 4096 over 131072 words: 8 7.63 ms, 16 7.30, 32 7.22, 64 (all of it) 6.85. With 32 the loss is off by 1.5e-7 to 3e-7
 // (FP32 throughout: 2.8e-7 to 9e-7).
 constexpr int PROMOTE = 32;
+// The same of the two gradient products: 1024 additions in the tensor core, which truncates, before a sum goes on in FP32 registers. (Over
+// 131072 tokens at once the weight's gradient was off by 6.5e-4 of its terms, always towards zero, with this by 1e-4. The step of
+// 8192 x 4096 x 131072, whose products over 32768 words take two chains, 23.3 instead of 23.1 ms.)
+constexpr int PROMOTE_GRAD = 256;
 // Tile rows that are walked together, so that a band's rows stay in L2 while the weight passes by once per band (8, 16, 32:
 // 29987, 29527, 31442 us for a training step of 8192 x 4096 x 131072).
 constexpr int BAND = 16;
@@ -261,6 +265,20 @@ __device__ __forceinline__ void epilogue_stats(const Params& p, const CUtensorMa
   }
 }
 
+// What a chain of k-blocks left in the accumulator, added to the sums of those before it. A gradient has few such chains, long ones: the
+// sums may live in local memory.
+__device__ __forceinline__ void add_columns(uint32_t taddr, float* sums, bool first) {
+#pragma unroll 1
+  for (int c = 0; c < HALF; c += 32) {
+    uint32_t raw[32];
+    __syncwarp();
+    tmem_ld_32x32(taddr + c, raw);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) sums[c + j] = (first ? 0.0f : sums[c + j]) + __uint_as_float(raw[j]);
+  }
+}
+
 // 64 columns of the accumulator row of each lane: two loads under way at a time.
 __device__ __forceinline__ void load_columns(uint32_t taddr, float (&v)[64]) {
   uint32_t lo[32], hi[32];
@@ -270,6 +288,15 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, float (&v)[64]) {
   tmem_ld_wait();
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(lo[j]), v[32 + j] = __uint_as_float(hi[j]);
+}
+// The same, or from sums of several chains.
+__device__ __forceinline__ void load_columns(uint32_t taddr, const float* sums, int c, float (&v)[64]) {
+  if (sums == nullptr) {
+    load_columns(taddr + c, v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 64; ++j) v[j] = sums[c + j];
 }
 
 // The reduction over a warp's lanes of each of C columns (halving: a lane hands half of its columns to its partner and
@@ -392,7 +419,8 @@ __device__ __forceinline__ void finish_grad_hidden(const Params& p, int row, int
 }
 
 // lost: nothing is in the accumulator.
-__device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t taddr, int row, bool row_ok, int col, bool lost) {
+__device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t taddr, const float* sums, int row, bool row_ok, int col,
+                                                     bool lost) {
   const float2 by = row_ok && p.last ? row_coefficients(p, row) : both(0.0f);
 #pragma unroll 1
   for (int c = 0; c < HALF; c += 64) {
@@ -402,7 +430,7 @@ __device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t t
 #pragma unroll
       for (int j = 0; j < 64; ++j) v[j] = not_a_number();
     } else {
-      load_columns(taddr + c, v);
+      load_columns(taddr, sums, c, v);
     }
     if (row_ok) {
 #pragma unroll
@@ -413,12 +441,13 @@ __device__ __forceinline__ void epilogue_grad_hidden(const Params& p, uint32_t t
 }
 
 // A part of a tile that is cut along k: its sums as they are.
-__device__ __forceinline__ void epilogue_part(const Params& p, uint32_t taddr, int part, int row_in_tile, bool row_ok, int half) {
+__device__ __forceinline__ void epilogue_part(const Params& p, uint32_t taddr, const float* sums, int part, int row_in_tile, bool row_ok,
+                                              int half) {
   float* dst = p.part_sums + (static_cast<long long>(part) * TILE + row_in_tile) * TILE + half * HALF;
 #pragma unroll 1
   for (int c = 0; c < HALF; c += 64) {
     float v[64];
-    load_columns(taddr + c, v);
+    load_columns(taddr, sums, c, v);
     if (row_ok) {
 #pragma unroll
       for (int j = 0; j < 64; j += 4) *reinterpret_cast<float4*>(dst + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
@@ -450,8 +479,8 @@ __global__ void __launch_bounds__(256) join_parts_kernel(Params p, int pairs) {
   finish_grad_hidden(p, row, col, v, p.last ? row_coefficients(p, row) : both(0.0f));
 }
 
-__device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
-                                                     unsigned& issued, int first_row, int row, bool row_ok, int col, int lane,
+__device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUtensorMap* tm, uint32_t taddr, const float* sums,
+                                                     uint8_t* stage, unsigned& issued, int first_row, int row, bool row_ok, int col, int lane,
                                                      bool empty, float filler) {
   const float scale = has_failed(p.failed, p.status) ? not_a_number() : *p.scale;
   const int slot = row_ok ? p.slots[p.first_word + row] : -1;
@@ -465,7 +494,7 @@ __device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUte
 #pragma unroll
       for (int j = 0; j < 64; ++j) v[j] = filler;
     } else {
-      load_columns(taddr + c, v);
+      load_columns(taddr, sums, c, v);
 #pragma unroll
       for (int j = 0; j < 64; ++j) v[j] *= factor;
       if (slot >= 0) {
@@ -492,7 +521,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                  const __grid_constant__ CUtensorMap tm_c, Params p) {
   constexpr int A_MAJOR = KIND == GRAD_WEIGHT ? HMC_MAJOR_MN : HMC_MAJOR_K;
   constexpr int B_MAJOR = KIND == GRAD_WEIGHT || KIND == GRAD_HIDDEN ? HMC_MAJOR_MN : HMC_MAJOR_K;
-  constexpr int CHAIN = PROMOTE;  // STATS only
+  constexpr int CHAIN = KIND == STATS ? PROMOTE : PROMOTE_GRAD;  // not PROBS
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* store_stage = smem + STAGES * STAGE_BYTES;
@@ -596,8 +625,8 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       constexpr uint32_t B_KSTEP = B_MAJOR == HMC_MAJOR_MN ? (16 * 128) >> 4 : 32 >> 4;
       for (long long idx = pair; ok && walker.get(idx, u); idx += pairs) {
         // one accumulator per unit, or per CHAIN k-blocks of it
-        for (int first = u.kb0; ok && first < u.kb1; first += KIND == STATS ? CHAIN : u.kb1 - u.kb0) {
-          const int end = KIND == STATS ? min(u.kb1, first + CHAIN) : u.kb1;
+        for (int first = u.kb0; ok && first < u.kb1; first += KIND == PROBS ? u.kb1 - u.kb0 : CHAIN) {
+          const int end = KIND == PROBS ? u.kb1 : min(u.kb1, first + CHAIN);
           if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_word, PIPE_BUDGET_NS)) {
             if (lane == 0) give_up(p.failed, p.status, 1, acc, 0);
             ok = false;
@@ -675,7 +704,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       const bool row_ok = row < p.m;
       const int col = u.ni * TILE + half * HALF;
       if (kiters == 0) {  // no token counts: the weight's gradient is zero
-        if (KIND == GRAD_WEIGHT) epilogue_grad_weight(p, &tm_c, 0, my_stage, issued, first_row, row, row_ok, col, lane, true, 0.0f);
+        if (KIND == GRAD_WEIGHT) epilogue_grad_weight(p, &tm_c, 0, nullptr, my_stage, issued, first_row, row, row_ok, col, lane, true, 0.0f);
         continue;
       }
       if (KIND == STATS) {
@@ -701,21 +730,32 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         __syncwarp();
         continue;
       }
+      float chains[HALF];
+      const float* sums = nullptr;
+      if (KIND != PROBS && u.kb1 - u.kb0 > CHAIN) {  // all chains but the last
+        sums = chains;
+        for (int first = u.kb0; ok && first + CHAIN < u.kb1; first += CHAIN) {
+          if (!filled()) break;
+          add_columns(lane_base + static_cast<uint32_t>(acc * TILE), chains, first == u.kb0);
+          release();
+        }
+      }
       if (!ok || !filled()) {
         // of a tile that is cut, the launch that joins its parts writes NaN
-        if (KIND == GRAD_HIDDEN && u.part < 0) epilogue_grad_hidden(p, 0, row, row_ok, col, true);
+        if (KIND == GRAD_HIDDEN && u.part < 0) epilogue_grad_hidden(p, 0, nullptr, row, row_ok, col, true);
         if (KIND == GRAD_WEIGHT)
-          epilogue_grad_weight(p, &tm_c, 0, my_stage, issued, first_row, row, row_ok, col, lane, true, not_a_number());
+          epilogue_grad_weight(p, &tm_c, 0, nullptr, my_stage, issued, first_row, row, row_ok, col, lane, true, not_a_number());
         continue;
       }
       const uint32_t taddr = lane_base + static_cast<uint32_t>(acc * TILE);
+      if (sums != nullptr) add_columns(taddr, chains, false);
       if (KIND == PROBS) epilogue_probs(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, 2 * u.ni + half, lane);
       if (KIND == GRAD_HIDDEN) {
-        if (u.part >= 0) epilogue_part(p, taddr, u.part, in_tile + lane, row_ok, half);
-        else epilogue_grad_hidden(p, taddr, row, row_ok, col, false);
+        if (u.part >= 0) epilogue_part(p, taddr, sums, u.part, in_tile + lane, row_ok, half);
+        else epilogue_grad_hidden(p, taddr, sums, row, row_ok, col, false);
       }
       if (KIND == GRAD_WEIGHT)
-        epilogue_grad_weight(p, &tm_c, taddr, my_stage, issued, first_row, row, row_ok, col, lane, false, 0.0f);
+        epilogue_grad_weight(p, &tm_c, taddr, sums, my_stage, issued, first_row, row, row_ok, col, lane, false, 0.0f);
       release();
     }
     if (issued > 0 && lane == 0) bulk_wait_all();  // this thread's stores are in global memory
