@@ -1,4 +1,4 @@
-"""MegaCrossEntropy: the head of a model and its loss over the vocabulary in one, without logits in full.
+"""MegaCrossEntropy: the head of a model and its loss over the vocabulary in one; logits are held in 16 bits, or not at all.
 
 The reference ends before the head; this is the operator that follows the last norm in training and in scoring.
 """
@@ -100,17 +100,20 @@ class _CrossEntropyFunction(torch.autograd.Function):
 
 def mega_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
                        reduction: str = "mean", recompute: bool = False) -> torch.Tensor:
-    """Cross entropy of ``hidden @ weight.T`` against ``targets``, FP32, without logits in full.
+    """Cross entropy of ``hidden @ weight.T`` against ``targets``, FP32. Where a gradient follows, the call holds its logits in 16 bits
+    until then, up to 4 GiB of them: as much as BF16 logits would take. With ``recompute=True`` it holds none.
 
     ``hidden`` BF16 [..., H] with any strides, ``weight`` BF16 [V, H] with H a multiple of 8, ``targets`` INT32 or INT64 [...].
     ``reduction`` "none" gives a loss per token (0 where the target is ``ignore_index``), "sum" and "mean" run over the other
     tokens; the mean over none of them is NaN, as in torch. Ignored tokens are not read: whatever their hidden states hold,
     their gradient is zero and they add nothing to the weight's. A target outside [0, V) that is not ``ignore_index`` is not
-    noticed on the host: its loss is NaN, and so are the gradients it enters. Differentiable once in ``hidden`` and ``weight``;
-    the gradients are BF16. For the backward pass the forward keeps logits as 16-bit distances from their row's largest, of as many
-    words as fit 4 GiB (none up to 128 tokens), and the others are computed again; with ``recompute`` all of them are and nothing of
-    tokens x vocab is held. The backward pass takes scratch of up to 512 MiB for probabilities (4096 words of them where that is
-    more), 8 bytes per element of ``hidden`` and 8 bytes per word.
+    noticed on the host: its loss is NaN, and so are the gradients it enters. Differentiable once, in reverse, in ``hidden`` and ``weight``;
+    the gradients are BF16, and so are the probabilities that enter them, whose sums over the words of a token and over the tokens of a
+    word are FP32 and kept. What is held are the logits' distances from the largest of 128, of as many words as fit 4 GiB (none up to 128
+    tokens); the others are computed again, with ``recompute`` all of them, which takes a quarter longer. Every call whose graph lives
+    holds its own. The backward pass takes scratch of up to 512 MiB for probabilities (4096 words of them where that is
+    more) and a twelfth of that for their sums, 8 bytes per element of ``hidden`` and per word, and 50 MiB. A wait inside a kernel that gives up
+    makes the loss, or the gradients, NaN.
     """
     if recompute is not False and recompute is not True:
         raise ValueError(f"recompute must be a bool, got {recompute!r}.")

@@ -996,8 +996,8 @@ int hmc_row_norm_grad(const void* x, int64_t x_stride, const void* grad, int64_t
                       int dtype, const void* weight, int affine_dtype, int center, const float* mean, const float* rstd,
                       void* grad_x, void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Cross entropy of hidden states over a vocabulary: loss_i = log sum_j exp(x_i . w_j) - x_i . w_target(i), without
- * logits in full. x [tokens, hidden] and weight [vocab, hidden] BF16 with rows x_stride and weight_stride elements
+/* Cross entropy of hidden states over a vocabulary: loss_i = log sum_j exp(x_i . w_j) - x_i . w_target(i).
+ * Logits are held in 16 bits (`keep`) or not at all. x [tokens, hidden] and weight [vocab, hidden] BF16 with rows x_stride and weight_stride elements
  * apart (weight rows on 16-byte boundaries, hidden a multiple of 8), targets INT32 or INT64. Tokens whose target is
  * ignore_index have no loss and are not read; a target outside [0, vocab), or a largest logit that is infinite, gives a
  * loss of NaN. reduction: loss [tokens] (0 for

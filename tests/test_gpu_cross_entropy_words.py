@@ -24,13 +24,14 @@ def check_words(grad_w, x, weight, targets, grad, words, kept):
     logits = x64 @ w64.t()
     error = x.shape[1] / 16 * 2.0 ** -22 * (x64.abs() @ w64.abs().t()).max()
     p = torch.exp(logits - torch.logsumexp(logits, 1, keepdim=True))
+    wrong = p.scatter(1, targets.unsqueeze(1), 0.0).sum(1)  # 1 - p of the target, also where that has no digits in 64 bits
     unseen = kept + 2 * error + 2.0 ** -19
     off = HALF + unseen
     for j in words:
         own = targets == j
         share = torch.where(own, 0.0, grad.double().abs() * p[:, j])
         signed = x64 * grad.double().sign().unsqueeze(1)
-        target = torch.where(own, grad.double() * (p[:, j] - 1), 0.0)
+        target = torch.where(own, -grad.double() * wrong, 0.0)
         exact = share @ signed + target @ x64
         main = signed[share.argmax()]
         size = share @ x64.abs() + target.abs() @ x64.abs()
