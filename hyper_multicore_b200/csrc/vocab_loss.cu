@@ -22,13 +22,13 @@
 // of the rounding where one token holds the word, or where all tokens rate it alike and what they have in common nearly cancels
 // against the tokens of the word (0.2 % of a row's norm there, 0.66 % without). What the scaling puts right as a whole it may take from the lesser
 // entries: one that is not the largest of its row or word may be off by twice 2^-8.
-// A training step of 8192 x 4096 x 131072 takes 23.2 ms with all its logits kept (2 GiB of 16-bit codes) and 28.4 ms with none,
-// 512 x 1024 x 32000 168 against 194 us. Gradients taken in the forward pass would hold the weight's gradient in FP32 until the
+// A training step of 8192 x 4096 x 131072 takes 23.5 ms with all its logits kept (2 GiB of 16-bit codes) and 29.6 ms with none,
+// 512 x 1024 x 32000 201 against 228 us (two inputs in turn). Gradients taken in the forward pass would hold the weight's gradient in FP32 until the
 // backward one and only fit a loss that is reduced.
 //
 // The GEMM: CTA pairs (tcgen05.mma.cta_group::2, M = N = 256), one TMA producer, one issuer, eight epilogue warps, two
 // accumulators; the layouts of the operands are those of the grouped GEMMs. Bound by the tensor cores: 4096 x 32768 x 4096 takes
-// 750 us in each of the four forms (1466 TFLOP/s, 0.90 of cuBLAS in a burst, tensor pipe 80 to 88 % busy); over seconds the
+// 750 to 785 us in its four forms (1400 to 1466 TFLOP/s, 0.86 to 0.90 of cuBLAS in a burst, tensor pipe 77 to 87 % busy); over seconds the
 // power limit leaves 1250 to 1330 (cuBLAS: 1380). Short k (1024 and below) is bound by L2: 1 MB per 256 x 256 tile.
 #include <cuda.h>
 
@@ -1548,7 +1548,7 @@ long long up256(long long bytes) { return (bytes + 255) / 256 * 256; }
 constexpr long long FEW_TOKENS = 128;
 
 // A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size. A training step of
-// 8192 x 4096 x 131072 without kept logits, with pieces of 256 MiB 29.0 ms, 512 28.6, 1 GiB 28.8, 2 GiB (one piece) 30.1.
+// 8192 x 4096 x 131072 without kept logits, with pieces of 256 MiB 29.4 ms, 512 29.6, 1 GiB 30.1, 2 GiB (one piece) 31.5.
 constexpr long long PIECE_BYTES = 512ll << 20;
 long long piece_words(long long tokens, long long vocab) {
   long long most = PIECE_BYTES / (2 * tokens) / TILE * TILE;
@@ -1558,8 +1558,8 @@ long long piece_words(long long tokens, long long vocab) {
 }
 
 // The words whose codes a forward leaves: as many pieces as KEEP_BYTES hold (a fortieth of the GPU's memory), in whole tiles.
-// Kept against computed again: 4096 x 1024 x 32000 743 and 878 us, 16384 x 2048 x 131072 (all of it) 24.0 and 28.7 ms, twice the
-// tokens (half of it) 53.9 and 61.8, 131072 x 512 x 65536 (a quarter of it) 44.9 and 45.9. The few-token kernel
+// Kept against computed again: 4096 x 1024 x 32000 779 and 966 us, 16384 x 2048 x 131072 (all of it) 25.4 and 30.7 ms, twice the
+// tokens (half of it) 57.9 and 62.3, 131072 x 512 x 65536 (a quarter of it) 49.8 and 50.9. The few-token kernel
 // keeps none: with so few rows the logits cost one pass over the weight.
 constexpr long long KEEP_BYTES = 4ll << 30;
 long long kept_words(long long tokens, long long vocab) {
