@@ -17,6 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import kernels
 from ._precision import preserve_fp32_parameters
+from ._rows import refuse_tangents
 
 _SCORING = ("sqrtsoftplus", "softmax", "sigmoid")
 
@@ -193,6 +194,7 @@ class MegaGate(torch.nn.Module):
 
     def forward(self, hidden_states: torch.Tensor, image_mask: torch.Tensor | None = None):
         """Returns (logits [T,E] fp32, routing_weights [T,K] fp32, expert_indices [T,K] int64)."""
+        refuse_tangents("MegaGate", hidden_states, self.weight)
         if image_mask is not None and self.bias_vl is None:
             raise ValueError("image_mask requires vision_enabled=True when constructing MegaGate")
         if image_mask is not None and image_mask.shape != hidden_states.shape[:2]:

@@ -16,6 +16,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import kernels
 from ._precision import preserve_fp32_parameters
+from ._rows import refuse_tangents
 
 MHC_STREAMS = 4
 MHC_MAPPINGS = MHC_STREAMS * MHC_STREAMS + 2 * MHC_STREAMS
@@ -179,6 +180,7 @@ def hyper_mega_mhc(previous_output, residual, previous_pre_mix, previous_post_mi
     """Run the fused shifted boundary with its matching autograd backward."""
     inputs = (previous_output, residual, previous_pre_mix, previous_post_mix, previous_residual_mix, phi, alpha,
               bias, norm_weight)
+    refuse_tangents("MegaMhc", *inputs)
     validate_mega_mhc_inputs(*inputs, num_iters, token_tile)
     if need_backward and torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
         return _HyperMegaMhcFunction.apply(*inputs, hc_eps, norm_eps, num_iters, token_tile)

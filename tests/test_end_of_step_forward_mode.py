@@ -1,10 +1,11 @@
-"""CPU: the row norms and the cross entropy refuse forward-mode derivatives instead of dropping them."""
+"""CPU: the modules refuse forward-mode derivatives instead of dropping them."""
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from hyper_multicore_b200 import MegaCrossEntropy, MegaRmsNorm, mega_cross_entropy, mega_layer_norm, mega_rms_norm
+from hyper_multicore_b200 import (MegaCrossEntropy, MegaGate, MegaRmsNorm, hyper_mega_mhc, mega_cross_entropy, mega_layer_norm,
+                                  mega_rms_norm)
 
 CALLS = {
     "layer norm": (lambda x, w, b: mega_layer_norm(x, w, b), [(3, 8), (8,), (8,)]),
@@ -28,3 +29,27 @@ def test_tangents_are_refused(name, which, requires_grad):
             call(*tensors)
         with pytest.raises(TypeError, match="CUDA"):  # the others have no tangent: the next refusal
             call(*(forward_ad.unpack_dual(t).primal for t in tensors))
+
+
+@pytest.mark.parametrize("which", range(2))
+def test_tangents_of_the_gate_are_refused(which):
+    gate = MegaGate(hidden_size=64, num_experts=8, top_k=2, scoring_func="softmax", routed_scaling_factor=1.0)
+    hidden = torch.randn(1, 4, 64).bfloat16()
+    with forward_ad.dual_level():
+        if which == 0:
+            hidden = forward_ad.make_dual(hidden, torch.ones_like(hidden))
+        else:
+            weight = gate.weight.detach()
+            del gate.weight
+            gate.weight = forward_ad.make_dual(weight, torch.ones_like(weight))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            gate(hidden)
+
+
+@pytest.mark.parametrize("which", range(9))
+def test_tangents_of_the_mhc_boundary_are_refused(which):
+    tensors = [torch.randn(4, 8) for _ in range(9)]
+    with forward_ad.dual_level():
+        tensors[which] = forward_ad.make_dual(tensors[which], torch.ones(4, 8))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            hyper_mega_mhc(*tensors)
