@@ -17,18 +17,17 @@
 // target's row enters with minus that sum, and the whole is scaled by what the sum should be (1 - p_t(i)) over what it is. An error
 // that all entries share, or that of one word which holds nearly all of the rest, then cancels too; left is
 // 2 * 2^-8 sum_j p_ij |w_j - w_c| at most, c the likeliest wrong word. (Rows of 256 over 1000 words with a common component of ten times
-// their own size: up to 1.8 % of a row's norm without this, its own rounding of 0.2 % with it.) A row of dw likewise: in the product a
-// word's entries are scaled to the sum over the tokens of |g_i| p_ij that they had before they were rounded, so that nothing is left
-// of the rounding where one token holds the word, or where all tokens rate it alike and what they have in common nearly cancels
-// against the tokens of the word (0.2 % of a row's norm there, 0.66 % without). What the scaling puts right as a whole it may take from the lesser
-// entries: one that is not the largest of its row or word may be off by twice 2^-8.
-// A training step of 8192 x 4096 x 131072 takes 23.5 ms with all its logits kept (2 GiB of 16-bit codes) and 29.6 ms with none,
-// 512 x 1024 x 32000 201 against 228 us (two inputs in turn). Gradients taken in the forward pass would hold the weight's gradient in FP32 until the
+// their own size: up to 1.8 % of a row's norm without this, its own rounding of 0.2 % with it. What the
+// scaling puts right as a whole it may take from the lesser entries: one that is not the largest may be off by twice 2^-8.) A row of dw is not
+// scaled: it is off by 2^-8 sum_i g_i p_ij |x_i| at most, each entry by its own rounding and no more; that does not average out where one
+// token holds a word or all tokens rate it alike (0.66 % of a row's norm where what they have in common nearly cancels).
+// A training step of 8192 x 4096 x 131072 takes 23.0 ms with all its logits kept (2 GiB of 16-bit codes) and 28.7 ms with none,
+// 512 x 1024 x 32000 186 against 207 us (two inputs in turn). Gradients taken in the forward pass would hold the weight's gradient in FP32 until the
 // backward one and only fit a loss that is reduced.
 //
 // The GEMM: CTA pairs (tcgen05.mma.cta_group::2, M = N = 256), one TMA producer, one issuer, eight epilogue warps, two
 // accumulators; the layouts of the operands are those of the grouped GEMMs. Bound by the tensor cores: 4096 x 32768 x 4096 takes
-// 750 to 785 us in its four forms (1400 to 1466 TFLOP/s, 0.86 to 0.90 of cuBLAS in a burst, tensor pipe 77 to 87 % busy); over seconds the
+// 750 to 785 us in its four forms (1400 to 1466 TFLOP/s, 0.86 to 0.90 of cuBLAS in a burst, tensor pipe 78 to 87 % busy); over seconds the
 // power limit leaves 1250 to 1330 (cuBLAS: 1380). Short k (1024 and below) is bound by L2: 1 MB per 256 x 256 tile.
 #include <cuda.h>
 
@@ -86,9 +85,6 @@ struct Params {
   float* tops;         // STATS: [kept / HALF][pitch] what the codes count from
   int first_word;       // PROBS, GRAD_*: first word of the piece
   float* row_sums;      // PROBS: [2 * n_tiles][pitch] sums of what is stored
-  uint32_t* word_parts;  // PROBS: [groups of GROUP rows][words_pitch], see word_part
-  long long words_pitch;
-  const float* word_factors;  // GRAD_WEIGHT: [m] what a word's entries are scaled by
   const float* others;  // GRAD_HIDDEN: [rows] sum of a packed row's stored entries over all pieces
   const int* row_of;    // GRAD_HIDDEN: token of a packed row
   float* sums;          // GRAD_HIDDEN: [rows, n] FP32 sums over pieces, or NULL
@@ -300,51 +296,28 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, const float* sums, 
   for (int j = 0; j < 64; ++j) v[j] = sums[c + j];
 }
 
-// The reduction over a warp's lanes of each of C columns (halving: a lane hands half of its columns to its partner and
-// takes the partner's values of the other half); column lane * (C / 32) + i ends in out[i].
-template <int C, bool MAX>
-__device__ __forceinline__ void reduce_columns(const float (&v)[C], float (&out)[C / 32], int lane) {
-  float w[C];
-#pragma unroll
-  for (int i = 0; i < C; ++i) w[i] = v[i];
-#pragma unroll
-  for (int s = 0; s < 5; ++s) {
-    const int half = C >> (s + 1);
-    const bool upper = (lane & (16 >> s)) != 0;
-#pragma unroll
-    for (int i = 0; i < half; ++i) {
-      const float keep = upper ? w[i + half] : w[i], send = upper ? w[i] : w[i + half];
-      const float other = __shfl_xor_sync(0xffffffffu, send, 16 >> s);
-      w[i] = MAX ? fmaxf(keep, other) : keep + other;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < C / 32; ++i) out[i] = w[i];
+// Eight values as BF16; their sum as rounded.
+__device__ __forceinline__ uint4 pack_8(const float* v, float2& sum) {
+  const uint4 q = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  sum = add2(sum, add2(add2(unpack_bf16x2(q.x), unpack_bf16x2(q.y)), add2(unpack_bf16x2(q.z), unpack_bf16x2(q.w))));
+  return q;
 }
 
-// Entries of a word over a group of packed rows, without the gradient's sign: what they add up to as stored, and what their rounding took
-// away. Both in BF16: the second is 2^-8 of the first at most, so 2^-16 of the sum is lost.
-constexpr int GROUP = 32;       // rows of a group
-constexpr int SMALL_GROUP = 8;  // where so few rows make a launch too short (spread_kernel)
-__device__ __forceinline__ uint32_t word_part(float whole, float stored) { return pack_bf16x2(stored, whole - stored); }
-
-// p of one row's 128 columns times the row's gradient, the target's entry left out; sums of what is stored, by rows and by words.
+// p of one row's 128 columns times the row's gradient, the target's entry left out, and the sum of what is stored.
 __device__ __forceinline__ void epilogue_probs(const Params& p, const CUtensorMap* tm, uint32_t taddr, uint8_t* stage,
                                                unsigned& issued, int first_row, int row, bool row_ok, int col, int half_tile,
                                                int lane) {
   float2 sum = both(0.0f);
   const float lse = row_ok ? p.lse[row] : 0.0f;
-  const float weight = row_ok ? p.weights[row] : 0.0f, size = fabsf(weight);
-  const uint32_t sign = __float_as_uint(weight) & 0x80000000u, signs = sign | sign >> 16;
+  const float weight = row_ok ? p.weights[row] : 0.0f;
   const int label = row_ok ? p.labels[row] - p.first_word - col : -1;
-  uint32_t* word_parts = p.word_parts + first_row / GROUP * p.words_pitch + col + lane;
 #pragma unroll 1
   for (int c = 0; c < HALF; c += 64) {
     if (col + c >= p.n) break;
     float v[64];
     load_columns(taddr + c, v);
 #pragma unroll
-    for (int j = 0; j < 64; ++j) v[j] = row_ok ? shifted_exp(v[j], lse) * size : 0.0f;
+    for (int j = 0; j < 64; ++j) v[j] = row_ok ? shifted_exp(v[j], lse) * weight : 0.0f;
     const int own = label - c;
     if (own >= 0 && own < 64) {
 #pragma unroll
@@ -360,26 +333,13 @@ __device__ __forceinline__ void epilogue_probs(const Params& p, const CUtensorMa
 #pragma unroll
     for (int h = 0; h < 64; h += 32) {
       if (col + c + h >= p.n) break;
-      uint32_t q[16];
-      float stored[32], whole[32], of_whole[1], of_stored[1];
+      uint4 q[4];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        q[i] = pack_bf16x2(v[h + 2 * i], v[h + 2 * i + 1]);
-        const float2 f = unpack_bf16x2(q[i]);
-        sum = add2(sum, f);
-        stored[2 * i] = f.x, stored[2 * i + 1] = f.y;
-        whole[2 * i] = v[h + 2 * i], whole[2 * i + 1] = v[h + 2 * i + 1];
-        q[i] ^= signs;
-      }
-      const uint4 box[4] = {make_uint4(q[0], q[1], q[2], q[3]), make_uint4(q[4], q[5], q[6], q[7]),
-                            make_uint4(q[8], q[9], q[10], q[11]), make_uint4(q[12], q[13], q[14], q[15])};
-      store_box(tm, stage, issued, box, col + c + h, first_row, lane);
-      reduce_columns<32, false>(whole, of_whole, lane);
-      reduce_columns<32, false>(stored, of_stored, lane);
-      if (first_row < p.m) word_parts[c + h] = word_part(of_whole[0], of_stored[0]);
+      for (int i = 0; i < 4; ++i) q[i] = pack_8(v + h + 8 * i, sum);
+      store_box(tm, stage, issued, q, col + c + h, first_row, lane);
     }
   }
-  if (row_ok) p.row_sums[half_tile * p.pitch + row] = __uint_as_float(__float_as_uint(sum.x + sum.y) ^ sign);
+  if (row_ok) p.row_sums[half_tile * p.pitch + row] = sum.x + sum.y;
 }
 
 // With the last piece: what a row of dx takes the target's row times, and what the whole is scaled by.
@@ -485,7 +445,6 @@ __device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUte
                                                      bool empty, float filler) {
   const float scale = has_failed(p.failed, p.status) ? not_a_number() : *p.scale;
   const int slot = row_ok ? p.slots[p.first_word + row] : -1;
-  const float factor = row_ok ? p.word_factors[row] : 0.0f;
   const float* more = p.word_sums + static_cast<long long>(slot >= 0 ? slot : 0) * p.n + col;
 #pragma unroll 1
   for (int c = 0; c < HALF; c += 64) {
@@ -496,8 +455,6 @@ __device__ __forceinline__ void epilogue_grad_weight(const Params& p, const CUte
       for (int j = 0; j < 64; ++j) v[j] = filler;
     } else {
       load_columns(taddr, sums, c, v);
-#pragma unroll
-      for (int j = 0; j < 64; ++j) v[j] *= factor;
       if (slot >= 0) {
 #pragma unroll
         for (int j = 0; j < 64; j += 4)
@@ -787,6 +744,28 @@ struct Few {
   static constexpr int COLS = N * 4 / WARPS;                   // columns per warp
   static constexpr int THREADS = 64 + 32 * WARPS;
 };
+
+// The reduction over a warp's lanes of each of C columns (halving: a lane hands half of its columns to its partner and
+// takes the partner's values of the other half); column lane * (C / 32) + i ends in out[i].
+template <int C, bool MAX>
+__device__ __forceinline__ void reduce_columns(const float (&v)[C], float (&out)[C / 32], int lane) {
+  float w[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) w[i] = v[i];
+#pragma unroll
+  for (int s = 0; s < 5; ++s) {
+    const int half = C >> (s + 1);
+    const bool upper = (lane & (16 >> s)) != 0;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float keep = upper ? w[i + half] : w[i], send = upper ? w[i] : w[i + half];
+      const float other = __shfl_xor_sync(0xffffffffu, send, 16 >> s);
+      w[i] = MAX ? fmaxf(keep, other) : keep + other;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C / 32; ++i) out[i] = w[i];
+}
 
 template <int N>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Few<N>::THREADS, 1)
@@ -1232,125 +1211,76 @@ __device__ __forceinline__ float power_of(uint32_t pair, uint32_t half, float ab
   return r;
 }
 
-// p of a piece of the vocabulary out of its codes, times the row's gradient, and the sums of what is stored: what PROBS computes from the
-// logits. A warp per group of rows and 256 words, four rows at a time; rows behind the last one that the products read with it are
-// zero. Bound by instructions: 4096 x 65536 217 us (1.07 GB, 4.9 TB/s; 178 us without the words' sums), where the product takes 1500.
-constexpr int SPREAD_WARPS = 8;
-constexpr int SPREAD_WORDS = 256;  // of a warp
-constexpr int SPREAD_ROWS = 4;     // under way together
-__global__ void __launch_bounds__(32 * SPREAD_WARPS, 3)
-spread_kernel(const uint16_t* __restrict__ codes, long long codes_pitch, const float* __restrict__ tops, long long tops_pitch,
-              int first_word, int width, const int* __restrict__ count, const float* __restrict__ lse, const float* __restrict__ weights,
-              long long tokens, __nv_bfloat16* __restrict__ probs, long long probs_pitch, float* __restrict__ row_sums,
-              uint32_t* __restrict__ word_parts, int group) {
+// p of a piece of the vocabulary out of its codes, times the row's gradient: what PROBS computes from the logits. A warp per row
+// and 1024 words, eight rows per block, and the sum of what it stores; rows behind the last one that the products read with it are
+// zero. Bound by memory, nearly by its instructions: 4096 x 65536 178 us (1.07 GB, 6.0 TB/s) where the product takes 1500; 2101 x 50257 78 us.
+constexpr int SPREAD_WORDS = 1024;
+__global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict__ codes, long long codes_pitch,
+                                                     const float* __restrict__ tops, long long tops_pitch, int first_word, int width,
+                                                     const int* __restrict__ count, const float* __restrict__ lse,
+                                                     const float* __restrict__ weights, long long tokens,
+                                                     __nv_bfloat16* __restrict__ probs, long long probs_pitch,
+                                                     float* __restrict__ row_sums) {
   chain_wait();
   chain_next();
-  const int rows = *count, lane = threadIdx.x & 31;
-  const long long end = min(static_cast<long long>((rows + TILE - 1) / TILE) * TILE, tokens);
-  const int part = blockIdx.y * SPREAD_WARPS + (threadIdx.x >> 5), col = part * SPREAD_WORDS + lane * 8;
-  if (part * SPREAD_WORDS >= width) return;
-  const long long first_row = static_cast<long long>(blockIdx.x) * group;
-  float2 whole[4], stored[4];  // over the rows, without the gradient's sign
+  const int rows = *count;
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= (rows + TILE - 1) / TILE * TILE || row >= tokens) return;
+  const int col = blockIdx.y * SPREAD_WORDS + (threadIdx.x & 31) * 8;
+  const bool row_ok = row < rows;
+  const float norm = row_ok ? lse[row] : 0.0f, weight = row_ok ? weights[row] : 0.0f;
+  const uint16_t* src = codes + row * codes_pitch + first_word + col;
+  __nv_bfloat16* dst = probs + row * probs_pitch + col;
+  uint4 q[SPREAD_WORDS / 256];
+  float from[SPREAD_WORDS / 256];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) whole[i] = stored[i] = both(0.0f);
-  for (int at = 0; at < group; at += SPREAD_ROWS) {
-    const long long row = first_row + at;
-    if (row >= end) break;
-    const uint16_t* src = codes + row * codes_pitch + first_word + col;
-    const float* top = tops + (first_word + col) / HALF * tops_pitch + row;
-    __nv_bfloat16* dst = probs + row * probs_pitch + col;
-    uint4 q[SPREAD_ROWS];
-    float above[SPREAD_ROWS], weight[SPREAD_ROWS], sums[SPREAD_ROWS];
-#pragma unroll
-    for (int r = 0; r < SPREAD_ROWS; ++r) {
-      if (row + r >= rows) continue;
-      q[r] = ld_16(src + r * codes_pitch);
-      above[r] = (top[r] - lse[row + r]) * LOG2_E;
-      weight[r] = weights[row + r];
-    }
-#pragma unroll
-    for (int r = 0; r < SPREAD_ROWS; ++r) {
-      sums[r] = 0.0f;
-      if (row + r >= end) continue;
-      uint4 out = make_uint4(0, 0, 0, 0);
-      if (row + r < rows) {
-        const float size = fabsf(weight[r]);
-        const uint32_t sign = __float_as_uint(weight[r]) & 0x80000000u, signs = sign | sign >> 16;
-        float2 sum = both(0.0f);
-        auto two = [&](uint32_t pair, int i) {
-          const float2 v = times2(make_float2(power_of(pair, 0x7610, above[r]), power_of(pair, 0x7632, above[r])), both(size));
-          const uint32_t word = pack_bf16x2(v.x, v.y);
-          const float2 f = unpack_bf16x2(word);
-          whole[i] = add2(whole[i], v), stored[i] = add2(stored[i], f), sum = add2(sum, f);
-          return word ^ signs;
-        };
-        out = make_uint4(two(q[r].x, 0), two(q[r].y, 1), two(q[r].z, 2), two(q[r].w, 3));
-        sums[r] = __uint_as_float(__float_as_uint(sum.x + sum.y) ^ sign);
-      }
-      st_16(dst + r * probs_pitch, out);
-    }
-    // the rows' sums over the lanes by halving: row r ends in the lanes from 32 / SPREAD_ROWS * r on
-    int lanes = 32;
-#pragma unroll
-    for (int half = SPREAD_ROWS / 2; half > 0; half /= 2) {
-      lanes /= 2;
-      const bool upper = (lane & lanes) != 0;
-#pragma unroll
-      for (int i = 0; i < half; ++i) {
-        const float keep = upper ? sums[i + half] : sums[i], send = upper ? sums[i] : sums[i + half];
-        sums[i] = keep + __shfl_xor_sync(0xffffffffu, send, lanes);
-      }
-    }
-#pragma unroll
-    for (int o = 16 / SPREAD_ROWS; o > 0; o >>= 1) sums[0] += __shfl_xor_sync(0xffffffffu, sums[0], o);
-    const long long mine = row + lane / (32 / SPREAD_ROWS);
-    if (lane % (32 / SPREAD_ROWS) == 0 && mine < rows) row_sums[part * tops_pitch + mine] = sums[0];
+  for (int i = 0; i < SPREAD_WORDS / 256; ++i) {
+    if (!row_ok || col + 256 * i >= width) continue;
+    q[i] = ld_16(src + 256 * i);
+    from[i] = tops[(first_word + col + 256 * i) / HALF * tops_pitch + row];
   }
-  if (first_row >= rows) return;
-  uint4 out[2];
-  uint32_t* words = reinterpret_cast<uint32_t*>(out);
+  float2 sum = both(0.0f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    words[2 * i] = word_part(whole[i].x, stored[i].x);
-    words[2 * i + 1] = word_part(whole[i].y, stored[i].y);
+  for (int i = 0; i < SPREAD_WORDS / 256; ++i) {
+    if (col + 256 * i >= width) break;
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (row_ok) {
+      const float above = (from[i] - norm) * LOG2_E;
+      auto two = [&](uint32_t pair) {
+        const uint32_t word = pack_bf16x2(power_of(pair, 0x7610, above) * weight, power_of(pair, 0x7632, above) * weight);
+        sum = add2(sum, unpack_bf16x2(word));
+        return word;
+      };
+      out = make_uint4(two(q[i].x), two(q[i].y), two(q[i].z), two(q[i].w));
+    }
+    st_16(dst + 256 * i, out);
   }
-  uint32_t* to = word_parts + static_cast<long long>(blockIdx.x) * probs_pitch + col;
-  st_16(to, out[0]);
-  st_16(to + 4, out[1]);
+  const float all = warp_sum(sum.x + sum.y);
+  if (row_ok && (threadIdx.x & 31) == 0) row_sums[blockIdx.y * tops_pitch + row] = all;
 }
 
-// A piece's sums. The first `row_blocks` blocks take 32 packed rows each: what is stored of a row, on top of earlier pieces, its parts in
-// 32 slices at a time and those in their order; the others 128 words each and 8 slices: what the entries of a word are scaled by in the
-// product. Bound by latency.
-constexpr int SUM_WORDS = 128;
-__global__ void __launch_bounds__(32 * JOIN_SLICES) piece_sums_kernel(const float* __restrict__ row_sums, long long pitch, int row_parts,
-                                                                      int row_blocks, const int* __restrict__ count, int add,
-                                                                      float* __restrict__ others, const uint32_t* __restrict__ word_parts,
-                                                                      long long words_pitch, int words, int group, float* __restrict__ word_factors) {
-  __shared__ float2 sums[32 * JOIN_SLICES];
+// Sums of a packed row's stored entries: this piece's parts in their order, 32 slices of them in parallel, on top of those of
+// earlier pieces. Bound by latency.
+__global__ void __launch_bounds__(32 * JOIN_SLICES) row_sums_kernel(const float* __restrict__ row_sums, long long pitch, int parts,
+                                                                    const int* __restrict__ count, int add,
+                                                                    float* __restrict__ others) {
+  __shared__ float sums[JOIN_SLICES][33];
   chain_wait();
   chain_next();
-  const bool by_row = static_cast<int>(blockIdx.x) < row_blocks;
-  const int width = by_row ? 32 : SUM_WORDS, slices = 32 * JOIN_SLICES / width;
-  const int rows = *count, x = threadIdx.x % width, slice = threadIdx.x / width;
-  const int at = (by_row ? blockIdx.x : blockIdx.x - row_blocks) * width + x;
-  const bool ok = at < (by_row ? rows : words);
-  float2 sum = both(0.0f);
-  if (ok && by_row) {
+  const int row = blockIdx.x * 32 + threadIdx.x;
+  const bool ok = row < *count;
+  float sum = 0.0f;
+  if (ok) {
 #pragma unroll 8
-    for (int i = slice; i < row_parts; i += slices) sum.x += row_sums[i * pitch + at];
-  } else if (ok) {
-    const int parts = (rows + group - 1) / group;
-#pragma unroll 8
-    for (int i = slice; i < parts; i += slices) sum = add2(sum, unpack_bf16x2(word_parts[i * words_pitch + at]));
+    for (int i = threadIdx.y; i < parts; i += JOIN_SLICES) sum += row_sums[i * pitch + row];
   }
-  sums[threadIdx.x] = sum;
+  sums[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
-  if (slice != 0 || !ok) return;
+  if (threadIdx.y != 0 || !ok) return;
+  sum = add ? others[row] : 0.0f;
 #pragma unroll 8
-  for (int s = 1; s < slices; ++s) sum = add2(sum, sums[s * width + x]);
-  if (by_row) others[at] = add ? others[at] + sum.x : sum.x;
-  else word_factors[at] = sum.x > 0.0f ? 1.0f + sum.y / sum.x : 1.0f;
+  for (int s = 0; s < JOIN_SLICES; ++s) sum += sums[s][threadIdx.x];
+  others[row] = sum;
 }
 
 // The sum of coef_i x_i over the rows that have a word as target, in their order, in slices of WORD_SLICE rows of a word:
@@ -1548,7 +1478,7 @@ long long up256(long long bytes) { return (bytes + 255) / 256 * 256; }
 constexpr long long FEW_TOKENS = 128;
 
 // A piece of the vocabulary: what T rows of BF16 probabilities may take, in whole tiles, pieces of equal size. A training step of
-// 8192 x 4096 x 131072 without kept logits, with pieces of 256 MiB 29.4 ms, 512 29.6, 1 GiB 30.1, 2 GiB (one piece) 31.5.
+// 8192 x 4096 x 131072 without kept logits, with pieces of 256 MiB 29.0 ms, 512 28.6, 1 GiB 28.8, 2 GiB (one piece) 30.1.
 constexpr long long PIECE_BYTES = 512ll << 20;
 long long piece_words(long long tokens, long long vocab) {
   long long most = PIECE_BYTES / (2 * tokens) / TILE * TILE;
@@ -1558,8 +1488,8 @@ long long piece_words(long long tokens, long long vocab) {
 }
 
 // The words whose codes a forward leaves: as many pieces as KEEP_BYTES hold (a fortieth of the GPU's memory), in whole tiles.
-// Kept against computed again: 4096 x 1024 x 32000 779 and 966 us, 16384 x 2048 x 131072 (all of it) 25.4 and 30.7 ms, twice the
-// tokens (half of it) 57.9 and 62.3, 131072 x 512 x 65536 (a quarter of it) 49.8 and 50.9. The few-token kernel
+// Kept against computed again: 4096 x 1024 x 32000 760 and 970 us, 16384 x 2048 x 131072 (all of it) 24.1 and 29.3 ms, twice the
+// tokens (half of it) 56.0 and 61.6, 131072 x 512 x 65536 (a quarter of it) 46.9 and 47.9. The few-token kernel
 // keeps none: with so few rows the logits cost one pass over the weight.
 constexpr long long KEEP_BYTES = 4ll << 30;
 long long kept_words(long long tokens, long long vocab) {
@@ -1614,17 +1544,9 @@ int launch_few(const CUtensorMap& words, const State& st, long long hidden, long
                         (p.k + BK - 1) / BK, p.count, p.labels, p.partial, p.pitch, p.failed, p.status);
 }
 
-// Rows of a group of word sums: fewer where whole groups would leave SMs without blocks of the pass over the codes (a step of 512 x
-// 1024 x 32000 takes 179 us with 8 rows, 183 with 32; of 1000 x 1024 x 50257, where whole groups fill the SMs, 383 and 377).
-int group_rows(long long tokens, long long words) {
-  const long long blocks = (tokens + GROUP - 1) / GROUP * ((words + SPREAD_WARPS * SPREAD_WORDS - 1) / (SPREAD_WARPS * SPREAD_WORDS));
-  return tokens > FEW_TOKENS && blocks < 3 * sm_count() ? SMALL_GROUP : GROUP;
-}
-
 struct GradSpace {
-  float *scale, *weights, *coef, *word_sums, *sums, *part_sums, *row_sums, *others, *word_factors;
+  float *scale, *weights, *coef, *word_sums, *sums, *part_sums, *row_sums, *others;
   unsigned* slots;
-  uint32_t* word_parts;
   int *members, *failed;
   __nv_bfloat16* probs;
   long long slot_bytes, bytes, piece;
@@ -1648,8 +1570,6 @@ struct GradSpace {
     part_sums = reinterpret_cast<float*>(take(2ll * (sm_count() / 2) * TILE * TILE * 4));
     row_sums = reinterpret_cast<float*>(take(4 * tokens * (piece / HALF)));
     others = reinterpret_cast<float*>(take(4 * tokens));
-    word_parts = reinterpret_cast<uint32_t*>(take(4 * ((tokens + group_rows(tokens, piece) - 1) / group_rows(tokens, piece)) * piece));
-    word_factors = reinterpret_cast<float*>(take(4 * piece));
     probs = reinterpret_cast<__nv_bfloat16*>(take(2 * tokens * piece));
     bytes = at;
   }
@@ -1786,15 +1706,13 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
     p.first_word = static_cast<int>(first);
     p.n = static_cast<int>(words), p.k = width;
     p.row_sums = w.row_sums, p.pitch = tokens;
-    p.word_parts = w.word_parts, p.words_pitch = w.piece;
-    int parts, group = GROUP;  // sums that the probabilities of a row leave, rows to a word's
+    int parts;  // sums that the probabilities of a row leave
     if (first < st.kept) {
       const int whole = static_cast<int>(tiles_of(words) * TILE);
-      parts = whole / SPREAD_WORDS;
-      group = group_rows(tokens, w.piece);
-      const dim3 grid(static_cast<unsigned>((tokens + group - 1) / group), (parts + SPREAD_WARPS - 1) / SPREAD_WARPS);
-      if (int rc = launch_chained(spread_kernel, grid, dim3(32 * SPREAD_WARPS), 0, s, st.codes, st.kept, st.tops, tokens, p.first_word, whole,
-                                  st.count, st.lse, w.weights, tokens, w.probs, w.piece, w.row_sums, w.word_parts, group))
+      parts = (whole + SPREAD_WORDS - 1) / SPREAD_WORDS;
+      if (int rc = launch_chained(spread_kernel, dim3(static_cast<unsigned>((tokens + 7) / 8), parts), dim3(256), 0, s, st.codes,
+                                  st.kept, st.tops, tokens, p.first_word, whole, st.count, st.lse, w.weights, tokens, w.probs, w.piece,
+                                  w.row_sums))
         return rc;
     } else {
       parts = static_cast<int>(2 * tiles_of(words));
@@ -1802,12 +1720,10 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
       if (int rc = map_store(&probs_store, w.probs, words, tokens, w.piece)) return rc;
       if (int rc = launch_product<PROBS>(rows_k, head_k, probs_store, p, tiles_of(tokens) * tiles_of(words), s)) return rc;
     }
-    const int row_blocks = grad_hidden != nullptr ? static_cast<int>((tokens + 31) / 32) : 0;
-    const int word_blocks = grad_weight != nullptr ? static_cast<int>((words + SUM_WORDS - 1) / SUM_WORDS) : 0;
-    if (int rc = launch_chained(piece_sums_kernel, dim3(row_blocks + word_blocks), dim3(32 * JOIN_SLICES), 0, s, w.row_sums, tokens, parts,
-                                row_blocks, st.count, first > 0, w.others, w.word_parts, w.piece, static_cast<int>(words), group, w.word_factors))
-      return rc;
     if (grad_hidden != nullptr) {
+      if (int rc = launch_chained(row_sums_kernel, dim3(static_cast<unsigned>((tokens + 31) / 32)), dim3(32, JOIN_SLICES), 0, s, w.row_sums,
+                                  tokens, parts, st.count, first > 0, w.others))
+        return rc;
       if (int rc = map_k_major(&probs_k, w.probs, words, tokens, w.piece)) return rc;
       if (int rc = map_mn_major(&head_mn, head, hidden, words, weight_stride)) return rc;
       p.n = width, p.k = static_cast<int>(words);
@@ -1828,7 +1744,6 @@ extern "C" int hmc_vocab_loss_grad(const void* state, const void* weight, int64_
       if (int rc = map_store(&grad_store, dst, hidden, words, hidden)) return rc;
       p.m = static_cast<int>(words), p.n = width;
       p.slots = reinterpret_cast<const int*>(w.slots), p.word_sums = w.word_sums;
-      p.word_factors = w.word_factors;
       if (int rc = launch_product<GRAD_WEIGHT>(probs_mn, rows_mn, grad_store, p, tiles_of(words) * tiles_of(width), s)) return rc;
     }
   }

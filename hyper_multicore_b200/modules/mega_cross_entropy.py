@@ -108,12 +108,11 @@ def mega_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torc
     tokens; the mean over none of them is NaN, as in torch. Ignored tokens are not read: whatever their hidden states hold,
     their gradient is zero and they add nothing to the weight's. A target outside [0, V) that is not ``ignore_index`` is not
     noticed on the host: its loss is NaN, and so are the gradients it enters. Differentiable once, in reverse, in ``hidden`` and ``weight``;
-    the gradients are BF16, and so are the probabilities that enter them, whose sums over the words of a token and over the tokens of a
-    word are FP32 and kept. What is held are the logits' distances from the largest of 128, of as many words as fit 4 GiB (none up to 128
-    tokens); the others are computed again, with ``recompute`` all of them, which takes a quarter longer. Every call whose graph lives
-    holds its own. The backward pass takes scratch of up to 512 MiB for probabilities (4096 words of them where that is
-    more) and a twelfth of that for their sums, 8 bytes per element of ``hidden`` and per word, and 50 MiB. A wait inside a kernel that gives up
-    makes the loss, or the gradients, NaN.
+    the gradients are BF16, and so are the probabilities that enter them; a token's keep their sum. What is held are the logits'
+    distances from the largest of 128, of as many words as fit 4 GiB (none up to 128 tokens); the others are computed again, with
+    ``recompute`` all of them, which takes a quarter longer. Every call whose graph lives holds its own. The backward pass takes
+    scratch of up to 512 MiB for probabilities (4096 words of them where that is more) and a 64th of that for their sums, 8 bytes per
+    element of ``hidden`` and per word, and 40 MiB. A wait inside a kernel that gives up makes the loss, or the gradients, NaN.
     """
     if recompute is not False and recompute is not True:
         raise ValueError(f"recompute must be a bool, got {recompute!r}.")
